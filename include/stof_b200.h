@@ -29,6 +29,9 @@ extern "C" {
 
 #define STOF_DTYPE_F16 0
 #define STOF_DTYPE_F32 1
+#define STOF_DTYPE_BF16 2
+#define STOF_DTYPE_INT8 3      /* entries of a key/value cache, value = entry * scale */
+#define STOF_DTYPE_E4M3 4      /* likewise, entries in fp8 e4m3 (no infinities) */
 
 /* Library version (major*100 + minor) and the last error text of the calling thread. */
 int stof_version(void);
@@ -239,6 +242,109 @@ int stof_gemm_bias_residual_layernorm(const void* a, long long lda, const void* 
 int stof_bias_residual_layernorm(const void* x, long long ldx, const void* bias, const void* residual, long long ldr,
                                  const void* gamma, const void* beta, float eps, void* y, long long ldy,
                                  int rows, int hidden, int* status_dev, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Attention with scores changed by a formula and masked by rules.  No counterpart in the reference, whose kernels take
+ * their mask as an array (src/ops/src/block_attn_mask.cpp:17-49) and add nothing to the scores.
+ *
+ * q (batch, heads, q_len, head_dim), k and v (batch, kv_heads, k_len, head_dim), out like q; fp16 or bf16
+ * (STOF_DTYPE_F16 / STOF_DTYPE_BF16), fp32 accumulation, head_dim 64 or 128; heads a multiple of kv_heads, query head h reads
+ * K/V head h / (heads / kv_heads).  Query i sits at position i + k_len - q_len among the keys.  With
+ *   x = softmax_scale * (q . k);  softcap > 0: x = softcap * tanh(x / softcap);
+ *   slopes (heads): x -= slopes[h] * |position - j|;
+ *   distance_bias (heads, 2 * bias_radius + 1): x += distance_bias[h][bias_radius + clamp(j - position, -radius, radius)];
+ * key j is visible to the query if
+ *   j < key_lens[b] (where given), documents[b][j] == documents[b][position] (where given), and
+ *   j < prefix_lens[b] (where given), or (not causal or j <= position) and (window == 0 or |position - j| < window).
+ * out = softmax over the visible keys, times v; a query without any gives zeros.  What K and V hold at or behind
+ * key_lens[b] takes no part, NaN included; a NaN or an infinity in V before it reaches every query whose 128-key tile
+ * holds it.
+ * Pointers 16-byte aligned, strides (batch, head, row; the last dimension is contiguous) positive multiples of 8 elements.
+ * slopes and distance_bias fp32, bias_radius at most STOF_SCORED_MAX_RADIUS; documents int32 (batch, k_len) with row stride
+ * `documents_stride`, at most STOF_SCORED_MAX_DOC_KEYS keys and q_len <= k_len; prefix_lens, key_lens int32 (batch).
+ * `out` must not overlap the inputs.
+ * ------------------------------------------------------------------------------------------ */
+#define STOF_SCORED_MAX_RADIUS 2048
+#define STOF_SCORED_MAX_DOC_KEYS 131072
+
+typedef struct stof_score_rules {
+    float softmax_scale;
+    float softcap;                 /* 0: none */
+    int causal;
+    int window;                    /* 0: none */
+    const float* slopes;           /* the pointers may be NULL */
+    const float* distance_bias;
+    int bias_radius;
+    const int* documents;
+    long long documents_stride;
+    const int* prefix_lens;
+    const int* key_lens;
+} stof_score_rules;
+
+int stof_scored_attn(const void* q, const void* k, const void* v, void* out, int dtype,
+                     int batch, int heads, int kv_heads, int q_len, int k_len, int head_dim,
+                     const long long q_strides[3], const long long k_strides[3],
+                     const long long v_strides[3], const long long out_strides[3],
+                     const stof_score_rules* rules, int* status_dev, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * The same attention for the last tokens of requests whose keys and values lie in a paged 8-bit cache.  No counterpart in the
+ * reference (it runs whole sequences only).
+ *
+ * Cache: k_pages, v_pages (pages, kv_heads, page_size, head_dim) of 8-bit entries (cache_dtype STOF_DTYPE_INT8 or _E4M3),
+ * contiguous; k_scales, v_scales (pages, kv_heads) fp32: an entry stands for entry * scale.  page_size 16, 32, 64 or 128,
+ * head_dim 64 or 128.  Key j of request b lies in page block_table[b][j / page_size], row j % page_size.
+ * q, out (requests, tokens, heads, head_dim), fp16 or bf16, strides (request, token, head) multiples of 8 elements: token t of
+ * request b sits at position lengths[b] - tokens + t; keys behind a token's position are not visible to it, nor, with
+ * window > 0, those window or more in front of it.  softcap, slopes, distance_bias as above (causal, documents, prefix_lens and
+ * key_lens of `rules` are not read).  lengths int32 (requests), counted to at most table_width * page_size; requests of length
+ * 0 give zeros.  A page number outside [0, pages) is reported through status_dev and its keys are left out.
+ * Work is dealt evenly over the GPU whatever the lengths; what a thread block computes of a request's head goes to `workspace`
+ * (stof_cache_attn_workspace_bytes bytes, 16-byte aligned, not shared with a call that may run at the same time) where it is not
+ * all of it, and a second kernel joins the parts in a fixed order.
+ * ------------------------------------------------------------------------------------------ */
+size_t stof_cache_attn_workspace_bytes(int requests, int tokens, int heads, int kv_heads, int head_dim, int page_size, int table_width);
+
+int stof_cache_attn(const void* q, void* out, int dtype, const long long q_strides[3], const long long out_strides[3],
+                    const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales, int cache_dtype,
+                    int pages, int page_size, int kv_heads, int head_dim,
+                    const int* block_table, long long table_stride, int table_width, const int* lengths,
+                    int requests, int tokens, int heads, const stof_score_rules* rules,
+                    void* workspace, size_t workspace_bytes, int* status_dev, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Writes new keys and values into such a cache.  No counterpart in the reference.
+ *
+ * k, v (tokens, kv_heads, head_dim) fp16 or bf16, strides (token, head) multiples of 8 elements; token t goes to slot
+ * slots[t] = page * page_size + row (negative: nowhere).  Tokens of consecutive slots inside one page are a run.  A run that
+ * begins its page sets the page's scale to its largest magnitude / 127 (int8) or / 448 (e4m3), per head, and what the page held
+ * counts no more; any other run keeps the larger of that and the scale that is there, and where the scale grows the
+ * entries in front of the run are rounded again to it.  entry = round(x * (1 / scale)), to nearest even; a scale below the
+ * smallest normal fp32 counts as 0.  A page may hold one run of a call only: two runs in the same page write it unordered.
+ * Slots at or behind pages * page_size are reported through status_dev and not written.
+ * ------------------------------------------------------------------------------------------ */
+int stof_cache_append(void* k_pages, void* v_pages, float* k_scales, float* v_scales, int cache_dtype,
+                      int pages, int page_size, int kv_heads, int head_dim,
+                      const void* k, const void* v, int dtype, const long long k_strides[2], const long long v_strides[2],
+                      const int* slots, int tokens, int* status_dev, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Block tables and slot maps from request lengths, with the pages kept on a stack.  No counterpart in the reference.
+ *
+ * Request r holds held[r] tokens in the first ceil(held / page_size) pages of its row of block_table (requests, table_width; row
+ * stride table_stride) and shall hold lengths[r].  Pages that are no longer needed are pushed on the stack (free_pages, of which
+ * the first *free_count are on it; free_capacity in all), request by request and front to back; then the pages that are needed
+ * are popped in the same order.  Outputs: the rows' new pages (entries behind a row's need stay as they are), `starts`
+ * (requests + 1): running count of new tokens max(0, lengths - held); slots[starts[r] + i] = slot of token held[r] + i of
+ * request r, -1 behind the last token; *free_count_out (may be free_count); *missing_out = 0.
+ * All or nothing: where the stack holds too few pages, or a row too few entries, *missing_out is the number of pages short, all
+ * slots are -1 and nothing else changes; where the pages given back do not fit the stack it is negative.
+ * Negative lengths count as 0; held is counted to at most table_width * page_size; starts and missing stop at 2^31 - 1.
+ * ------------------------------------------------------------------------------------------ */
+int stof_page_tables(const int* lengths, const int* held, int requests, int* block_table, long long table_stride, int table_width,
+                     int* free_pages, int free_capacity, const int* free_count, int page_size,
+                     int* slots, int slot_count, int* starts, int* free_count_out, int* missing_out,
+                     int* status_dev, void* stream);
 
 #ifdef __cplusplus
 }

@@ -76,6 +76,11 @@ struct Api {
     decltype(&stof_gemm_bias_act) gemm_bias_act;
     decltype(&stof_gemm_bias_residual_layernorm) gemm_ln;
     decltype(&stof_bias_residual_layernorm) layernorm;
+    decltype(&stof_scored_attn) scored_attn;
+    decltype(&stof_cache_attn_workspace_bytes) cache_attn_workspace_bytes;
+    decltype(&stof_cache_attn) cache_attn;
+    decltype(&stof_cache_append) cache_append;
+    decltype(&stof_page_tables) page_tables;
 } api = {};
 
 void check(int rc, const char* what) {
@@ -724,6 +729,324 @@ PyObject* py_stack(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// ------------------------------------------------------------------------------------------ attention by formula and rules, the 8-bit cache
+template <class F>
+void need_entry(F* f, const char* what) {
+    if (f == nullptr) fail("%s is not in the library that is loaded: build it with `python sc25-stof-ad_b200/build.py`", what);
+}
+
+// A tensor of a new operator: on the GPU, on the device of the first
+void need_same_device(const at::Tensor& first, const at::Tensor* t, const char* op) {
+    need_cuda(t);
+    if (t != nullptr && t->get_device() != first.get_device()) fail("%s: all tensors must be on one device", op);
+}
+
+int half_type(const at::Tensor& t, const char* op) {
+    if (t.scalar_type() == at::kHalf) return STOF_DTYPE_F16;
+    if (t.scalar_type() == at::kBFloat16) return STOF_DTYPE_BF16;
+    fail("%s: float16 or bfloat16 expected", op);
+}
+int entry_type(const at::Tensor& t, const char* op) {
+    if (t.scalar_type() == at::kChar) return STOF_DTYPE_INT8;
+    if (t.scalar_type() == at::kFloat8_e4m3fn) return STOF_DTYPE_E4M3;
+    fail("%s: cache pages must be int8 or float8_e4m3fn", op);
+}
+int as_int(int64_t v, const char* what) {
+    if (v < -0x7FFFFFFFll || v > 0x7FFFFFFFll) fail("%s beyond 32 bits", what);
+    return static_cast<int>(v);
+}
+
+// Can the kernels read it where it lies?  A contiguous last dimension, an address and strides that are multiples of 16 bytes, and no
+// stride 0 (an expanded dimension)
+bool in_place(const at::Tensor& t) {
+    const int64_t n = t.dim();
+    if (t.numel() == 0) return true;
+    if ((t.stride(n - 1) != 1 && t.size(n - 1) > 1) || (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) != 0) return false;
+    for (int64_t i = 0; i + 1 < n; ++i)
+        if (t.size(i) > 1 && (t.stride(i) <= 0 || t.stride(i) % 8 != 0)) return false;
+    return true;
+}
+at::Tensor readable(const at::Tensor& t) {
+    if (in_place(t)) return t;
+    const Released gil;
+    return t.contiguous().data_ptr() == t.data_ptr() ? t.clone(at::MemoryFormat::Contiguous) : t.contiguous();
+}
+// the first `n` strides; those of dimensions of size 1, which mean nothing, as if packed
+template <int N>
+void strides_of(const at::Tensor& t, long long (&st)[N]) {
+    long long packed_stride = 1;
+    for (int64_t i = t.dim() - 1; i >= 0; --i) {
+        if (i < N) st[i] = t.size(i) > 1 ? t.stride(i) : packed_stride;
+        packed_stride *= t.size(i) > 0 ? t.size(i) : 1;
+    }
+}
+// `t`, and whether two elements of it share memory cannot be told from outside in general: an output has to be in_place as it is
+void need_output(const at::Tensor& out, const at::Tensor& like, const char* op) {
+    if (out.sizes() != like.sizes() || out.scalar_type() != like.scalar_type()) fail("%s: out must have the shape and type of q", op);
+    if (!in_place(out)) fail("%s: out needs a contiguous last dimension and an address and strides that are multiples of 16 bytes", op);
+}
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+    if (a.numel() == 0 || b.numel() == 0) return false;
+    auto end = [](const at::Tensor& t) {
+        int64_t n = 1;
+        for (int64_t i = 0; i < t.dim(); ++i) n += (t.size(i) - 1) * t.stride(i);
+        return static_cast<const char*>(t.data_ptr()) + n * static_cast<int64_t>(t.element_size());
+    };
+    const char *a0 = static_cast<const char*>(a.data_ptr()), *b0 = static_cast<const char*>(b.data_ptr());
+    return a0 < end(b) && b0 < end(a);
+}
+
+// int32 vector of n elements; packed where it is strided
+const int* int_vector(const at::Tensor* t, int64_t n, const at::Tensor& first, at::Tensor& keep, const char* op, const char* name) {
+    if (t == nullptr) return nullptr;
+    need_same_device(first, t, op);
+    if (t->scalar_type() != at::kInt || t->dim() != 1 || t->size(0) != n) fail("%s: %s must be an int32 vector of %lld", op, name, static_cast<long long>(n));
+    keep = packed(*t);
+    return static_cast<const int*>(keep.data_ptr());
+}
+
+struct Rules {
+    stof_score_rules r = {};
+    at::Tensor keep[5];
+};
+// window, softcap, slopes, distance_bias, softmax_scale of either attention
+void score_args(Rules& x, PyObject* window, PyObject* softcap, const at::Tensor* slopes, const at::Tensor* bias, PyObject* scale, const at::Tensor& q,
+                int64_t heads, int64_t dim, const char* op) {
+    if (window != Py_None) {
+        const long w = long_arg(window);
+        if (w <= 0) fail("%s: window must be positive, got %ld", op, w);
+        x.r.window = static_cast<int>(std::min<long>(w, 0x3FFFFFFF));
+    }
+    if (softcap != Py_None) {
+        x.r.softcap = static_cast<float>(double_arg(softcap));
+        if (!(x.r.softcap > 0.f) || std::isinf(x.r.softcap)) fail("%s: softcap must be positive and finite", op);
+    }
+    x.r.softmax_scale = static_cast<float>(scale != Py_None ? double_arg(scale) : 1.0 / std::sqrt(static_cast<double>(dim)));
+    if (!(x.r.softmax_scale > 0.f) || std::isinf(x.r.softmax_scale)) fail("%s: softmax_scale must be positive and finite", op);
+    if (slopes != nullptr) {
+        need_same_device(q, slopes, op);
+        if (slopes->scalar_type() != at::kFloat || slopes->dim() != 1 || slopes->size(0) != heads) fail("%s: slopes must be a float32 vector of one per head", op);
+        x.keep[0] = packed(*slopes);
+        x.r.slopes = static_cast<const float*>(x.keep[0].data_ptr());
+    }
+    if (bias != nullptr) {
+        need_same_device(q, bias, op);
+        if (bias->scalar_type() != at::kFloat || bias->dim() != 2 || bias->size(0) != heads || bias->size(1) % 2 != 1)
+            fail("%s: distance_bias must be float32 (heads, 2 * radius + 1)", op);
+        if (bias->size(1) > 2 * STOF_SCORED_MAX_RADIUS + 1) fail("%s: distance_bias reaches %lld away, beyond the maximum of %d", op,
+                                                                 static_cast<long long>(bias->size(1) / 2), STOF_SCORED_MAX_RADIUS);
+        x.keep[1] = packed(*bias);
+        x.r.distance_bias = static_cast<const float*>(x.keep[1].data_ptr());
+        x.r.bias_radius = static_cast<int>(bias->size(1) / 2);
+    }
+}
+
+// scored_attention(q, k, v, out, causal, window, softcap, slopes, distance_bias, documents, prefix_lens, key_lens, softmax_scale) -> out
+PyObject* py_scored_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const char* op = "scored_attention";
+        need_args(n, 13, op);
+        const at::Tensor &q = tensor_needed(a[0], op), &k = tensor_needed(a[1], op), &v = tensor_needed(a[2], op);
+        const at::Tensor *out = tensor_arg(a[3], op), *documents = tensor_arg(a[9], op);
+        need_cuda(&q);
+        for (const at::Tensor* t : {&k, &v, out, documents}) need_same_device(q, t, op);
+        const int type = half_type(q, op);
+        if (k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type()) fail("%s: q, k and v must have one type", op);
+        if (q.dim() != 4 || k.dim() != 4) fail("%s: q must be (B, H, Sq, D), k and v (B, Hkv, Sk, D)", op);
+        if (k.sizes() != v.sizes()) fail("%s: k and v must have one shape", op);
+        const int64_t B = q.size(0), H = q.size(1), Sq = q.size(2), D = q.size(3), N = k.size(1), Sk = k.size(2);
+        if (k.size(0) != B || k.size(3) != D) fail("%s: batch or head size of k and v differ from q's", op);
+        if (D != 64 && D != 128) fail("%s: head size %lld not in {64, 128}", op, static_cast<long long>(D));
+        if (N <= 0 || H % N != 0) fail("%s: %lld heads are not a multiple of %lld K/V heads", op, static_cast<long long>(H), static_cast<long long>(N));
+        const int causal = PyObject_IsTrue(a[4]);
+        if (causal < 0) throw PythonFail{};
+        need_entry(api.scored_attn, "stof_scored_attn");
+        const Launch l(q);
+        Rules x;
+        score_args(x, a[5], a[6], tensor_arg(a[7], op), tensor_arg(a[8], op), a[12], q, H, D, op);
+        x.r.causal = causal;
+        if (documents != nullptr) {
+            if (documents->scalar_type() != at::kInt || documents->dim() != 2 || documents->size(0) != B || documents->size(1) != Sk)
+                fail("%s: documents must be int32 (B, Sk)", op);
+            if (Sq > Sk) fail("%s: documents name keys: %lld queries need as many keys, got %lld", op, static_cast<long long>(Sq), static_cast<long long>(Sk));
+            x.keep[2] = documents->size(1) <= 1 || documents->stride(1) == 1 ? *documents : packed(*documents);
+            if (B > 1 && x.keep[2].stride(0) < Sk) x.keep[2] = packed(x.keep[2]);
+            x.r.documents = static_cast<const int*>(x.keep[2].data_ptr());
+            x.r.documents_stride = B > 1 ? x.keep[2].stride(0) : Sk;
+        }
+        x.r.prefix_lens = int_vector(tensor_arg(a[10], op), B, q, x.keep[3], op, "prefix_lens");
+        x.r.key_lens = int_vector(tensor_arg(a[11], op), B, q, x.keep[4], op, "key_lens");
+        if (x.r.prefix_lens != nullptr && !causal) fail("%s: a prefix makes keys visible that a causal mask hides: it needs causal", op);
+        at::Tensor made;
+        if (out == nullptr) {
+            made = make(q.sizes(), q.scalar_type(), q);
+        } else {
+            need_output(*out, q, op);
+            if (overlap(*out, q) || overlap(*out, k) || overlap(*out, v)) fail("%s: out must not overlap the inputs", op);
+        }
+        const at::Tensor& o = out != nullptr ? *out : made;
+        if (Sk == 0 && q.numel() > 0) {
+            const Released gil;
+            const_cast<at::Tensor&>(o).zero_();
+        } else {
+            const at::Tensor qr = readable(q), kr = readable(k), vr = readable(v);
+            long long sq[3], sk[3], sv[3], so[3];
+            strides_of(qr, sq);
+            strides_of(kr, sk);
+            strides_of(vr, sv);
+            strides_of(o, so);
+            call("stof_scored_attn", api.scored_attn, qr.data_ptr(), kr.data_ptr(), vr.data_ptr(), o.data_ptr(), type, as_int(B, "batch"), as_int(H, "heads"),
+                 as_int(N, "K/V heads"), as_int(Sq, "queries"), as_int(Sk, "keys"), static_cast<int>(D), sq, sk, sv, so, &x.r, l.status, l.stream);
+        }
+        return out != nullptr ? same(a[3]) : wrap(made);
+    });
+}
+
+struct Cache {
+    int type, pages, page_size, heads, dim;
+    void *k, *v;
+    float *k_scales, *v_scales;
+};
+Cache cache_args(PyObject* const* a, const char* op) {
+    const at::Tensor &k = tensor_needed(a[0], op), &v = tensor_needed(a[1], op), &ks = tensor_needed(a[2], op), &vs = tensor_needed(a[3], op);
+    need_cuda(&k);
+    for (const at::Tensor* t : {&v, &ks, &vs}) need_same_device(k, t, op);
+    Cache c;
+    c.type = entry_type(k, op);
+    if (v.scalar_type() != k.scalar_type() || k.dim() != 4 || k.sizes() != v.sizes()) fail("%s: k_pages and v_pages must have one type and shape (pages, Hkv, page_size, D)", op);
+    if (!k.is_contiguous() || !v.is_contiguous() || ((reinterpret_cast<uintptr_t>(k.data_ptr()) | reinterpret_cast<uintptr_t>(v.data_ptr())) & 15u) != 0)
+        fail("%s: cache pages must be contiguous, at an address that is a multiple of 16 bytes", op);
+    for (const at::Tensor* t : {&ks, &vs})
+        if (t->scalar_type() != at::kFloat || t->dim() != 2 || t->size(0) != k.size(0) || t->size(1) != k.size(1) || !t->is_contiguous())
+            fail("%s: scales must be contiguous float32 (pages, Hkv)", op);
+    c.pages = as_int(k.size(0), "pages");
+    c.heads = as_int(k.size(1), "K/V heads");
+    c.page_size = as_int(k.size(2), "page size");
+    c.dim = as_int(k.size(3), "head size");
+    if (c.page_size != 16 && c.page_size != 32 && c.page_size != 64 && c.page_size != 128) fail("%s: page size %d not in {16, 32, 64, 128}", op, c.page_size);
+    if (c.dim != 64 && c.dim != 128) fail("%s: head size %d not in {64, 128}", op, c.dim);
+    c.k = k.data_ptr();
+    c.v = v.data_ptr();
+    c.k_scales = static_cast<float*>(ks.data_ptr());
+    c.v_scales = static_cast<float*>(vs.data_ptr());
+    return c;
+}
+
+// A (B, W) int32 block table with contiguous rows
+void need_table(const at::Tensor& t, int64_t rows, const char* op) {
+    if (t.scalar_type() != at::kInt || t.dim() != 2 || t.size(0) != rows || (t.size(1) > 1 && t.stride(1) != 1) || (rows > 1 && t.stride(0) < t.size(1)))
+        fail("%s: block_table must be int32 (requests, width) with contiguous rows", op);
+}
+
+// cache_attention(q, k_pages, v_pages, k_scales, v_scales, block_table, lengths, out, window, softcap, slopes, distance_bias, softmax_scale) -> out
+PyObject* py_cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const char* op = "cache_attention";
+        need_args(n, 13, op);
+        const at::Tensor &q = tensor_needed(a[0], op), &table = tensor_needed(a[5], op);
+        const at::Tensor* out = tensor_arg(a[7], op);
+        need_cuda(&q);
+        const int type = half_type(q, op);
+        const Cache c = cache_args(a + 1, op);
+        need_same_device(q, &tensor_needed(a[1], op), op);
+        need_same_device(q, &table, op);
+        need_same_device(q, out, op);
+        if (q.dim() != 4) fail("%s: q must be (requests, tokens, heads, D)", op);
+        const int64_t B = q.size(0), T = q.size(1), H = q.size(2), D = q.size(3);
+        if (D != c.dim) fail("%s: head size of q (%lld) differs from the cache's (%d)", op, static_cast<long long>(D), c.dim);
+        if (c.heads <= 0 || H <= 0 || H % c.heads != 0) fail("%s: %lld heads are not a multiple of %d K/V heads", op, static_cast<long long>(H), c.heads);
+        need_table(table, B, op);
+        need_entry(api.cache_attn, "stof_cache_attn");
+        need_entry(api.cache_attn_workspace_bytes, "stof_cache_attn_workspace_bytes");
+        const Launch l(q);
+        Rules x;
+        score_args(x, a[8], a[9], tensor_arg(a[10], op), tensor_arg(a[11], op), a[12], q, H, D, op);
+        const int* lengths = int_vector(&tensor_needed(a[6], op), B, q, x.keep[2], op, "lengths");
+        at::Tensor made;
+        if (out == nullptr) {
+            made = make(q.sizes(), q.scalar_type(), q);
+        } else {
+            need_output(*out, q, op);
+            if (overlap(*out, q)) fail("%s: out must not overlap q", op);
+        }
+        const at::Tensor& o = out != nullptr ? *out : made;
+        if (q.numel() > 0) {
+            const at::Tensor qr = readable(q);
+            long long sq[3], so[3];
+            strides_of(qr, sq);
+            strides_of(o, so);
+            const int b = as_int(B, "requests"), t = as_int(T, "tokens"), h = as_int(H, "heads"), width = as_int(table.size(1), "width of the block table");
+            const size_t bytes = api.cache_attn_workspace_bytes(b, t, h, c.heads, c.dim, c.page_size, width);
+            const at::Tensor workspace = make({static_cast<int64_t>(bytes)}, at::kByte, q);
+            call("stof_cache_attn", api.cache_attn, qr.data_ptr(), o.data_ptr(), type, sq, so, c.k, c.v, c.k_scales, c.v_scales, c.type, c.pages, c.page_size,
+                 c.heads, c.dim, static_cast<const int*>(table.data_ptr()), static_cast<long long>(B > 1 ? table.stride(0) : table.size(1)), width, lengths, b, t, h,
+                 &x.r, workspace.data_ptr(), bytes, l.status, l.stream);
+        }
+        return out != nullptr ? same(a[7]) : wrap(made);
+    });
+}
+
+// cache_append(k_pages, v_pages, k_scales, v_scales, k, v, slots)
+PyObject* py_cache_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const char* op = "cache_append";
+        need_args(n, 7, op);
+        const Cache c = cache_args(a, op);
+        const at::Tensor &pages = tensor_needed(a[0], op), &k = tensor_needed(a[4], op), &v = tensor_needed(a[5], op);
+        for (const at::Tensor* t : {&k, &v}) need_same_device(pages, t, op);
+        const int type = half_type(k, op);
+        if (v.scalar_type() != k.scalar_type() || k.dim() != 3 || k.sizes() != v.sizes()) fail("%s: k and v must have one type and shape (tokens, Hkv, D)", op);
+        if (k.size(1) != c.heads || k.size(2) != c.dim) fail("%s: k and v must be (tokens, %d, %d), as the cache is", op, c.heads, c.dim);
+        need_entry(api.cache_append, "stof_cache_append");
+        const Launch l(pages);
+        at::Tensor keep;
+        const int* slots = int_vector(&tensor_needed(a[6], op), k.size(0), pages, keep, op, "slots");
+        if (k.numel() > 0) {
+            const at::Tensor kr = readable(k), vr = readable(v);
+            long long sk[2], sv[2];
+            strides_of(kr, sk);
+            strides_of(vr, sv);
+            call("stof_cache_append", api.cache_append, c.k, c.v, c.k_scales, c.v_scales, c.type, c.pages, c.page_size, c.heads, c.dim, kr.data_ptr(), vr.data_ptr(),
+                 type, sk, sv, slots, as_int(k.size(0), "tokens"), l.status, l.stream);
+        }
+        Py_RETURN_NONE;
+    });
+}
+
+// page_tables(lengths, held, block_table, free_pages, free_count, page_size, new_tokens) -> (slots, starts, free_count, missing)
+PyObject* py_page_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const char* op = "page_tables";
+        need_args(n, 7, op);
+        const at::Tensor &lengths = tensor_needed(a[0], op), &table = tensor_needed(a[2], op), &stack = tensor_needed(a[3], op), &count = tensor_needed(a[4], op);
+        need_cuda(&lengths);
+        for (const at::Tensor* t : {&table, &stack, &count}) need_same_device(lengths, t, op);
+        if (lengths.dim() != 1) fail("%s: lengths must be an int32 vector", op);
+        const int64_t B = lengths.size(0);
+        const long page = long_arg(a[5]), fresh = long_arg(a[6]);
+        if (fresh < 0) fail("%s: new_tokens must not be negative", op);
+        need_table(table, B, op);
+        if (stack.scalar_type() != at::kInt || stack.dim() != 1 || (stack.size(0) > 1 && stack.stride(0) != 1)) fail("%s: free_pages must be a contiguous int32 vector", op);
+        if (count.scalar_type() != at::kInt || count.numel() != 1) fail("%s: free_count must be one int32", op);
+        need_entry(api.page_tables, "stof_page_tables");
+        const Launch l(lengths);
+        at::Tensor keep[2];
+        const int* len = int_vector(&lengths, B, lengths, keep[0], op, "lengths");
+        const int* held = int_vector(&tensor_needed(a[1], op), B, lengths, keep[1], op, "held");
+        const at::Tensor slots = make({fresh}, at::kInt, lengths), starts = make({B + 1}, at::kInt, lengths), left = make({1}, at::kInt, lengths),
+                         missing = make({1}, at::kInt, lengths);
+        call("stof_page_tables", api.page_tables, len, held, as_int(B, "requests"), static_cast<int*>(table.data_ptr()),
+             static_cast<long long>(B > 1 ? table.stride(0) : table.size(1)), as_int(table.size(1), "width of the block table"), static_cast<int*>(stack.data_ptr()),
+             as_int(stack.size(0), "free pages"), static_cast<const int*>(count.data_ptr()), as_int(page, "page size"), static_cast<int*>(slots.data_ptr()),
+             as_int(fresh, "new tokens"), static_cast<int*>(starts.data_ptr()), static_cast<int*>(left.data_ptr()), static_cast<int*>(missing.data_ptr()),
+             l.status, l.stream);
+        PyObject* tuple = PyTuple_New(4);
+        const at::Tensor* o[4] = {&slots, &starts, &left, &missing};
+        for (int i = 0; i < 4; ++i) PyTuple_SET_ITEM(tuple, i, wrap(*o[i]));
+        return tuple;
+    });
+}
+
 // ------------------------------------------------------------------------------------------ mask -> block index
 // What a compaction in progress keeps for itself on a device: a header that its kernel leaves at zero and a record in host
 // memory that the kernel writes its counts to.  A fixed number per device, made at its first compaction; a call holds one until
@@ -878,6 +1201,13 @@ PyObject* py_bind(PyObject*, PyObject* args) {
     get(x.gemm_bias_act, "stof_gemm_bias_act");
     get(x.gemm_ln, "stof_gemm_bias_residual_layernorm");
     get(x.layernorm, "stof_bias_residual_layernorm");
+    // a library that lacks these serves the other operators
+    auto may_get = [&](auto& f, const char* name) { f = reinterpret_cast<std::remove_reference_t<decltype(f)>>(dlsym(h, name)); };
+    may_get(x.scored_attn, "stof_scored_attn");
+    may_get(x.cache_attn_workspace_bytes, "stof_cache_attn_workspace_bytes");
+    may_get(x.cache_attn, "stof_cache_attn");
+    may_get(x.cache_append, "stof_cache_append");
+    may_get(x.page_tables, "stof_page_tables");
     if (!ok) return nullptr;
     api = x;
     g_error = same(err);
@@ -897,6 +1227,10 @@ PyMethodDef methods[] = {
     FAST("attention_inplace", py_attention_inplace),
     FAST("merged_attention", py_merged_attention),
     FAST("stack", py_stack),
+    FAST("scored_attention", py_scored_attention),
+    FAST("cache_attention", py_cache_attention),
+    FAST("cache_append", py_cache_append),
+    FAST("page_tables", py_page_tables),
     FAST("sparse_storage", py_sparse_storage),
     {"forget", py_forget, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -8,15 +8,23 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # STOF_B200_LIBRARY selects another build of the same library (for instance a debug build)
 _LIB_PATH = os.environ.get("STOF_B200_LIBRARY") or os.path.join(_HERE, "libstof_b200.so")
 
-STOF_DTYPE_F16, STOF_DTYPE_F32 = 0, 1
+STOF_DTYPE_F16, STOF_DTYPE_F32, STOF_DTYPE_BF16, STOF_DTYPE_INT8, STOF_DTYPE_E4M3 = 0, 1, 2, 3, 4
 EPI_BIAS, EPI_BIAS_GELU_ERF, EPI_BIAS_GELU_TANH, EPI_BIAS_RESIDUAL, EPI_BIAS_RELU = 0, 1, 2, 3, 4
 
 EXPORTS = ("stof_version", "stof_last_error", "stof_mask_workspace_bytes", "stof_mask_classify", "stof_mask_classify_notify", "stof_mask_fill", "stof_mask_compact_static",
-           "stof_block_attn_plan_bytes", "stof_block_attn_plan", "stof_block_attn_plan_paired", "stof_block_attn", "stof_block_attn_scheduled", "stof_gemm_bias_act", "stof_gemm_bias_residual_layernorm", "stof_bias_residual_layernorm")
+           "stof_block_attn_plan_bytes", "stof_block_attn_plan", "stof_block_attn_plan_paired", "stof_block_attn", "stof_block_attn_scheduled", "stof_gemm_bias_act", "stof_gemm_bias_residual_layernorm", "stof_bias_residual_layernorm",
+           "stof_scored_attn", "stof_cache_attn_workspace_bytes", "stof_cache_attn", "stof_cache_append", "stof_page_tables")
 
 
 class StofError(RuntimeError):
     pass
+
+
+class ScoreRules(ctypes.Structure):
+    """`stof_score_rules`: how scores are changed and masked."""
+    _fields_ = [("softmax_scale", ctypes.c_float), ("softcap", ctypes.c_float), ("causal", ctypes.c_int), ("window", ctypes.c_int),
+                ("slopes", ctypes.c_void_p), ("distance_bias", ctypes.c_void_p), ("bias_radius", ctypes.c_int), ("documents", ctypes.c_void_p),
+                ("documents_stride", ctypes.c_longlong), ("prefix_lens", ctypes.c_void_p), ("key_lens", ctypes.c_void_p)]
 
 
 def library_path() -> str:
@@ -68,6 +76,17 @@ def lib() -> ctypes.CDLL:
     L.stof_gemm_bias_residual_layernorm.argtypes = [vp, i64, vp, i64, vp, vp, i64, vp, vp, f32, vp, i64, i32, i32, i32, vp, vp]
     L.stof_bias_residual_layernorm.restype = i32
     L.stof_bias_residual_layernorm.argtypes = [vp, i64, vp, vp, i64, vp, vp, f32, vp, i64, i32, i32, vp, vp]
+    rules = ctypes.POINTER(ScoreRules)
+    L.stof_scored_attn.restype = i32
+    L.stof_scored_attn.argtypes = [vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i64x3, i64x3, i64x3, i64x3, rules, vp, vp]
+    L.stof_cache_attn_workspace_bytes.restype = sz
+    L.stof_cache_attn_workspace_bytes.argtypes = [i32] * 7
+    L.stof_cache_attn.restype = i32
+    L.stof_cache_attn.argtypes = [vp, vp, i32, i64x3, i64x3, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, i64, i32, vp, i32, i32, i32, rules, vp, sz, vp, vp]
+    L.stof_cache_append.restype = i32
+    L.stof_cache_append.argtypes = [vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, vp, i32, i64x3, i64x3, vp, i32, vp, vp]
+    L.stof_page_tables.restype = i32
+    L.stof_page_tables.argtypes = [vp, vp, i32, vp, i64, i32, vp, i32, vp, i32, vp, i32, vp, vp, vp, vp, vp]
     _lib = L
     return L
 
