@@ -91,7 +91,9 @@ __device__ __forceinline__ void write_run(const AppendParams& p, int side, int h
         for (int i = part * 32 + lane; i < row * D / 16; i += parts * 32) {
             const uint4 u = front[i];
             auto again = [&](uint32_t w) {
-                const float2 a = unpack_pair<false>(entries_to_half2<E4M3>(w)), b = unpack_pair<false>(entries_to_half2<E4M3>(w >> 16));
+                uint32_t lo, hi;
+                entries_to_half<E4M3>(w, lo, hi);
+                const float2 a = unpack_pair<false>(lo), b = unpack_pair<false>(hi);
                 return quantise2<E4M3>(a.x, a.y, ratio) | (quantise2<E4M3>(b.x, b.y, ratio) << 16);
             };
             front[i] = make_uint4(again(u.x), again(u.y), again(u.z), again(u.w));

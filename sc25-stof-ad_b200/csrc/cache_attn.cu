@@ -3,17 +3,17 @@
 // The query rows that share a K/V head (heads / kv_heads heads of each token) are the columns of both products, in tiles of 8:
 //   S^T (16 keys x 8 rows) = K (16 keys x D) Q^T       O^T (D x 8 rows) += V^T (D x 16 keys) P^T
 // on mma.sync m16n8k16.  A tcgen05 product has at least 64 rows of which a decoding step fills one to eight, and takes its operands
-// from shared memory as 8 or 16 bits; here the entries go from global memory to registers, become fp16 there (exactly) and are
-// multiplied, with no shared memory in between.  The scales stay out of the products: K's goes into the score, V's into P,
+// from shared memory as 8 or 16 bits; here the entries become fp16 (exactly) on their way from shared memory to registers and are
+// multiplied.  The scales stay out of the products: K's goes into the score, V's into P,
 // relative to a reference that the accumulator carries (so that P keeps fp16's precision whatever the scales are).
 //
-// Which lane holds which entry is free as long as both operands agree, so that every load is 16 bytes of a row: with g = lane / 4,
+// Which lane holds which entry is free as long as both operands agree, so that every read is 16 bytes of a row: with g = lane / 4,
 // c = lane % 4, a lane reads chunk c (and c + 4) of the rows of keys g and g + 8 for S, and chunk g of the rows of keys 2c, 2c + 1,
 // 2c + 8, 2c + 9 for O.  P leaves the first product with keys along g and is wanted with rows along g: one 8 x 8 transpose.
 //
-// Work is counted in units of 64 keys (16 for each of a block's four warps) over all requests and K/V heads; every block takes an
-// equal stretch of that line, whatever the lengths.  A (request, head) that one block covers is written at once, the others in parts
-// that cache_attn_join_kernel adds in the order of the blocks.
+// Work is counted in units of 128 keys (32 for each of a block's four warps).  The units of a (request, K/V head, row group) are cut into
+// pieces of about the same length everywhere, a piece a block, whatever the lengths of the requests (which only the device knows).
+// What one block covers is written at once, the rest in parts that cache_attn_join_kernel adds in the order of the blocks.
 #include "cache_common.cuh"
 #include "stof_host.h"
 #include "stof_ptx.cuh"
@@ -22,7 +22,20 @@ namespace stof {
 namespace {
 
 constexpr int CT_WARPS = 4, CT_THREADS = CT_WARPS * 32;
-constexpr int CT_UNIT = 16 * CT_WARPS;       // keys of a unit
+constexpr int CT_TILES = 2;                  // tiles of 16 keys that a warp takes at a time: independent chains of products, and half the work around them
+constexpr int CT_STEP = 16 * CT_TILES, CT_UNIT = CT_STEP * CT_WARPS;     // keys of a warp's step, of a block's: the unit
+#ifndef CT_STAGES
+#define CT_STAGES 2
+#endif
+#ifndef CT_LONG
+#define CT_LONG 16
+#endif
+#ifndef CT_WAVES
+#define CT_WAVES 4
+#endif
+#ifndef CT_BLOCKS
+#define CT_BLOCKS 3
+#endif
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct CacheAttnParams {
@@ -35,17 +48,19 @@ struct CacheAttnParams {
     long long table_stride;
     const int* lengths;
     const float *slopes, *distance_bias;
-    float* workspace;
+    int2* parts;                             // workspace: (first block, blocks) of every request's (K/V head, row group) ...
+    float* workspace;                        // ... and the partial result of every block
     int* status;
     float scale, softcap;
     int window, radius;
     int requests, tokens, heads, kv_heads, group;            // group = heads / kv_heads
     int rows, row_groups;                                    // query rows of a K/V head, and how many blocks of them
     int table_width, page_count, page_shift;
+    int resident;                                            // blocks that the GPU holds at once
     int bf16;
 };
 
-// keys [first, first + 64 * units) cover what the request's tokens see
+// keys [first, first + 128 * units) cover what the request's tokens see
 struct Span { int length, first, units; };
 __device__ __forceinline__ Span span_of(const CacheAttnParams& p, int b) {
     const long long most = static_cast<long long>(p.table_width) << p.page_shift;
@@ -55,22 +70,15 @@ __device__ __forceinline__ Span span_of(const CacheAttnParams& p, int b) {
     return {length, first, (length - first + CT_UNIT - 1) / CT_UNIT};
 }
 
-__device__ __forceinline__ long long block_sum(long long v, long long* shared) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
-    __syncthreads();
-    long long s = 0;
-#pragma unroll
-    for (int i = 0; i < CT_WARPS; ++i) s += shared[i];
-    return s;
+// How long the pieces are that the (request, K/V head, row group)s are cut into, in units, for `total` units in `pairs` of them: such that
+// there are about as many pieces as blocks that the GPU holds at once (a piece too many would wait for a whole round: every pair rounds
+// up, by half a piece on average), or more of CT_LONG units where there is work for more, so that blocks that get on faster take over
+// from the others towards the end.
+__device__ __forceinline__ unsigned piece_units(unsigned total, unsigned pairs, unsigned resident) {
+    const unsigned at_once = pairs < resident ? resident - pairs / 2 : resident;
+    const unsigned target = max(at_once, min(total / CT_LONG, resident * CT_WAVES));
+    return max((total + target - 1) / target, 1u);
 }
-
-// blocks that get a stretch of the line: each at least a unit
-__device__ __forceinline__ int blocks_at_work(long long total, int blocks) { return static_cast<int>(min(total, static_cast<long long>(blocks))); }
-// where block i's stretch of the line begins
-__device__ __forceinline__ long long stretch(long long total, int i, int blocks) { return total * i / blocks; }
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -82,77 +90,129 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     return r;
 }
 
-// what a lane loads of 16 keys
+// A warp's ring in shared memory, CT_TILES tiles of 16 keys a stage, filled by 16-byte asynchronous copies that only the warp itself waits for.  The
+// chunks of a row are permuted, in D = 64 the rows of V too, so that the eight (or sixteen) lanes that a shared-memory access serves at
+// once meet all banks.
 template <int D>
-struct Tile {
-    uint4 k[2][D / 64];                      // keys g, g + 8
-    uint4 v[4];                              // keys 2c, 2c + 1, 2c + 8, 2c + 9 (D = 64: the first half)
-    float k_scale, v_scale;
-    int key;                                 // first key; -1: no page, nothing loaded
+struct Ring {
+    static constexpr int STAGES = CT_STAGES;
+    static constexpr int SIDE = 16 * D, TILE = 2 * SIDE + 16, STAGE = CT_TILES * TILE;       // of a tile: K, V, {k scale, v scale, valid, -}
+    static constexpr int BYTES = STAGES * STAGE;
+    static constexpr int CHUNKS = D / 16, LOADS = CHUNKS / 2;                // of a row; copies of a lane per side
+    static __device__ __forceinline__ int k_at(int row, int chunk) {
+        return D == 128 ? row * D + ((chunk ^ ((row & 1) << 2)) << 4) : row * D + (chunk << 4);
+    }
+    static __device__ __forceinline__ int v_at(int row, int chunk) {
+        if (D == 128) return row * D + ((chunk ^ (row & 6)) << 4);
+        const int place = (row >> 1) | ((row & 1) << 3);
+        return place * D + ((chunk ^ (place & 2)) << 4);
+    }
 };
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
 
 template <int NT, int D, bool E4M3>
-__global__ void __launch_bounds__(CT_THREADS, NT == 1 ? 4 : 3) cache_attn_kernel(const CacheAttnParams p) {
+__global__ void __launch_bounds__(CT_THREADS, NT == 1 ? CT_BLOCKS : 2) cache_attn_kernel(const CacheAttnParams p) {
     constexpr int CH = D / 64, KS = D / 16, MT = D / 16, ROWS = NT * 8;
     constexpr int V_BYTES = D / 8;           // of a row, per lane
-    __shared__ long long sums[CT_WARPS];
-    __shared__ long long found_base;
-    __shared__ int found_request;
+    using R = Ring<D>;
+    extern __shared__ __align__(128) unsigned char ca_smem[];
     __shared__ float merge_m[CT_WARPS][ROWS], merge_l[CT_WARPS][ROWS];
-    __shared__ __align__(16) float merge_o[ROWS][D + 4];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+    float (*merge_o)[D + 4] = reinterpret_cast<float (*)[D + 4]>(ca_smem);   // the rings are free when it is used
+    static_assert(CT_WARPS * ROWS * (D + 4) * 4 <= CT_WARPS * R::BYTES, "merge_o lies over the rings");
+    unsigned char* ring = ca_smem + warp * R::BYTES;
+    const uint32_t ring_addr = smem_u32(ring);
     grid_dependency_wait();
     grid_launch_dependents();
     if (__syncthreads_or(failure_reported(p.status))) return;
-    const int pairs = p.kv_heads * p.row_groups;             // of a request
-    long long total = 0;
-    for (int b = threadIdx.x; b < p.requests; b += CT_THREADS) total += span_of(p, b).units;
-    total = block_sum(total, sums) * pairs;
-    const int blocks = blocks_at_work(total, gridDim.x);
-    if (static_cast<int>(blockIdx.x) >= blocks) return;
-    long long at = stretch(total, blockIdx.x, blocks);
-    const long long end = stretch(total, blockIdx.x + 1, blocks);
-    // the request in which the stretch begins
-    long long base = 0;
-    for (int b0 = 0; b0 < p.requests; b0 += CT_THREADS) {
-        const int b = b0 + static_cast<int>(threadIdx.x);
-        long long mine = b < p.requests ? static_cast<long long>(span_of(p, b).units) * pairs : 0, upto = mine;
+    // which piece is this block's?  Every warp finds out for itself, a lane a request (no barrier, the lengths are in the cache)
+    const unsigned pairs = static_cast<unsigned>(p.kv_heads * p.row_groups);     // of a request
+    unsigned total = 0, some = 0;
+    for (int i = lane; i < p.requests; i += 32) {
+        const int units = span_of(p, i).units;
+        total += static_cast<unsigned>(units);
+        some += units > 0 ? 1u : 0u;
+    }
+    total = __reduce_add_sync(0xffffffffu, total) * pairs;
+    some = __reduce_add_sync(0xffffffffu, some) * pairs;
+    const unsigned length_each = piece_units(total, some, static_cast<unsigned>(p.resident));
+    int b = -1;
+    unsigned base = 0;
+    for (int b0 = 0; b0 < p.requests; b0 += 32) {
+        const unsigned units = b0 + lane < p.requests ? static_cast<unsigned>(span_of(p, b0 + lane).units) : 0u;
+        const unsigned mine = (units + length_each - 1) / length_each * pairs;
+        unsigned upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+            const unsigned v = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += v;
         }
-        __syncthreads();
-        if (lane == 31) sums[warp] = upto;
-        __syncthreads();
-        long long all = 0;
-        for (int i = 0; i < CT_WARPS; ++i) {
-            if (i < warp) upto += sums[i];
-            all += sums[i];
+        const unsigned here = __ballot_sync(0xffffffffu, blockIdx.x >= base + upto - mine && blockIdx.x < base + upto);
+        if (here != 0) {
+            const int at = __ffs(here) - 1;
+            b = b0 + at;
+            base += __shfl_sync(0xffffffffu, upto - mine, at);
+            break;
         }
-        if (at >= base + upto - mine && at < base + upto) {
-            found_request = b;
-            found_base = base + upto - mine;
-        }
-        base += all;
-        if (at < base) break;
+        base += __shfl_sync(0xffffffffu, upto, 31);
     }
-    __syncthreads();
-    int b = found_request;
-    base = found_base;
-
-    while (at < end) {
-        const Span span = span_of(p, b);
-        const long long behind = base + static_cast<long long>(span.units) * pairs;
-        if (at >= behind) {                                  // (requests of length 0 are passed over here)
-            base = behind;
-            ++b;
-            continue;
+    if (b < 0) return;
+    const Span span = span_of(p, b);
+    const unsigned pieces = (static_cast<unsigned>(span.units) + length_each - 1) / length_each;
+    const unsigned pair = (blockIdx.x - base) / pieces, piece = (blockIdx.x - base) - pair * pieces;
+    const unsigned each = static_cast<unsigned>(span.units) / pieces, extra = static_cast<unsigned>(span.units) - each * pieces;
+    const int u0 = static_cast<int>(piece * each + min(piece, extra)), u1 = u0 + static_cast<int>(each + (piece < extra ? 1u : 0u));
+    const int kv = static_cast<int>(pair) / p.row_groups, row0 = (static_cast<int>(pair) % p.row_groups) * ROWS;
+    if (piece == 0 && threadIdx.x == 0) p.parts[b * pairs + pair] = make_int2(static_cast<int>(blockIdx.x), static_cast<int>(pieces));   // for the kernel that joins them
+    {
+        const int* pages = p.block_table + b * p.table_stride;
+        const int last_key = min(span.length, span.first + u1 * CT_UNIT);
+        struct Pages { int of[CT_TILES]; };
+        auto pages_of = [&](int key) {                       // of the tiles from this key on; -1 behind the last
+            Pages r;
+#pragma unroll
+            for (int i = 0; i < CT_TILES; ++i) r.of[i] = key + 16 * i < last_key ? pages[(key + 16 * i) >> p.page_shift] : -1;
+            return r;
+        };
+        // asks for the tiles from this key on; what cannot be had is marked
+        auto ask = [&](int key, int stage, const Pages& page) {
+#pragma unroll
+            for (int i = 0; i < CT_TILES; ++i) {
+                const int offset = stage * R::STAGE + i * R::TILE;
+                const bool there = key + 16 * i < last_key, good = there && static_cast<unsigned>(page.of[i]) < static_cast<unsigned>(p.page_count);
+                if (lane == 0) {
+                    *reinterpret_cast<int*>(ring + offset + 2 * R::SIDE + 8) = good;
+                    if (there && !good && p.status != nullptr) atomicCAS(p.status, 0, STATUS_BAD_INDEX);
+                }
+                if (good) {
+                    const uint32_t dst = ring_addr + offset;
+                    const size_t slot = static_cast<size_t>(page.of[i]) * p.kv_heads + kv;
+                    const size_t at = ((slot << p.page_shift) + ((key + 16 * i) & ((1 << p.page_shift) - 1))) * D + lane * 16;
+                    const char *kp = static_cast<const char*>(p.k_pages) + at, *vp = static_cast<const char*>(p.v_pages) + at;
+#pragma unroll
+                    for (int j = 0; j < R::LOADS; ++j) copy16(dst + R::k_at((j * 32 + lane) / R::CHUNKS, lane % R::CHUNKS), kp + j * 512);
+#pragma unroll
+                    for (int j = 0; j < R::LOADS; ++j) copy16(dst + R::SIDE + R::v_at((j * 32 + lane) / R::CHUNKS, lane % R::CHUNKS), vp + j * 512);
+                    if (lane < 2) copy4(dst + 2 * R::SIDE + lane * 4, (lane == 0 ? p.k_scales : p.v_scales) + slot);
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        // STAGES - 1 steps on their way while one is used; pages' numbers are asked for a step before their tiles
+        int key = span.first + u0 * CT_UNIT + warp * CT_STEP, far = key;
+        Pages page = pages_of(far);
+#pragma unroll
+        for (int i = 0; i < R::STAGES - 1; ++i) {
+            const Pages after = pages_of(far + CT_UNIT);
+            ask(far, i, page);
+            page = after;
+            far += CT_UNIT;
         }
-        const int pair = static_cast<int>((at - base) / span.units), u0 = static_cast<int>((at - base) % span.units);
-        const int u1 = static_cast<int>(min(static_cast<long long>(span.units), u0 + (end - at)));
-        const int kv = pair / p.row_groups, row0 = (pair % p.row_groups) * ROWS;
-
         // ---- the query rows: fp16, each row times a power of two (bf16 has more range than fp16; fp16 rows are taken as they are)
         uint32_t qf[NT][KS][2];
         float row_scale[NT][2], slope[NT][2];
@@ -207,17 +267,19 @@ __global__ void __launch_bounds__(CT_THREADS, NT == 1 ? 4 : 3) cache_attn_kernel
                 const float f = __shfl_sync(0xffffffffu, shrink, (2 * c + e) * 4);
                 const int rr = row0 + nt * 8 + 2 * c + e, head = kv * p.group + rr % p.group;
                 const bool on = rr < p.rows;
-                row_scale[nt][e] = p.scale / f;
+                row_scale[nt][e] = p.scale / f * LOG2E;
                 pos[nt][e] = on ? span.length - p.tokens + rr / p.group : -1;
-                slope[nt][e] = on && p.slopes != nullptr ? p.slopes[head] : 0.f;
+                slope[nt][e] = on && p.slopes != nullptr ? p.slopes[head] * LOG2E : 0.f;
                 table[nt][e] = on && p.distance_bias != nullptr ? p.distance_bias + static_cast<size_t>(head) * (2 * p.radius + 1) + p.radius : p.distance_bias;
             }
         }
 
-        float o[NT][MT][4], m[NT][2], l[NT][2], v_ref = 0.f;
+        // m: reference of the row's P, 0 as long as it has seen nothing; most: what a score may be above it, minus infinity until then
+        float o[NT][MT][4], m[NT][2], most[NT][2], l[NT][2], v_ref = 0.f, v_ref_inv = 1.f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            m[nt][0] = m[nt][1] = -INFINITY;
+            m[nt][0] = m[nt][1] = 0.f;
+            most[nt][0] = most[nt][1] = -INFINITY;
             l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
@@ -225,86 +287,98 @@ __global__ void __launch_bounds__(CT_THREADS, NT == 1 ? 4 : 3) cache_attn_kernel
                 for (int e = 0; e < 4; ++e) o[nt][mt][e] = 0.f;
         }
 
-        const int* pages = p.block_table + b * p.table_stride;
-        auto page_of = [&](int u) {                          // of this warp's keys in unit u; -1 behind the last key
-            const int key = span.first + u * CT_UNIT + warp * 16;
-            return u < u1 && key < span.length ? pages[key >> p.page_shift] : -1;
-        };
-        auto load = [&](Tile<D>& t, int u, int page) {
-            const int key = span.first + u * CT_UNIT + warp * 16;
-            t.key = -1;
-            if (u >= u1 || key >= span.length) return;
-            if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.page_count)) {
-                if (lane == 0 && p.status != nullptr) atomicCAS(p.status, 0, STATUS_BAD_INDEX);
-                return;
-            }
-            t.key = key;
-            const size_t slot = static_cast<size_t>(page) * p.kv_heads + kv;
-            t.k_scale = __ldca(p.k_scales + slot);
-            t.v_scale = __ldca(p.v_scales + slot);
-            const size_t row = (slot << p.page_shift) + (key & ((1 << p.page_shift) - 1));
-            const char *kp = static_cast<const char*>(p.k_pages) + row * D, *vp = static_cast<const char*>(p.v_pages) + row * D;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < CH; ++i) t.k[h][i] = __ldcs(reinterpret_cast<const uint4*>(kp + (g + 8 * h) * D + (c + 4 * i) * 16));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const char* src = vp + (2 * c + (j & 1) + 8 * (j >> 1)) * D + g * V_BYTES;
-                if constexpr (D == 128) {
-                    t.v[j] = __ldcs(reinterpret_cast<const uint4*>(src));
-                } else {
-                    const uint2 w = __ldcs(reinterpret_cast<const uint2*>(src));
-                    t.v[j].x = w.x;
-                    t.v[j].y = w.y;
-                }
-            }
-        };
         auto word = [](const uint4& u, int i) { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; };
-        auto compute = [&](Tile<D>& t) {
-            if (t.key < 0) return;
-            const int left = span.length - t.key;            // keys of the tile that exist; what lies behind them may be anything
-            if (left < 16) {
+        // up to here every row of the block sees all keys, where no rule hides any
+        const int all_see = p.slopes == nullptr && p.distance_bias == nullptr && p.window == 0 ? span.length - p.tokens + row0 / p.group : -1;
+        auto compute = [&](int key, const unsigned char* tiles) {
+            float k_scale[CT_TILES], v_scale[CT_TILES];
+            int left[CT_TILES];                              // keys of the tile that exist; what lies behind them may be anything
+            bool any = false;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (2 * c + (j & 1) + 8 * (j >> 1) >= left) t.v[j] = make_uint4(0u, 0u, 0u, 0u);
+            for (int i = 0; i < CT_TILES; ++i) {
+                const float4 head = *reinterpret_cast<const float4*>(tiles + i * R::TILE + 2 * R::SIDE);
+                const bool good = __float_as_int(head.z) != 0;
+                any = any || good;
+                k_scale[i] = good ? head.x : 0.f;
+                v_scale[i] = good && !(fabsf(head.y) < 1.17549435e-38f) ? head.y : 0.f;      // (1 / scale has to be finite)
+                left[i] = good ? span.length - key - 16 * i : 0;
             }
-            float s[NT][4];
+            if (!any) return;
+            float s[CT_TILES][NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int t = 0; t < CT_TILES; ++t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int i = 0; i < CH; ++i)
+                    for (int e = 0; e < 4; ++e) s[t][nt][e] = 0.f;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const uint32_t x = word(t.k[0][i], w), y = word(t.k[1][i], w);
-                    const uint32_t a0 = entries_to_half2<E4M3>(x), a2 = entries_to_half2<E4M3>(x >> 16);
-                    const uint32_t a1 = entries_to_half2<E4M3>(y), a3 = entries_to_half2<E4M3>(y >> 16);
+            for (int i = 0; i < CH; ++i) {
+                uint4 x[CT_TILES], y[CT_TILES];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma16816(s[nt], a0, a1, a2, a3, qf[nt][4 * i + w][0], qf[nt][4 * i + w][1]);
+                for (int t = 0; t < CT_TILES; ++t) {
+                    x[t] = *reinterpret_cast<const uint4*>(tiles + t * R::TILE + R::k_at(g, c + 4 * i));
+                    y[t] = *reinterpret_cast<const uint4*>(tiles + t * R::TILE + R::k_at(g + 8, c + 4 * i));
                 }
-            // scores in units of log2; element e: key g + 8 * (e / 2), row 2c + e % 2
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+                for (int w = 0; w < 4; ++w)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float x = s[nt][e] * (t.k_scale * row_scale[nt][e & 1]);
-                    if (p.softcap > 0.f) {
-                        // tanh(y) = 1 - 2 / (1 + e^(2y))
-                        const float ex = fast_exp2(x * (2.f * LOG2E / p.softcap));
-                        x = p.softcap - 2.f * p.softcap * __frcp_rn(1.f + ex);
+                    for (int t = 0; t < CT_TILES; ++t) {
+                        uint32_t a0, a1, a2, a3;
+                        entries_to_half<E4M3>(word(x[t], w), a0, a2);
+                        entries_to_half<E4M3>(word(y[t], w), a1, a3);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma16816(s[t][nt], a0, a1, a2, a3, qf[nt][4 * i + w][0], qf[nt][4 * i + w][1]);
                     }
-                    const int away = t.key + g + 8 * (e >> 1) - pos[nt][e & 1];      // at most 0 where visible
-                    x += slope[nt][e & 1] * static_cast<float>(away);
-                    const bool on = pos[nt][e & 1] >= 0 && away <= 0 && (p.window == 0 || away > -p.window);
-                    if (p.distance_bias != nullptr && on) x += __ldca(table[nt][e & 1] + max(away, -p.radius));
-                    s[nt][e] = on ? x * LOG2E : -INFINITY;
-                }
+            }
+            // scores in units of log2, less the row's reference; element e: key g + 8 * (e / 2), row 2c + e % 2
+            if (p.softcap > 0.f) {
+                // tanh(y) = 1 - 2 / (1 + e^(2y))
+                const float to = 2.f / p.softcap, from = p.softcap * LOG2E;
+#pragma unroll
+                for (int t = 0; t < CT_TILES; ++t)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            s[t][nt][e] = fmaf(-2.f * from, fast_reciprocal(1.f + fast_exp2(s[t][nt][e] * (k_scale[t] * row_scale[nt][e & 1] * to))), from);
+            } else {
+#pragma unroll
+                for (int t = 0; t < CT_TILES; ++t)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[t][nt][e] *= k_scale[t] * row_scale[nt][e & 1];
+            }
+            if (key + CT_STEP - 1 <= all_see && left[0] > 0 && left[CT_TILES - 1] > 0) {
+#pragma unroll
+                for (int t = 0; t < CT_TILES; ++t)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[t][nt][e] -= m[nt][e & 1];
+            } else {
+#pragma unroll
+                for (int t = 0; t < CT_TILES; ++t)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float x = s[t][nt][e];
+                            const int away = key + 16 * t + g + 8 * (e >> 1) - pos[nt][e & 1];   // at most 0 where visible
+                            x += slope[nt][e & 1] * static_cast<float>(away);
+                            const bool on = left[t] > 0 && pos[nt][e & 1] >= 0 && away <= 0 && (p.window == 0 || away > -p.window);
+                            if (p.distance_bias != nullptr && on) x += __ldca(table[nt][e & 1] + max(away, -p.radius)) * LOG2E;
+                            s[t][nt][e] = on ? x - m[nt][e & 1] : -INFINITY;
+                        }
+            }
             // V's scale against the reference that o is held in
-            if (t.v_scale > v_ref * 256.f || v_ref == 0.f) {
-                const float f = t.v_scale > 0.f ? v_ref / t.v_scale : 1.f;
-                v_ref = t.v_scale > 0.f ? t.v_scale : v_ref;
+            float v_size = 0.f;
+#pragma unroll
+            for (int t = 0; t < CT_TILES; ++t) v_size = fabsf(v_scale[t]) <= v_size ? v_size : fabsf(v_scale[t]);    // (a NaN stays)
+            if (!(v_size <= v_ref * 256.f) || v_ref == 0.f) {
+                const float f = v_size != 0.f ? v_ref / v_size : 1.f;
+                v_ref = v_size != 0.f ? v_size : v_ref;
+                v_ref_inv = v_ref > 0.f ? 1.f / v_ref : 1.f;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -312,70 +386,112 @@ __global__ void __launch_bounds__(CT_THREADS, NT == 1 ? 4 : 3) cache_attn_kernel
 #pragma unroll
                         for (int e = 0; e < 4; ++e) o[nt][mt][e] *= f;
             }
-            const float v_rel = v_ref > 0.f ? t.v_scale / v_ref : t.v_scale;
-            uint32_t pf[NT][2];
+            // a row's reference follows its maximum when that has grown by more than 2^8 (P is at most that, then)
+            bool grown = false;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                float top0 = fmaxf(s[nt][0], s[nt][2]), top1 = fmaxf(s[nt][1], s[nt][3]);
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int d = 4; d < 32; d <<= 1) {
-                    top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, d));
-                    top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, d));
+                for (int e = 0; e < 2; ++e) {
+                    float top = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
+#pragma unroll
+                    for (int t = 1; t < CT_TILES; ++t) top = fmaxf(top, fmaxf(s[t][nt][e], s[t][nt][2 + e]));
+                    grown = grown || top > most[nt][e];
                 }
-                if (__any_sync(0xffffffffu, top0 > m[nt][0] || top1 > m[nt][1])) {
-                    const float n0 = fmaxf(m[nt][0], top0), n1 = fmaxf(m[nt][1], top1);
-                    const float a0 = n0 == m[nt][0] ? 1.f : fast_exp2(m[nt][0] - n0), a1 = n1 == m[nt][1] ? 1.f : fast_exp2(m[nt][1] - n1);
-                    m[nt][0] = n0;
-                    m[nt][1] = n1;
-                    l[nt][0] *= a0;
-                    l[nt][1] *= a1;
+            if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        o[nt][mt][0] *= a0;
-                        o[nt][mt][1] *= a1;
-                        o[nt][mt][2] *= a0;
-                        o[nt][mt][3] *= a1;
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float top = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
+#pragma unroll
+                        for (int t = 1; t < CT_TILES; ++t) top = fmaxf(top, fmaxf(s[t][nt][e], s[t][nt][2 + e]));
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        if (top > -INFINITY && (top > 0.f || most[nt][e] < 0.f)) {
+                            const float f = most[nt][e] < 0.f ? 0.f : fast_exp2(-top);       // 0: the first that this row sees
+                            m[nt][e] += top;
+                            most[nt][e] = 8.f;
+                            l[nt][e] *= f;
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) {
+                                o[nt][mt][e] *= f;
+                                o[nt][mt][2 + e] *= f;
+                            }
+#pragma unroll
+                            for (int t = 0; t < CT_TILES; ++t) {
+                                s[t][nt][e] -= top;
+                                s[t][nt][2 + e] -= top;
+                            }
+                        }
                     }
+            }
+            uint32_t pf[CT_TILES][NT][2];
+#pragma unroll
+            for (int t = 0; t < CT_TILES; ++t) {
+                const float v_rel = v_scale[t] * v_ref_inv;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const float p0 = fast_exp2(s[t][nt][0]), p1 = fast_exp2(s[t][nt][1]), p2 = fast_exp2(s[t][nt][2]), p3 = fast_exp2(s[t][nt][3]);
+                    l[nt][0] += p0 + p2;
+                    l[nt][1] += p1 + p3;
+                    // to fp16 for the product, as the other attention kernels do; the sum is of the values before rounding
+                    pf[t][nt][0] = transpose8x8(pack_half2(p0 * v_rel, p1 * v_rel));
+                    pf[t][nt][1] = transpose8x8(pack_half2(p2 * v_rel, p3 * v_rel));
                 }
-                const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
-                const float p0 = fast_exp2(s[nt][0] - m0), p1 = fast_exp2(s[nt][1] - m1), p2 = fast_exp2(s[nt][2] - m0), p3 = fast_exp2(s[nt][3] - m1);
-                l[nt][0] += p0 + p2;
-                l[nt][1] += p1 + p3;
-                // to fp16 for the product, as the other attention kernels do; the sum is of the values before rounding
-                pf[nt][0] = transpose8x8(pack_half2(p0 * v_rel, p1 * v_rel));
-                pf[nt][1] = transpose8x8(pack_half2(p2 * v_rel, p3 * v_rel));
             }
 #pragma unroll
-            for (int w = 0; w < V_BYTES / 4; ++w) {
-                const uint32_t x0 = word(t.v[0], w), x1 = word(t.v[1], w), y0 = word(t.v[2], w), y1 = word(t.v[3], w);
+            for (int t = 0; t < CT_TILES; ++t) {
+                uint4 v[4];                                  // keys 2c, 2c + 1, 2c + 8, 2c + 9 (D = 64: the first half)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t x = __byte_perm(x0, x1, h == 0 ? 0x5140 : 0x7362), y = __byte_perm(y0, y1, h == 0 ? 0x5140 : 0x7362);
-                    const uint32_t a0 = entries_to_half2<E4M3>(x), a1 = entries_to_half2<E4M3>(x >> 16);
-                    const uint32_t a2 = entries_to_half2<E4M3>(y), a3 = entries_to_half2<E4M3>(y >> 16);
+                for (int j = 0; j < 4; ++j) {
+                    const int row = 2 * c + (j & 1) + 8 * (j >> 1);
+                    const unsigned char* src = tiles + t * R::TILE + R::SIDE + R::v_at(row, D == 128 ? g : g >> 1);
+                    if constexpr (D == 128) {
+                        v[j] = *reinterpret_cast<const uint4*>(src);
+                    } else {
+                        const uint2 w = *reinterpret_cast<const uint2*>(src + (g & 1) * 8);
+                        v[j] = make_uint4(w.x, w.y, 0u, 0u);
+                    }
+                }
+                if (left[t] < 16) {
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][2 * w + h], a0, a1, a2, a3, pf[nt][0], pf[nt][1]);
+                    for (int j = 0; j < 4; ++j)
+                        if (2 * c + (j & 1) + 8 * (j >> 1) >= left[t]) v[j] = make_uint4(0u, 0u, 0u, 0u);
+                }
+#pragma unroll
+                for (int w = 0; w < V_BYTES / 4; ++w) {
+                    const uint32_t x0 = word(v[0], w), x1 = word(v[1], w), y0 = word(v[2], w), y1 = word(v[3], w);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t a0, a1, a2, a3;
+                        entries_to_half<E4M3>(__byte_perm(x0, x1, h == 0 ? 0x5140 : 0x7362), a0, a1);
+                        entries_to_half<E4M3>(__byte_perm(y0, y1, h == 0 ? 0x5140 : 0x7362), a2, a3);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][2 * w + h], a0, a1, a2, a3, pf[t][nt][0], pf[t][nt][1]);
+                    }
                 }
             }
         };
-        // two tiles in flight: one is loaded while the other is used; a page's number is asked for a unit earlier still
-        Tile<D> t0, t1;
-        int page0 = page_of(u0), page1 = page_of(u0 + 1);
-        load(t0, u0, page0);
-        for (int u = u0; u < u1; u += 2) {
-            page0 = page_of(u + 2);
-            load(t1, u + 1, page1);
-            compute(t0);
-            page1 = page_of(u + 3);
-            load(t0, u + 2, page0);
-            compute(t1);
+        for (int u = u0, stage = 0; u < u1; ++u) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(R::STAGES - 2) : "memory");
+            __syncwarp();                                    // the tiles are there for all lanes, and all have used those before
+            const Pages after = pages_of(far + CT_UNIT);
+            ask(far, stage == 0 ? R::STAGES - 1 : stage - 1, page);
+            page = after;
+            far += CT_UNIT;
+            compute(key, ring + stage * R::STAGE);
+            key += CT_UNIT;
+            stage = stage + 1 == R::STAGES ? 0 : stage + 1;
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();                                     // merge_o lies over the rings
 
         // ---- the four warps' results are added in smem, in their order
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
+                if (most[nt][e] < 0.f) m[nt][e] = -INFINITY;
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], d);
                 if (g == 0) {
@@ -396,31 +512,20 @@ __global__ void __launch_bounds__(CT_THREADS, NT == 1 ? 4 : 3) cache_attn_kernel
                 // a row without a maximum saw nothing (sum 0) or only NaN (sum NaN, which has to come out)
                 weight[nt][e] = m[nt][e] == -INFINITY ? l[nt][e] : fast_exp2(m[nt][e] - top) * v_ref;
             }
-        for (int w = 0; w < CT_WARPS; ++w) {
-            if (warp == w) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float* dst = &merge_o[nt * 8 + 2 * c + e][g * 2 * MT];
+            for (int e = 0; e < 2; ++e) {
+                float* dst = &merge_o[warp * ROWS + nt * 8 + 2 * c + e][g * 2 * MT];
+                const float f = weight[nt][e];
 #pragma unroll
-                        for (int i = 0; i < 2 * MT; i += 4) {
-                            // d = g * 2 MT + i: m-tile i / 2, first row or second
-                            float4 x = make_float4(o[nt][i / 2][e], o[nt][i / 2][2 + e], o[nt][i / 2 + 1][e], o[nt][i / 2 + 1][2 + e]);
-                            const float f = weight[nt][e];
-                            x = f == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
-                            if (w > 0) {
-                                const float4 y = *reinterpret_cast<const float4*>(dst + i);
-                                x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
-                            }
-                            *reinterpret_cast<float4*>(dst + i) = x;
-                        }
-                    }
+                for (int i = 0; i < 2 * MT; i += 4)          // d = g * 2 MT + i: m-tile i / 2, first row or second
+                    *reinterpret_cast<float4*>(dst + i) = f == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                                                   : make_float4(o[nt][i / 2][e] * f, o[nt][i / 2][2 + e] * f, o[nt][i / 2 + 1][e] * f, o[nt][i / 2 + 1][2 + e] * f);
             }
-            __syncthreads();
-        }
-        const bool whole = u0 == 0 && u1 == span.units;
-        float* part = p.workspace + (static_cast<size_t>(blockIdx.x) * 2 + (u0 == 0 ? 1 : 0)) * (ROWS * (D + 2));
+        __syncthreads();
+        const bool whole = pieces == 1;
+        float* part = p.workspace + static_cast<size_t>(blockIdx.x) * (ROWS * (D + 2));
         for (int i = threadIdx.x; i < ROWS * (D / 8); i += CT_THREADS) {
             const int r = i / (D / 8), d = i % (D / 8) * 8;
             if (row0 + r >= p.rows) continue;
@@ -429,7 +534,13 @@ __global__ void __launch_bounds__(CT_THREADS, NT == 1 ? 4 : 3) cache_attn_kernel
             float sum = 0.f;
             for (int w = 0; w < CT_WARPS; ++w)
                 sum += merge_m[w][r] > -INFINITY ? merge_l[w][r] * fast_exp2(merge_m[w][r] - top) : merge_l[w][r];
-            const float4 x = *reinterpret_cast<const float4*>(&merge_o[r][d]), y = *reinterpret_cast<const float4*>(&merge_o[r][d + 4]);
+            float4 x = *reinterpret_cast<const float4*>(&merge_o[r][d]), y = *reinterpret_cast<const float4*>(&merge_o[r][d + 4]);
+#pragma unroll
+            for (int w = 1; w < CT_WARPS; ++w) {
+                const float4 xw = *reinterpret_cast<const float4*>(&merge_o[w * ROWS + r][d]), yw = *reinterpret_cast<const float4*>(&merge_o[w * ROWS + r][d + 4]);
+                x = make_float4(x.x + xw.x, x.y + xw.y, x.z + xw.z, x.w + xw.w);
+                y = make_float4(y.x + yw.x, y.y + yw.y, y.z + yw.z, y.w + yw.w);
+            }
             if (whole) {
                 const float inv = sum != 0.f ? 1.f / sum : 0.f;
                 uint4 u;
@@ -447,81 +558,102 @@ __global__ void __launch_bounds__(CT_THREADS, NT == 1 ? 4 : 3) cache_attn_kernel
                 }
             }
         }
-        __syncthreads();                                     // smem is free again
-        at += u1 - u0;
     }
 }
 
-// Adds the parts of the (request, K/V head, row group)s that more than one block worked on, and writes the zeros of empty requests.
+// Adds the parts of what more than one block worked on, a row a block, in the order of the blocks within each warp; and writes the zeros of
+// empty requests.
 template <int NT, int D>
-__global__ void __launch_bounds__(CT_THREADS) cache_attn_join_kernel(const CacheAttnParams p, int launched) {
-    constexpr int ROWS = NT * 8, EACH = D / 32;
-    __shared__ long long sums[CT_WARPS];
+__global__ void __launch_bounds__(CT_THREADS) cache_attn_join_kernel(const CacheAttnParams p) {
+    constexpr int ROWS = NT * 8, EACH = D / 32, AHEAD = 8;
+    __shared__ float add_o[CT_WARPS][D], add_l[CT_WARPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     grid_dependency_wait();
     grid_launch_dependents();
     if (__syncthreads_or(failure_reported(p.status))) return;
     const int pairs = p.kv_heads * p.row_groups;
-    const int b = blockIdx.x / pairs, pair = blockIdx.x % pairs, kv = pair / p.row_groups, row0 = (pair % p.row_groups) * ROWS;
-    long long total = 0, base = 0;
-    for (int i = threadIdx.x; i < p.requests; i += CT_THREADS) {
-        const int units = span_of(p, i).units;
-        total += units;
-        if (i < b) base += units;
-    }
-    total = block_sum(total, sums) * pairs;
-    base = block_sum(base, sums) * pairs;
-    const int blocks = blocks_at_work(total, launched);
-    const int units = span_of(p, b).units;
-    const long long from = base + static_cast<long long>(pair) * units, to = from + units;
-    // blocks whose stretch meets [from, to)
-    int i0 = 0, i1 = 0;
-    if (units > 0) {
-        i0 = static_cast<int>(from * blocks / total);
-        while (i0 > 0 && stretch(total, i0, blocks) > from) --i0;
-        while (stretch(total, i0 + 1, blocks) <= from) ++i0;
-        i1 = i0 + 1;
-        while (i1 < blocks && stretch(total, i1, blocks) < to) ++i1;
-        if (i1 == i0 + 1) return;                            // one block had all of it
-    }
-    for (int r = warp; r < ROWS && row0 + r < p.rows; r += CT_WARPS) {
-        auto part = [&](int i) { return p.workspace + (static_cast<size_t>(i) * 2 + (stretch(total, i, blocks) <= from ? 1 : 0)) * (ROWS * (D + 2)); };
-        float top = -INFINITY, sum = 0.f, o[EACH];
+    const int b = blockIdx.x / pairs, pair = blockIdx.x % pairs, kv = pair / p.row_groups, row = (pair % p.row_groups) * ROWS + blockIdx.y;
+    if (row >= p.rows) return;
+    const int2 parts = __ldca(p.parts + blockIdx.x);
+    const bool empty = span_of(p, b).units == 0;             // (its entry was not written)
+    if (!empty && parts.y == 1) return;                      // one block had all of it
+    const int count = empty ? 0 : parts.y, r = blockIdx.y;
+    auto part = [&](int i) { return p.workspace + static_cast<size_t>(parts.x + i) * (ROWS * (D + 2)); };
+    float top = -INFINITY, sum = 0.f, o[EACH];
 #pragma unroll
-        for (int e = 0; e < EACH; ++e) o[e] = 0.f;
-        for (int i = i0 + lane; i < i1; i += 32) top = fmaxf(top, __ldca(part(i) + r));
+    for (int e = 0; e < EACH; ++e) o[e] = 0.f;
+    for (int i = lane; i < count; i += 32) top = fmaxf(top, __ldca(part(i) + r));
 #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        for (int i = i0; i < i1; ++i) {
-            const float* x = part(i);
-            const float m = __ldca(x + r), f = m > -INFINITY ? fast_exp2(m - top) : 1.f;
-            sum += __ldca(x + ROWS + r) * f;
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    for (int i0 = warp; i0 < count; i0 += CT_WARPS * AHEAD) {
+        float m[AHEAD], l[AHEAD], x[AHEAD][EACH];
 #pragma unroll
-            for (int e = 0; e < EACH; ++e) o[e] += f * __ldca(x + 2 * ROWS + r * D + lane * EACH + e);
+        for (int j = 0; j < AHEAD; ++j) {
+            const int i = i0 + j * CT_WARPS;
+            m[j] = -INFINITY;
+            l[j] = 0.f;
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) x[j][e] = 0.f;
+            if (i < count) {
+                const float* at = part(i);
+                m[j] = __ldca(at + r);
+                l[j] = __ldca(at + ROWS + r);
+                at += 2 * ROWS + r * D + lane * EACH;
+                if constexpr (EACH == 4) {
+                    const float4 v = __ldca(reinterpret_cast<const float4*>(at));
+                    x[j][0] = v.x; x[j][1] = v.y; x[j][2] = v.z; x[j][3] = v.w;
+                } else {
+                    const float2 v = __ldca(reinterpret_cast<const float2*>(at));
+                    x[j][0] = v.x; x[j][1] = v.y;
+                }
+            }
         }
-        const float inv = sum != 0.f ? 1.f / sum : 0.f;
-        uint16_t* dst = static_cast<uint16_t*>(p.out) + b * p.out_stride[0] + ((row0 + r) / p.group) * p.out_stride[1] + (kv * p.group + (row0 + r) % p.group) * p.out_stride[2] + lane * EACH;
 #pragma unroll
-        for (int e = 0; e < EACH; e += 2) {
-            const float x = o[e] * inv, y = o[e + 1] * inv;
-            *reinterpret_cast<uint32_t*>(dst + e) = p.bf16 ? pack_pair<true>(x, y) : pack_pair<false>(x, y);
+        for (int j = 0; j < AHEAD; ++j) {
+            const float f = m[j] > -INFINITY ? fast_exp2(m[j] - top) : 1.f;  // (a part that saw nothing is 0, or NaN)
+            sum += l[j] * f;
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) o[e] += x[j][e] * f;
         }
+    }
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) add_o[warp][lane * EACH + e] = o[e];
+    if (lane == 0) add_l[warp] = sum;
+    __syncthreads();
+    if (threadIdx.x < D / 2) {
+        const int d = threadIdx.x * 2;
+        float l = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+        for (int w = 0; w < CT_WARPS; ++w) {
+            l += add_l[w];
+            x += add_o[w][d];
+            y += add_o[w][d + 1];
+        }
+        const float inv = l != 0.f ? 1.f / l : 0.f;
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + b * p.out_stride[0] + (row / p.group) * p.out_stride[1] + (kv * p.group + row % p.group) * p.out_stride[2] + d;
+        *reinterpret_cast<uint32_t*>(dst) = p.bf16 ? pack_pair<true>(x * inv, y * inv) : pack_pair<false>(x * inv, y * inv);
     }
 }
 
 struct Shape {
     int rows, nt, row_groups;
-    long long blocks;
+    int resident;
+    long long blocks, joins, units;          // joins: (request, K/V head, row group)s; units: at most
 };
-// row tiles of 8: one up to 8 rows, else two at a time; blocks: what the GPU holds at once, no more than there can be units
+// row tiles of 8: one up to 8 rows, else two at a time; blocks: as many as there may be pieces (piece_units)
 Shape shape_of(int requests, int tokens, int heads, int kv_heads, int page_size, int table_width) {
     Shape s;
     s.rows = tokens * (heads / kv_heads);
     s.nt = s.rows <= 8 ? 1 : 2;
     s.row_groups = (s.rows + 8 * s.nt - 1) / (8 * s.nt);
-    const long long units = static_cast<long long>(requests) * kv_heads * s.row_groups * ((static_cast<long long>(table_width) * page_size + CT_UNIT - 1) / CT_UNIT);
-    s.blocks = static_cast<long long>(sm_count()) * (s.nt == 1 ? 4 : 3);
-    if (s.blocks > units) s.blocks = units > 0 ? units : 1;
+    s.joins = static_cast<long long>(requests) * kv_heads * s.row_groups;
+    s.units = s.joins * ((static_cast<long long>(table_width) * page_size + CT_UNIT - 1) / CT_UNIT);
+    s.resident = sm_count() * (s.nt == 1 ? CT_BLOCKS : 2);
+    long long pieces = s.units / CT_LONG;
+    if (pieces > static_cast<long long>(s.resident) * CT_WAVES) pieces = static_cast<long long>(s.resident) * CT_WAVES;
+    if (pieces < s.resident) pieces = s.resident;
+    s.blocks = pieces + s.joins;
+    if (s.blocks > s.units) s.blocks = s.units > 0 ? s.units : 1;
     return s;
 }
 
@@ -533,7 +665,7 @@ using namespace stof;
 extern "C" size_t stof_cache_attn_workspace_bytes(int requests, int tokens, int heads, int kv_heads, int head_dim, int page_size, int table_width) {
     if (requests <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || page_size <= 0 || table_width < 0) return 0;
     const Shape s = shape_of(requests, tokens, heads, kv_heads, page_size, table_width);
-    return static_cast<size_t>(s.blocks) * 2 * (8 * s.nt) * (static_cast<size_t>(head_dim) + 2) * sizeof(float);
+    return (static_cast<size_t>(s.joins) * sizeof(int2) + 15) / 16 * 16 + static_cast<size_t>(s.blocks) * (8 * s.nt) * (static_cast<size_t>(head_dim) + 2) * sizeof(float);
 }
 
 extern "C" int stof_cache_attn(const void* q, void* out, int dtype, const long long q_strides[3], const long long out_strides[3], const void* k_pages,
@@ -547,7 +679,7 @@ extern "C" int stof_cache_attn(const void* q, void* out, int dtype, const long l
     STOF_REQUIRE(page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128, "cache_attn: page size %d not in {16, 32, 64, 128}", page_size);
     STOF_REQUIRE(cache_dtype == STOF_DTYPE_INT8 || cache_dtype == STOF_DTYPE_E4M3, "cache_attn: cache entries must be int8 or e4m3");
     STOF_REQUIRE(dtype == STOF_DTYPE_F16 || dtype == STOF_DTYPE_BF16, "cache_attn: queries must be fp16 or bf16");
-    STOF_REQUIRE(static_cast<long long>(table_width) * page_size < (1ll << 31) - 256, "cache_attn: a row of the block table spans more than 2^31 tokens");
+    STOF_REQUIRE(static_cast<long long>(table_width) * page_size <= (1ll << 30), "cache_attn: a row of the block table spans more than 2^30 tokens");
     STOF_REQUIRE(rules != nullptr, "cache_attn: null rules");
     STOF_REQUIRE(rules->softmax_scale > 0.f && rules->softmax_scale < INFINITY, "cache_attn: softmax_scale must be positive and finite");
     STOF_REQUIRE(rules->softcap >= 0.f && rules->softcap < INFINITY, "cache_attn: softcap must not be negative");
@@ -567,8 +699,7 @@ extern "C" int stof_cache_attn(const void* q, void* out, int dtype, const long l
         set_error("cache_attn: workspace of %zu bytes, need %zu", workspace == nullptr ? static_cast<size_t>(0) : workspace_bytes, need);
         return STOF_E_WORKSPACE;
     }
-    const long long joins = static_cast<long long>(requests) * kv_heads * s.row_groups;
-    STOF_REQUIRE(joins < (1ll << 31), "cache_attn: requests * K/V heads * row groups beyond 2^31");
+    STOF_REQUIRE(s.joins < (1ll << 31) && s.units < (1ll << 31), "cache_attn: requests * K/V heads * row groups * units of %d keys beyond 2^31", CT_UNIT);
     CacheAttnParams p;
     p.q = q; p.out = out;
     for (int i = 0; i < 3; ++i) {
@@ -578,18 +709,21 @@ extern "C" int stof_cache_attn(const void* q, void* out, int dtype, const long l
     p.k_pages = k_pages; p.v_pages = v_pages; p.k_scales = k_scales; p.v_scales = v_scales;
     p.block_table = block_table; p.table_stride = table_stride; p.lengths = lengths;
     p.slopes = rules->slopes; p.distance_bias = rules->distance_bias; p.radius = rules->bias_radius;
-    p.workspace = static_cast<float*>(workspace); p.status = status_dev;
+    p.parts = static_cast<int2*>(workspace);
+    p.workspace = reinterpret_cast<float*>(static_cast<char*>(workspace) + (static_cast<size_t>(s.joins) * sizeof(int2) + 15) / 16 * 16); p.status = status_dev;
     p.scale = rules->softmax_scale; p.softcap = rules->softcap; p.window = rules->window;
     p.requests = requests; p.tokens = tokens; p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads;
-    p.rows = s.rows; p.row_groups = s.row_groups;
+    p.rows = s.rows; p.row_groups = s.row_groups; p.resident = s.resident;
     p.table_width = table_width; p.page_count = pages; p.bf16 = dtype == STOF_DTYPE_BF16;
     p.page_shift = 0;
     while ((1 << p.page_shift) < page_size) ++p.page_shift;
     auto launch = [&](auto kernel, auto join) -> int {
-        LaunchConfig lc(dim3(static_cast<unsigned>(s.blocks)), CT_THREADS, 0, stream);
+        const int smem = CT_WARPS * (head_dim == 64 ? Ring<64>::BYTES : Ring<128>::BYTES);
+        STOF_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        LaunchConfig lc(dim3(static_cast<unsigned>(s.blocks)), CT_THREADS, static_cast<size_t>(smem), stream);
         STOF_CUDA(cudaLaunchKernelEx(&lc.cfg, kernel, p));
-        LaunchConfig lj(dim3(static_cast<unsigned>(joins)), CT_THREADS, 0, stream);
-        STOF_CUDA(cudaLaunchKernelEx(&lj.cfg, join, p, static_cast<int>(s.blocks)));
+        LaunchConfig lj(dim3(static_cast<unsigned>(s.joins), static_cast<unsigned>(s.rows < 8 * s.nt ? s.rows : 8 * s.nt)), CT_THREADS, 0, stream);
+        STOF_CUDA(cudaLaunchKernelEx(&lj.cfg, join, p));
         return STOF_OK;
     };
     const bool e4m3 = cache_dtype == STOF_DTYPE_E4M3;

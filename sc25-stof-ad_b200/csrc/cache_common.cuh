@@ -7,21 +7,27 @@
 
 namespace stof {
 
-// Two entries (the low 16 bits of `w`) as fp16 numbers; both types' entries are exact in fp16.
+// Four entries as fp16 numbers (exact for both types): the first two and the last two.
 template <bool E4M3>
-__device__ __forceinline__ uint32_t entries_to_half2(uint32_t w);
-template <>
-__device__ __forceinline__ uint32_t entries_to_half2<true>(uint32_t w) {
-    uint32_t h;
-    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(h) : "r"(w));
-    return h;
+__device__ __forceinline__ void entries_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    if constexpr (E4M3) {
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+    } else {
+        // 1024 + (entry + 128) is the fp16 number with the biased byte as its low mantissa bits
+        const uint32_t biased = w ^ 0x80808080u;
+        const __half2 off(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+        const uint32_t a = __byte_perm(biased, 0x64646464u, 0x4140), b = __byte_perm(biased, 0x64646464u, 0x4342);
+        const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off), y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+        lo = *reinterpret_cast<const uint32_t*>(&x);
+        hi = *reinterpret_cast<const uint32_t*>(&y);
+    }
 }
-// int8: 1024 + (entry + 128) is the fp16 number with the biased byte as its low mantissa bits
-template <>
-__device__ __forceinline__ uint32_t entries_to_half2<false>(uint32_t w) {
-    const uint32_t biased = __byte_perm(w ^ 0x8080u, 0x64646464u, 0x4140);
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&biased), __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t*>(&h);
+
+// 1 / x to a unit in the last place
+__device__ __forceinline__ float fast_reciprocal(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 template <bool E4M3>

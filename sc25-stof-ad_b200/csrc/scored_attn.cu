@@ -68,7 +68,7 @@ __device__ __forceinline__ float2 tanh_near(float2 u) {
     return mul2(p, u);
 }
 // tanh(u) = 1 - 2 / (1 + e^(2u)) for any u
-__device__ __forceinline__ float tanh_any(float u) { return 1.f - 2.f * __frcp_rn(1.f + fast_exp2(u * (2.f * SA_LOG2E))); }
+__device__ __forceinline__ float tanh_any(float u) { return 1.f - 2.f * fast_reciprocal(1.f + fast_exp2(u * (2.f * SA_LOG2E))); }
 
 template <int D>
 __device__ __noinline__ void rescale_o(uint32_t t_o, float alpha) {

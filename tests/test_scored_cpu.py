@@ -71,7 +71,7 @@ def _cache(lib, rules=None, dtype=0, cache_dtype=3, pages=4, page=16, kv_heads=1
     (dict(dim=80), -1, b"head_dim"), (dict(page=24), -1, b"page size"), (dict(page=256), -1, b"page size"), (dict(heads=3, kv_heads=2), -1, b"multiple"),
     (dict(dtype=3), -1, b"fp16 or bf16"), (dict(cache_dtype=0), -1, b"int8 or e4m3"), (dict(stride=1), -1, b"row stride"), (dict(table=None), -1, b"block table"),
     (dict(workspace=None), -3, b"workspace"), (dict(nbytes=64), -3, b"workspace"), (dict(st=4), -1, b"strides"), (dict(q=ctypes.c_void_p(8)), -1, b"16-byte"),
-    (dict(width=1 << 27, stride=1 << 27), -1, b"2^31"), (dict(rules=dict(window=-2)), -1, b"window"), (dict(rules=dict(softcap=-2.0)), -1, b"softcap"),
+    (dict(width=1 << 27, stride=1 << 27), -1, b"2^30"), (dict(rules=dict(window=-2)), -1, b"window"), (dict(rules=dict(softcap=-2.0)), -1, b"softcap"),
     (dict(rules=dict(softmax_scale=-1.0)), -1, b"softmax_scale"), (dict(rules=dict(distance_bias=16, bias_radius=5000)), -1, b"radius"), (dict(tokens=-1), -1, b"bad shape")])
 def test_cache_attn_refusals(lib, kw, code, text):
     kw = dict(kw)
