@@ -1,10 +1,14 @@
 // New keys and values into the slots of a paged 8-bit cache, one scale per page and head (HBM-bound for prompts, latency-bound for
 // the tokens of a step).
 //
+// What bounds it: the chain slots -> rows -> maximum -> entries, of which the SM has to hold many at once: 18000 tokens of 8 heads of 128
+// (111 MB) take 24 us, 4.6 TB/s, with eight blocks of 64 registers on an SM; 29 with six of 80, 30 with ten of 48 that spill, 31 with twice
+// the warps for a run, 97 with keys and values in blocks of their own and runs held whole (168 registers).
+//
 // A run is a stretch of tokens whose slots follow one another inside a page; its scale needs the largest magnitude of all its
 // rows, so a run belongs to one warp (up to four tokens) or one thread block: the rows are read once, held in registers as they
-// came, reduced, and written as entries.  Runs are found from the slots alone: a thread block looks at a few neighbouring tokens of
-// one head and serves the runs that begin there.
+// came, reduced, and written as entries.  Runs are found from the slots alone: a thread block looks at a few neighbouring tokens for
+// one head and serves the runs that begin there; every warp finds them for itself, from ballots, without a barrier.
 #include "cache_common.cuh"
 #include "stof_host.h"
 #include "stof_ptx.cuh"
@@ -14,7 +18,7 @@ namespace {
 
 constexpr int CA_WARPS = 4;
 constexpr int CA_SHORT = 4;                  // tokens up to which a warp serves a run alone
-constexpr int CA_MAX_CHUNK = 16;
+constexpr int CA_MAX_CHUNK = 32;
 
 struct AppendParams {
     void* pages[2];
@@ -47,112 +51,153 @@ struct Rows {
     }
 };
 
-// One run: tokens [token, token + n) into rows [row, row + n) of a page.  `part` of `parts` warps work on it (1: this warp alone),
-// NV loads hold a warp's share.
+// One run: tokens [token, token + n) into rows [row, row + n) of a page, keys and values.  `part` of `parts` warps work on it (1: this warp
+// alone).  NV loads a side hold a warp's share of a pass; a run of more than one pass is read twice, the second time from cache.
 template <bool BF16, bool E4M3, int D, int NV>
-__device__ __forceinline__ void write_run(const AppendParams& p, int side, int head, int token, int n, int page, int row, int part, int parts, float* shared) {
+__device__ __forceinline__ void write_run(const AppendParams& p, int head, int token, int n, int page, int row, int part, int parts, float (*shared)[2]) {
     using R = Rows<BF16, E4M3, D>;
     const int lane = threadIdx.x & 31, sub = lane / R::LANES, col = lane % R::LANES;
-    const uint16_t* x = static_cast<const uint16_t*>(p.x[side]) + head * p.head_stride[side] + col * 8;
     const long long at = static_cast<long long>(page) * p.heads + head;
-    uint8_t* entries = static_cast<uint8_t*>(p.pages[side]) + ((at << p.page_shift) + row) * D;
-    float* scale = p.scales[side] + at;
-    uint4 v[NV];
-    float top = 0.f;
+    const int pass = NV * parts * R::EACH;                   // rows of a pass
+    uint4 v[2][NV];
+    auto load = [&](int from) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int r = (i * parts + part) * R::EACH + sub;
-        v[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (r < n) v[i] = __ldca(reinterpret_cast<const uint4*>(x + (token + r) * p.token_stride[side]));
+        for (int side = 0; side < 2; ++side) {
+            const uint16_t* x = static_cast<const uint16_t*>(p.x[side]) + head * p.head_stride[side] + col * 8;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int r = from + (i * parts + part) * R::EACH + sub;
+                v[side][i] = make_uint4(0u, 0u, 0u, 0u);
+                if (r < n) v[side][i] = __ldca(reinterpret_cast<const uint4*>(x + (token + r) * p.token_stride[side]));
+            }
+        }
+    };
+    float old[2] = {0.f, 0.f}, top[2] = {0.f, 0.f};
+    int from = 0;
+    while (true) {
+        load(from);
+        if (from == 0 && row > 0) {
+            old[0] = p.scales[0][at];
+            old[1] = p.scales[1][at];
+        }
+#pragma unroll
+        for (int side = 0; side < 2; ++side)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) top[side] = fmaxf(top[side], R::magnitude(v[side][i]));
+        if (from + pass >= n) break;
+        from += pass;
     }
-    const float old = row > 0 ? *scale : 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) top = fmaxf(top, R::magnitude(v[i]));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int o = 16; o > 0; o >>= 1) {
+        top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
+        top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], o));
+    }
     if (parts > 1) {
-        if (lane == 0) shared[part] = top;
-        __syncthreads();                                     // (and everyone has read the old scale)
-        top = fmaxf(fmaxf(shared[0], shared[1]), fmaxf(shared[2], shared[3]));
-    }
-    float now = top * (1.0f / entry_max<E4M3>());
-    if (now < 1.17549435e-38f) now = 0.f;
-    now = fmaxf(now, old);
-    const float inv = now > 0.f ? 1.0f / now : 0.f;
-    if (part == 0 && lane == 0) *scale = now;
+        if (lane < 2) shared[part][lane] = lane == 0 ? top[0] : top[1];
+        __syncthreads();                                     // (and everyone has read the old scales)
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int r = (i * parts + part) * R::EACH + sub;
-        if (r < n) *reinterpret_cast<uint2*>(entries + static_cast<size_t>(r) * D + col * 8) = R::entries(v[i], inv);
+        for (int w = 0; w < CA_WARPS; ++w) {
+            top[0] = fmaxf(top[0], shared[w][0]);
+            top[1] = fmaxf(top[1], shared[w][1]);
+        }
     }
-    if (row > 0 && now > old) {                              // the entries in front of the run, rounded again to the new scale
-        const float ratio = old / now;
-        uint4* front = reinterpret_cast<uint4*>(entries - static_cast<size_t>(row) * D);
+    float inv[2], ratio[2];
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+        float now = top[side] * (1.0f / entry_max<E4M3>());
+        if (now < 1.17549435e-38f) now = 0.f;
+        now = fmaxf(now, old[side]);
+        inv[side] = now > 0.f ? 1.0f / now : 0.f;
+        ratio[side] = row > 0 && now > old[side] ? old[side] / now : 1.f;    // 1: what is in front of the run stays
+        if (part == 0 && lane == 0) p.scales[side][at] = now;
+    }
+    const bool again[2] = {ratio[0] != 1.f, ratio[1] != 1.f};
+    while (true) {                                           // from the last pass, which is still there, to the first
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            uint8_t* entries = static_cast<uint8_t*>(p.pages[side]) + ((at << p.page_shift) + row) * D + col * 8;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int r = from + (i * parts + part) * R::EACH + sub;
+                if (r < n) *reinterpret_cast<uint2*>(entries + static_cast<size_t>(r) * D) = R::entries(v[side][i], inv[side]);
+            }
+        }
+        if (from == 0) break;
+        from -= pass;
+        load(from);
+    }
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+        if (!again[side]) continue;                          // the entries in front of the run, rounded again to the new scale
+        uint4* front = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.pages[side]) + (at << p.page_shift) * D);
         for (int i = part * 32 + lane; i < row * D / 16; i += parts * 32) {
             const uint4 u = front[i];
-            auto again = [&](uint32_t w) {
+            auto round_again = [&](uint32_t w) {
                 uint32_t lo, hi;
                 entries_to_half<E4M3>(w, lo, hi);
                 const float2 a = unpack_pair<false>(lo), b = unpack_pair<false>(hi);
-                return quantise2<E4M3>(a.x, a.y, ratio) | (quantise2<E4M3>(b.x, b.y, ratio) << 16);
+                return quantise2<E4M3>(a.x, a.y, ratio[side]) | (quantise2<E4M3>(b.x, b.y, ratio[side]) << 16);
             };
-            front[i] = make_uint4(again(u.x), again(u.y), again(u.z), again(u.w));
+            front[i] = make_uint4(round_again(u.x), round_again(u.y), round_again(u.z), round_again(u.w));
         }
     }
 }
 
 template <bool BF16, bool E4M3, int D>
-__global__ void __launch_bounds__(CA_WARPS * 32) cache_append_kernel(const AppendParams p) {
-    __shared__ int run_token[CA_MAX_CHUNK], run_length[CA_MAX_CHUNK], runs;
-    __shared__ float shared[CA_WARPS];
+__global__ void __launch_bounds__(CA_WARPS * 32, 8) cache_append_kernel(const AppendParams p) {
+    __shared__ float shared[CA_WARPS][2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int head = blockIdx.y, side = blockIdx.z, page = 1 << p.page_shift;
+    const int head = blockIdx.y, page = 1 << p.page_shift;
     grid_dependency_wait();
     grid_launch_dependents();
+    // every warp looks at the chunk's tokens and at as many behind them as a run can take: where a run begins (or nothing is written)
+    constexpr int SEEN = 1 + 128 / 32;
+    const int t0 = blockIdx.x * p.chunk;
+    int slot[SEEN];
+#pragma unroll
+    for (int i = 0; i < SEEN; ++i) slot[i] = t0 + 32 * i + lane < p.tokens ? p.slots[t0 + 32 * i + lane] : -1;
+    const int in_front = t0 > 0 ? p.slots[t0 - 1] : -2;
     if (__syncthreads_or(failure_reported(p.status))) return;
     const long long slot_end = static_cast<long long>(p.page_count) << p.page_shift;
-    if (warp == 0) {
-        const int t = blockIdx.x * p.chunk + lane;
-        bool first = false;
-        if (lane < p.chunk && t < p.tokens) {
-            const int s = p.slots[t];
-            first = s >= 0 && (t == 0 || s != p.slots[t - 1] + 1 || (s & (page - 1)) == 0);
-            if (first && s >= slot_end) {
-                if (p.status != nullptr) atomicCAS(p.status, 0, STATUS_BAD_INDEX);
-                first = false;
+    unsigned begins[SEEN], good = 0;
+#pragma unroll
+    for (int i = 0; i < SEEN; ++i) {
+        int before = __shfl_up_sync(0xffffffffu, slot[i], 1);
+        const int carried = i > 0 ? __shfl_sync(0xffffffffu, slot[i > 0 ? i - 1 : 0], 31) : in_front;
+        if (lane == 0) before = carried;
+        begins[i] = __ballot_sync(0xffffffffu, slot[i] < 0 || slot[i] != before + 1 || (slot[i] & (page - 1)) == 0);
+        if (i == 0) {
+            good = __ballot_sync(0xffffffffu, lane < p.chunk && slot[0] >= 0 && slot[0] < slot_end);
+            if (lane < p.chunk && slot[0] >= slot_end && p.status != nullptr) atomicCAS(p.status, 0, STATUS_BAD_INDEX);
+        }
+    }
+    int found = 0;
+    for (unsigned leads = begins[0] & good; leads != 0; leads &= leads - 1) {
+        const int at = __ffs(leads) - 1;
+        // to the next beginning
+        int n = -at;
+        const unsigned later = at == 31 ? 0u : begins[0] & ~((2u << at) - 1u);
+        if (later != 0) {
+            n += __ffs(later) - 1;
+        } else {
+            n += 32;
+#pragma unroll
+            for (int i = 1; i < SEEN; ++i) {
+                if (begins[i] != 0) {
+                    n += __ffs(begins[i]) - 1;
+                    break;
+                }
+                n += 32;
             }
         }
-        const unsigned found = __ballot_sync(0xffffffffu, first);
-        if (first) run_token[__popc(found & ((1u << lane) - 1u))] = t;
-        if (lane == 0) runs = __popc(found);
-    }
-    __syncthreads();
-    const int count = runs;
-    for (int i = warp; i < count; i += CA_WARPS) {           // lengths, and the short runs at once
-        const int t = run_token[i], s = p.slots[t], most = min(page - (s & (page - 1)), p.tokens - t);
-        int n = 1;
-        for (int at = 1; at < most; at += 32) {
-            const bool on = at + lane < most && p.slots[t + at + lane] == s + at + lane;
-            const unsigned run = __ballot_sync(0xffffffffu, on);
-            const int more = run == 0xffffffffu ? 32 : __ffs(~run) - 1;
-            n += more;
-            if (more < 32) break;
+        const int s = __shfl_sync(0xffffffffu, slot[0], at);
+        if (n <= CA_SHORT) {                                 // a warp each, in turn
+            if (found++ % CA_WARPS == warp)
+                write_run<BF16, E4M3, D, CA_SHORT / Rows<BF16, E4M3, D>::EACH>(p, head, t0 + at, n, s >> p.page_shift, s & (page - 1), 0, 1, shared);
+        } else {
+            __syncthreads();                                 // `shared` is free
+            write_run<BF16, E4M3, D, 32 / (CA_WARPS * Rows<BF16, E4M3, D>::EACH)>(p, head, t0 + at, n, s >> p.page_shift, s & (page - 1), warp, CA_WARPS, shared);
         }
-        if (lane == 0) run_length[i] = n;
-        if (n <= CA_SHORT)
-            write_run<BF16, E4M3, D, CA_SHORT / Rows<BF16, E4M3, D>::EACH>(p, side, head, t, n, s >> p.page_shift, s & (page - 1), 0, 1, shared);
-    }
-    __syncthreads();
-    for (int i = 0; i < count; ++i) {
-        const int n = run_length[i];
-        if (n <= CA_SHORT) continue;
-        const int t = run_token[i], s = p.slots[t];
-        constexpr int SHARE = CA_WARPS * Rows<BF16, E4M3, D>::EACH;      // rows of one load of the whole block
-        if (n <= 32)
-            write_run<BF16, E4M3, D, 32 / SHARE>(p, side, head, t, n, s >> p.page_shift, s & (page - 1), warp, CA_WARPS, shared);
-        else
-            write_run<BF16, E4M3, D, 128 / SHARE>(p, side, head, t, n, s >> p.page_shift, s & (page - 1), warp, CA_WARPS, shared);
-        __syncthreads();                                     // `shared` is free again
     }
 }
 
@@ -184,7 +229,7 @@ extern "C" int stof_cache_append(void* k_pages, void* v_pages, float* k_scales, 
     while ((1 << p.page_shift) < page_size) ++p.page_shift;
     // few tokens: a warp for every run; many: runs are as long as pages, and a block that finds none costs its launch
     p.chunk = tokens <= 1024 ? CA_WARPS : CA_MAX_CHUNK;
-    const dim3 grid(static_cast<unsigned>((tokens + p.chunk - 1) / p.chunk), static_cast<unsigned>(kv_heads), 2);
+    const dim3 grid(static_cast<unsigned>((tokens + p.chunk - 1) / p.chunk), static_cast<unsigned>(kv_heads));
     auto launch = [&](auto kernel) -> int {
         LaunchConfig lc(grid, CA_WARPS * 32, 0, stream);
         STOF_CUDA(cudaLaunchKernelEx(&lc.cfg, kernel, p));
