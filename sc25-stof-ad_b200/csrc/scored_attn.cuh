@@ -1,0 +1,671 @@
+// Attention whose scores are changed by a formula (tanh cap, distance bias) and masked by rules (causal, window, prefix, documents,
+// padding), for sm_100a: TMA-fed tcgen05 products with the accumulators in tensor memory, online softmax in registers.
+//
+// Per thread block one stretch of 128 query rows, or two (HALVES) that share every K/V tile of 128 keys.  Each half has its own S
+// (128 x 128 fp32 in tensor memory), P (16-bit numbers, also in tensor memory) and O (128 x D fp32), its own softmax warps - one row a
+// thread - and its own list of tiles: those that the rules leave anything of.  While one half's warps work on their scores the tensor
+// core serves the other half.
+//   warps 0..3 (and 4..7)   softmax of the half
+//   next warp               TMA producer: Q, then K and V tiles through a ring of two slots each
+//   last warp               tcgen05 issuer
+// Where tensor memory has room (OWN_P: all but two halves of D = 128) P lies beside S, and S = Q K^T of the next tile is issued as soon
+// as S has been read into registers; else P lies over S and the next product waits for O += P V.  P is handed over in two parts.
+// A tile is classified per warp (32 rows): nothing to mask, or masked by 128 bits a row.
+// What a call does not use is not in its kernel's loop (MODE): the loop a warp spends its time in has to fit the instruction caches.
+#pragma once
+#include <type_traits>
+
+#include "cache_common.cuh"
+#include "stof_host.h"
+#include "stof_ptx.cuh"
+
+namespace stof {
+
+constexpr int SA_T = 128;                    // rows of a half, keys of a tile
+constexpr int SA_PAD = 256;                  // the distance table in shared memory goes on for so long on both sides: a tile that meets the table needs no clamp
+constexpr float SA_RESCALE = 8.0f;           // log2 units by which a row's maximum may outgrow the reference of its P (P <= 2^8)
+constexpr float SA_LOG2E = 1.4426950408889634f;
+#ifndef SA_POLY_PAIRS
+#define SA_POLY_PAIRS 2                      // of every 8 pairs of exponentials, so many on the FMA pipe
+#endif
+enum { SA_PLAIN = 0, SA_CAP = 1, SA_ANY = 2 };       // what is done to scores: nothing, the cap alone, whatever the call asks for
+
+struct ScoredParams {
+    void* out;
+    long long out_stride[3];
+    const float *slopes, *distance_bias;
+    const int *documents, *prefix_lens, *key_lens;
+    long long documents_stride;
+    int* status;
+    float scale, softcap;
+    int causal, window, radius;
+    int batch, heads, group, q_len, k_len, q_tiles;
+    int slot_s[3], slot_h[3], slot_b[3];     // of q, k, v: which coordinate of the tensor map is the row, the head, the batch
+    int table_bytes, range_bytes;
+};
+
+// barriers, two of each (a half's, or a slot's): Q is there; S is there; parts 0 and 1 of P are there; S has been read; O is complete (OWN_P: up
+// to the last P, else the whole); slots
+enum { SB_Q = 0, SB_S = 2, SB_P0 = 4, SB_P1 = 6, SB_READ = 8, SB_O = 10, SB_FIX = 12, SB_K_FULL = 13, SB_K_EMPTY = 15, SB_V_FULL = 17, SB_V_EMPTY = 19, SB_COUNT = 21 };
+
+static __device__ __forceinline__ void load_tile(unsigned char* dst, const CUtensorMap* map, uint64_t* bar, int col, int row, int head, int batch, int slot_s, int slot_h) {
+    // the three outer coordinates are in the order of their strides
+    const int c1 = slot_s == 1 ? row : slot_h == 1 ? head : batch;
+    const int c2 = slot_s == 2 ? row : slot_h == 2 ? head : batch;
+    const int c3 = slot_s == 3 ? row : slot_h == 3 ? head : batch;
+    tma_load_4d(dst, map, bar, col, c1, c2, c3);
+}
+
+static __device__ __forceinline__ float max3f(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// tanh of a pair, |u| <= 1: odd polynomial, relative error below 7e-6 (a weighted least-squares fit moved towards the minimax one).
+// A score of 40 is then off by 3e-4, less than P's rounding to fp16 makes of it.
+static __device__ __forceinline__ float2 tanh_near(float2 u) {
+    const float2 w = mul2(u, u);
+    float2 p = fma2(w, pk2(0.009036419913172722f, 0.009036419913172722f), pk2(-0.044817544519901276f, -0.044817544519901276f));
+    p = fma2(p, w, pk2(0.13036811351776123f, 0.13036811351776123f));
+    p = fma2(p, w, pk2(-0.3329806625843048f, -0.3329806625843048f));
+    p = fma2(p, w, pk2(0.999993085861206f, 0.999993085861206f));
+    return mul2(p, u);
+}
+// tanh(u) = 1 - 2 / (1 + e^(2u)) for any u
+static __device__ __forceinline__ float tanh_any(float u) { return 1.f - 2.f * fast_reciprocal(1.f + fast_exp2(u * (2.f * SA_LOG2E))); }
+
+// tanh of a whole row's scores in tensor memory that are not near enough for tanh_near: s = from_u * tanh(s * to_u), in place
+static __device__ __noinline__ void cap_in_tmem(uint32_t t_s, float to_u, float from_u) {
+#pragma unroll 1
+    for (int c = 0; c < SA_T; c += 16) {
+        uint32_t s[16];
+        tmem_ld16(t_s + c, s);
+        tc_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = __float_as_uint(tanh_any(__uint_as_float(s[i]) * to_u) * from_u);
+        tmem_st16(t_s + c, s);
+    }
+    tc_wait_st();
+}
+
+// Bits of the 128 keys of a tile that a row sees: those in [from, to] or in front of `front`, and in front of `end` (all relative to the
+// tile); and, with `stage`, those whose document is the row's.
+static __device__ __noinline__ uint4 visible_keys(int from, int to, int front, int end, const int* stage, int my_doc) {
+    // bits lo .. hi of word w
+    auto bits = [](int lo, int hi, int w) -> uint32_t {
+        lo -= 32 * w;
+        hi -= 32 * w;
+        if (hi < 0 || lo > 31 || hi < lo) return 0u;
+        const uint32_t upto = hi >= 31 ? 0xFFFFFFFFu : (2u << hi) - 1u;
+        return lo <= 0 ? upto : upto & (0xFFFFFFFFu << lo);
+    };
+    uint32_t r[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        r[w] = (bits(from, to, w) | bits(0, front - 1, w)) & bits(0, end - 1, w);
+        if (stage != nullptr) {
+            uint32_t same = 0;
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+                const int4 k = *reinterpret_cast<const int4*>(stage + 32 * w + c);
+                same |= (k.x == my_doc ? 1u << c : 0u) | (k.y == my_doc ? 2u << c : 0u) | (k.z == my_doc ? 4u << c : 0u) | (k.w == my_doc ? 8u << c : 0u);
+            }
+            r[w] &= same;
+        }
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+// COUNT K = 16 products in one instruction sequence: the issuing thread is one lane, and every instruction that it spends between two
+// products delays all of them.  `a` and `b` advance by 32 bytes (2 in descriptor units) a product, by a panel after four.
+template <int COUNT>
+static __device__ __forceinline__ void mma_chain_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+    static_assert(COUNT == 4 || COUNT == 8, "64 or 128 of K");
+#define SA_MMA(off, p) "add.s64 a, %1, " #off ";\n\tadd.s64 b, %2, " #off ";\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, " #p ";\n\t"
+    if constexpr (COUNT == 4)
+        asm volatile("{\n\t.reg .pred p0, p1;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p0, 0, 0;\n\tsetp.eq.b32 p1, 0, 0;\n\t"
+                     SA_MMA(0, p0) SA_MMA(2, p1) SA_MMA(4, p1) SA_MMA(6, p1) "}" ::"r"(d), "l"(a), "l"(b), "r"(idesc) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p0, p1;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p0, 0, 0;\n\tsetp.eq.b32 p1, 0, 0;\n\t"
+                     SA_MMA(0, p0) SA_MMA(2, p1) SA_MMA(4, p1) SA_MMA(6, p1) SA_MMA(1024, p1) SA_MMA(1026, p1) SA_MMA(1028, p1) SA_MMA(1030, p1)
+                     "}" ::"r"(d), "l"(a), "l"(b), "r"(idesc) : "memory");
+#undef SA_MMA
+}
+// Four K = 16 products with A in tensor memory (8 columns each) and B key-row-major (16 rows of 128 bytes each); the first one
+// overwrites the accumulator where `accumulate` is 0
+static __device__ __forceinline__ void mma_chain_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p0, p1;\n\t.reg .b64 b;\n\t.reg .b32 a;\n\t"
+        "setp.ne.b32 p0, %4, 0;\n\t"
+        "setp.eq.b32 p1, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p0;\n\t"
+        "add.u32 a, %1, 8;\n\tadd.s64 b, %2, 128;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, p1;\n\t"
+        "add.u32 a, %1, 16;\n\tadd.s64 b, %2, 256;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, p1;\n\t"
+        "add.u32 a, %1, 24;\n\tadd.s64 b, %2, 384;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, p1;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+template <int D>
+static __device__ __noinline__ void rescale_o(uint32_t t_o, float alpha) {
+#pragma unroll 1
+    for (int c = 0; c < D; c += 16) {
+        uint32_t o[16];
+        tmem_ld16(t_o + c, o);
+        tc_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+        tmem_st16(t_o + c, o);
+    }
+    tc_wait_st();
+}
+
+// What a stretch of rows sees: tiles [lo, hi) and [0, prefix), where documents agree
+struct Reach {
+    int lo, hi, prefix, doc_min, doc_max;
+};
+
+template <int D, int HALVES, bool BF16, int MODE>
+__global__ void __launch_bounds__(HALVES * 128 + 64, HALVES == 1 && D == 64 ? 2 : 1) scored_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                                        const __grid_constant__ CUtensorMap map_v, const ScoredParams p) {
+    constexpr int PANELS = D / 64;                           // 64-column panels of a tile, 128 rows of 128 swizzled bytes each
+    constexpr int PANEL_BYTES = SA_T * 128, TILE_BYTES = PANELS * PANEL_BYTES;
+    constexpr int W_LOAD = HALVES * 4, W_MMA = W_LOAD + 1;
+    constexpr bool OWN_P = HALVES * (SA_T + SA_T / 2 + D) <= 512;
+    constexpr int COL_O = HALVES * SA_T, COL_P = OWN_P ? COL_O + HALVES * D : 0, P_STEP = OWN_P ? SA_T / 2 : SA_T;
+    constexpr int TMEM_COLS = (OWN_P ? COL_P + HALVES * SA_T / 2 : COL_O + HALVES * D) > 256 ? 512 : 256;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    unsigned char* q_smem = smem;
+    unsigned char* ring = q_smem + HALVES * TILE_BYTES;
+    float* table = reinterpret_cast<float*>(ring + 4 * TILE_BYTES);      // (two slots of K, two of V)
+    int2* range = reinterpret_cast<int2*>(reinterpret_cast<unsigned char*>(table) + p.table_bytes);
+    __shared__ __align__(8) uint64_t bars[SB_COUNT];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_word;
+    __shared__ int2 row_docs[HALVES * 4];                    // smallest and largest document of each softmax warp's rows
+    __shared__ __align__(16) int key_docs[HALVES][2][SA_T];
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    volatile int* abort_flag = &abort_word;
+    const WaitCtx wctx{abort_flag, p.status};
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars[SB_Q + i], 1);
+            mbar_init(&bars[SB_S + i], 1);
+            mbar_init(&bars[SB_P0 + i], 4);
+            mbar_init(&bars[SB_P1 + i], 4);
+            mbar_init(&bars[SB_READ + i], 4);
+            mbar_init(&bars[SB_O + i], 1);
+        }
+        mbar_init(&bars[SB_FIX], 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars[SB_K_FULL + i], 1);
+            mbar_init(&bars[SB_K_EMPTY + i], 1);
+            mbar_init(&bars[SB_V_FULL + i], 1);
+            mbar_init(&bars[SB_V_EMPTY + i], 1);
+        }
+        fence_mbar_init();
+    }
+    if (warp == W_MMA) {
+        tmem_alloc(&tmem_slot, TMEM_COLS);
+        tmem_relinquish();
+    }
+    grid_dependency_wait();
+    grid_launch_dependents();
+    if (threadIdx.x == 0) *abort_flag = failure_reported(p.status) ? 1 : 0;
+
+    // the heaviest stretches first: with a causal mask those at the end of the sequence
+    const int heads_all = p.batch * p.heads;
+    const int row_tile = p.q_tiles - 1 - static_cast<int>(blockIdx.x / heads_all), bh = static_cast<int>(blockIdx.x % heads_all);
+    const int b = bh / p.heads, head = bh % p.heads, kv = head / p.group;
+    const int q0 = row_tile * (SA_T * HALVES), shift = p.k_len - p.q_len;
+    const int k_end = p.key_lens != nullptr ? min(max(p.key_lens[b], 0), p.k_len) : p.k_len;
+    const int prefix = p.prefix_lens != nullptr ? min(max(p.prefix_lens[b], 0), k_end) : 0;
+    const int* docs = p.documents != nullptr ? p.documents + b * p.documents_stride : nullptr;
+
+    auto reach_of = [&](int h) {
+        Reach r = {0, 0, 0, 0, 0};
+        const int r0 = q0 + h * SA_T, r1 = min(r0 + SA_T, p.q_len) - 1;
+        if (r0 > r1) return r;
+        int end = p.causal ? r1 + shift + 1 : p.window > 0 ? r1 + shift + p.window : p.k_len;
+        end = min(max(end, prefix), k_end);
+        const int begin = p.window > 0 ? max(r0 + shift - p.window + 1, 0) : 0;
+        r.lo = begin / SA_T;
+        r.hi = end > 0 ? (end + SA_T - 1) / SA_T : 0;
+        r.prefix = (prefix + SA_T - 1) / SA_T;
+        return r;
+    };
+    Reach reach[HALVES];
+    int t_begin = 0x7FFFFFFF, t_end = 0;
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) {
+        reach[h] = reach_of(h);
+        if (reach[h].hi > 0) t_begin = min(t_begin, reach[h].prefix > 0 ? 0 : reach[h].lo);
+        t_end = max(t_end, reach[h].hi);
+    }
+    // tables into shared memory
+    if (p.distance_bias != nullptr) {
+        const float* src = p.distance_bias + static_cast<size_t>(head) * (2 * p.radius + 1);
+        for (int i = threadIdx.x; i < 2 * p.radius + 1 + 2 * SA_PAD; i += blockDim.x) table[i] = __ldca(src + min(max(i - SA_PAD, 0), 2 * p.radius)) * SA_LOG2E;
+    }
+    int my_doc = 0;
+    if (docs != nullptr) {
+        for (int t = t_begin + warp; t < t_end; t += HALVES * 4 + 2) {
+            int lo = 0x7FFFFFFF, hi = -0x7FFFFFFF - 1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = t * SA_T + 32 * i + lane;
+                if (j < k_end) {
+                    const int d = __ldca(docs + j);
+                    lo = min(lo, d);
+                    hi = max(hi, d);
+                }
+            }
+            lo = __reduce_min_sync(0xffffffffu, lo);
+            hi = __reduce_max_sync(0xffffffffu, hi);
+            if (lane == 0) range[t] = make_int2(lo, hi);
+        }
+        if (warp < HALVES * 4) {
+            const int row = q0 + static_cast<int>(threadIdx.x);
+            if (row < p.q_len) my_doc = __ldca(docs + row + shift);
+            const int lo = __reduce_min_sync(0xffffffffu, row < p.q_len ? my_doc : 0x7FFFFFFF), hi = __reduce_max_sync(0xffffffffu, row < p.q_len ? my_doc : -0x7FFFFFFF - 1);
+            if (lane == 0) row_docs[warp] = make_int2(lo, hi);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    if (docs != nullptr) {
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+            reach[h].doc_min = min(min(row_docs[4 * h].x, row_docs[4 * h + 1].x), min(row_docs[4 * h + 2].x, row_docs[4 * h + 3].x));
+            reach[h].doc_max = max(max(row_docs[4 * h].y, row_docs[4 * h + 1].y), max(row_docs[4 * h + 2].y, row_docs[4 * h + 3].y));
+        }
+    }
+    auto wanted = [&](int h, int t) {
+        const Reach& r = reach[h];
+        if (t >= r.hi || (t < r.lo && t >= r.prefix)) return false;
+        if (docs == nullptr) return true;
+        const int2 d = range[t];
+        return d.x <= r.doc_max && d.y >= r.doc_min;
+    };
+    auto next = [&](int t) {                                 // first tile from t on that a half wants
+        for (; t < t_end; ++t) {
+            bool any = wanted(0, t);
+            if constexpr (HALVES == 2) any = any || wanted(1, t);
+            if (any) break;
+        }
+        return t;
+    };
+    // the tile in which the keys end before the tensor does: what V holds there behind the last key is set to zero (P is zero there,
+    // but zero times a NaN is none)
+    const int fix_tile = k_end < p.k_len && k_end % SA_T != 0 ? k_end / SA_T : -1;
+
+    if (*abort_flag == 0) {
+        if (warp == W_LOAD) {
+            // ---------------------------------------------------------------- TMA producer
+            int fix_slot = -1;
+            uint32_t fix_phase = 0;
+            if (lane == 0) {
+                tma_prefetch_desc(&map_q);
+                tma_prefetch_desc(&map_k);
+                tma_prefetch_desc(&map_v);
+                // the n-th tile goes into slot n % 2 of its side, K a tile ahead of V
+                auto load = [&](int kind, int t, unsigned n) {
+                    const int s = static_cast<int>(n & 1);
+                    uint64_t *full = &bars[(kind == 0 ? SB_K_FULL : SB_V_FULL) + s], *empty = &bars[(kind == 0 ? SB_K_EMPTY : SB_V_EMPTY) + s];
+                    mbar_wait_addr(smem_u32(empty), ((n >> 1) & 1) ^ 1, wctx, (kind == 0 ? SB_K_EMPTY : SB_V_EMPTY) + s);
+                    mbar_arrive_expect_tx(full, TILE_BYTES);
+                    for (int c = 0; c < PANELS; ++c)
+                        load_tile(ring + (2 * kind + s) * TILE_BYTES + c * PANEL_BYTES, kind == 0 ? &map_k : &map_v, full, c * 64, t * SA_T, kv, b, p.slot_s[1 + kind],
+                                  p.slot_h[1 + kind]);
+                };
+                int t = next(t_begin);
+                if (t < t_end) {
+                    for (int h = 0; h < HALVES; ++h) {
+                        if (q0 + h * SA_T >= p.q_len) break;
+                        mbar_arrive_expect_tx(&bars[SB_Q + h], TILE_BYTES);
+                        for (int c = 0; c < PANELS; ++c)
+                            load_tile(q_smem + h * TILE_BYTES + c * PANEL_BYTES, &map_q, &bars[SB_Q + h], c * 64, q0 + h * SA_T, head, b, p.slot_s[0], p.slot_h[0]);
+                        if (h == 0) load(0, t, 0);
+                    }
+                }
+                for (unsigned n = 0; t < t_end; ++n) {
+                    const int tn = next(t + 1);
+                    if (tn < t_end) load(0, tn, n + 1);
+                    load(1, t, n);
+                    if (t == fix_tile) {
+                        fix_slot = static_cast<int>(n & 1);
+                        fix_phase = (n >> 1) & 1;
+                    }
+                    t = tn;
+                }
+            }
+            fix_slot = __shfl_sync(0xffffffffu, fix_slot, 0);
+            fix_phase = __shfl_sync(0xffffffffu, fix_phase, 0);
+            if (fix_slot >= 0) {                             // it is the last tile of all: nothing more goes into its slot
+                mbar_wait(&bars[SB_V_FULL + fix_slot], fix_phase, wctx, SB_V_FULL + fix_slot);
+                for (int i = (k_end % SA_T) * 8 + lane; i < SA_T * 8; i += 32)
+#pragma unroll
+                    for (int c = 0; c < PANELS; ++c)
+                        *reinterpret_cast<uint4*>(ring + (2 + fix_slot) * TILE_BYTES + c * PANEL_BYTES + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars[SB_FIX]);
+            }
+        } else if (warp == W_MMA) {
+            // ---------------------------------------------------------------- tcgen05 issuer
+            if (elect_one()) {
+                constexpr uint32_t type = BF16 ? (1u << 7) | (1u << 10) : 0u;
+                constexpr uint32_t idesc_qk = make_idesc_f16(SA_T, SA_T, false) | type, idesc_pv = make_idesc_f16(SA_T, D, true) | type;
+                const uint64_t q_desc = make_smem_desc_sw128(smem_u32(q_smem), 16, 1024);
+                const uint64_t k_desc = make_smem_desc_sw128(smem_u32(ring), 16, 1024);
+                const uint64_t v_desc = make_smem_desc_sw128(smem_u32(ring + 2 * TILE_BYTES), PANEL_BYTES, 1024);
+                const uint32_t bar0 = smem_u32(bars);
+                auto wait = [&](int bar, uint32_t parity) { mbar_wait_addr(bar0 + 8 * bar, parity, wctx, bar); };
+                int done[HALVES];                            // tiles whose PV has been issued
+#pragma unroll
+                for (int h = 0; h < HALVES; ++h) done[h] = 0;
+                auto qk = [&](int h, unsigned n) {           // S = Q K^T of the n-th tile
+                    if (done[h] == 0) wait(SB_Q + h, 0);
+                    tc_fence_after();
+                    mma_chain_ss<D / 16>(tmem + h * SA_T, q_desc + static_cast<uint64_t>(h * (TILE_BYTES >> 4)), k_desc + static_cast<uint64_t>((n & 1) * (TILE_BYTES >> 4)), idesc_qk);
+                    tc_commit_addr(bar0 + 8 * (SB_S + h));
+                };
+                auto pv = [&](int h, unsigned n) {           // O (+)= P V
+                    const uint64_t v = v_desc + static_cast<uint64_t>((n & 1) * (TILE_BYTES >> 4));
+                    const uint32_t parity = static_cast<uint32_t>(done[h] & 1), o = tmem + COL_O + h * D, q = tmem + COL_P + h * P_STEP;
+                    wait(SB_P0 + h, parity);
+                    tc_fence_after();
+                    mma_chain_ts(o, q, v, idesc_pv, done[h] > 0 ? 1u : 0u);
+                    wait(SB_P1 + h, parity);
+                    tc_fence_after();
+                    mma_chain_ts(o, q + 32, v + 512, idesc_pv, 1u);
+                    if constexpr (OWN_P) tc_commit_addr(bar0 + 8 * (SB_O + h));
+                    ++done[h];
+                };
+                int t = next(t_begin);
+                if (t < t_end) {
+                    wait(SB_K_FULL, 0);
+#pragma unroll
+                    for (int h = 0; h < HALVES; ++h)
+                        if (wanted(h, t)) qk(h, 0);
+                    tc_commit_addr(bar0 + 8 * SB_K_EMPTY);
+                }
+                for (unsigned n = 0; t < t_end; ++n) {
+                    const int tn = next(t + 1);
+                    const int ks = static_cast<int>((n + 1) & 1), vs = static_cast<int>(n & 1);
+                    if (tn < t_end) wait(SB_K_FULL + ks, ((n + 1) >> 1) & 1);
+                    if constexpr (OWN_P) {
+#pragma unroll
+                        for (int h = 0; h < HALVES; ++h) {
+                            if (tn < t_end && wanted(h, tn)) {
+                                if (wanted(h, t)) wait(SB_READ + h, static_cast<uint32_t>(done[h] & 1));     // S is in registers
+                                qk(h, n + 1);
+                            }
+                        }
+                        if (tn < t_end) tc_commit_addr(bar0 + 8 * (SB_K_EMPTY + ks));
+                    }
+                    wait(SB_V_FULL + vs, (n >> 1) & 1);
+                    if (t == fix_tile) wait(SB_FIX, 0);
+#pragma unroll
+                    for (int h = 0; h < HALVES; ++h) {
+                        if (wanted(h, t)) pv(h, n);
+                        if constexpr (!OWN_P)
+                            if (tn < t_end && wanted(h, tn)) qk(h, n + 1);
+                    }
+                    tc_commit_addr(bar0 + 8 * (SB_V_EMPTY + vs));
+                    if constexpr (!OWN_P)
+                        if (tn < t_end) tc_commit_addr(bar0 + 8 * (SB_K_EMPTY + ks));
+                    t = tn;
+                }
+                if constexpr (!OWN_P) {
+#pragma unroll
+                    for (int h = 0; h < HALVES; ++h) tc_commit_addr(bar0 + 8 * (SB_O + h));
+                }
+            }
+        } else {
+            // ---------------------------------------------------------------- softmax: one row a thread
+            const int h = HALVES == 2 ? warp >> 2 : 0, tid = threadIdx.x & 127;
+            const Reach mine = h == 0 ? reach[0] : reach[HALVES - 1];
+            const int row = q0 + h * SA_T + tid, pos = row + shift;
+            const int warp_row = q0 + static_cast<int>(threadIdx.x & ~31u);
+            const int pos0 = warp_row + shift, pos1 = min(warp_row + 31, p.q_len - 1) + shift;       // of the warp's first and last row
+            const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+            const uint32_t t_s = t_lane + h * SA_T, t_o = t_lane + COL_O + h * D, t_p = t_lane + COL_P + h * P_STEP;
+            constexpr bool changed = MODE != SA_PLAIN;
+            const bool capped = MODE == SA_CAP || (MODE == SA_ANY && p.softcap > 0.f);
+            const float to_u = capped ? p.scale / p.softcap : 0.f, from_u = p.softcap * SA_LOG2E;
+            const uint32_t s_bar = smem_u32(&bars[SB_S + h]);
+            const float raw_scale = p.scale * SA_LOG2E;      // of a score that nothing changes, to log2 units
+            const float sc = changed ? 1.f : raw_scale;      // what is left to multiply by when the exponential is taken
+            const float slope = p.slopes != nullptr ? __ldca(p.slopes + head) * SA_LOG2E : 0.f;
+            const int2 warp_docs = docs != nullptr ? row_docs[warp] : make_int2(0, 0);
+            const int see_lo = p.window > 0 ? pos - p.window + 1 : -0x40000000, see_hi = p.causal ? pos : p.window > 0 ? pos + p.window - 1 : 0x40000000;
+            float m_ref = -INFINITY, l_sum = 0.f;
+            int done = 0;
+            for (int t = t_begin; t < t_end; ++t) {
+                if (!wanted(h, t)) continue;
+                const int k0 = t * SA_T;
+                // all of the tile visible to all of the warp's rows?
+                const bool full = k0 + SA_T <= k_end &&
+                            (k0 + SA_T <= prefix || ((p.window == 0 || k0 >= pos1 - p.window + 1) &&
+                                                     (p.causal ? k0 + SA_T - 1 <= pos0 : p.window == 0 || k0 + SA_T - 1 <= pos0 + p.window - 1)));
+                bool same_doc = true, mixed = false;         // mixed: the half's rows or the tile's keys are of more than one document
+                if (docs != nullptr) {
+                    const int2 d = range[t];
+                    same_doc = d.x == d.y && warp_docs.x == warp_docs.y && d.x == warp_docs.x;
+                    mixed = d.x != d.y || mine.doc_min != mine.doc_max;
+                    if (mixed) {                             // the keys' documents, 128 threads together: all warps of the half or none
+                        int* stage = key_docs[h][done & 1];
+                        stage[tid] = k0 + tid < k_end ? __ldca(docs + k0 + tid) : 0;
+                        if (HALVES == 1 || h == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
+                        else asm volatile("bar.sync 2, 128;" ::: "memory");
+                    }
+                }
+                mbar_wait_addr(s_bar, static_cast<uint32_t>(done & 1), wctx, SB_S + h);
+                tc_fence_after();
+                uint32_t s[4][32];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tmem_ld32(t_s + 32 * i, s[i]);
+                tc_wait_ld();
+#define S_AT(c) s[(c) >> 5][(c) & 31]
+                if constexpr (MODE != SA_PLAIN) {
+                    if (capped) {
+                        float top = 0.f;
+#pragma unroll
+                        for (int c = 0; c < SA_T; c += 2) top = max3f(top, fabsf(__uint_as_float(S_AT(c))), fabsf(__uint_as_float(S_AT(c + 1))));
+                        if (__all_sync(0xffffffffu, top * to_u <= 1.f)) {
+                            const float2 to2 = pk2(to_u, to_u), from2 = pk2(from_u, from_u);
+#pragma unroll
+                            for (int c = 0; c < SA_T; c += 2) {
+                                const float2 y = mul2(tanh_near(mul2(pk2(__uint_as_float(S_AT(c)), __uint_as_float(S_AT(c + 1))), to2)), from2);
+                                S_AT(c) = __float_as_uint(y.x);
+                                S_AT(c + 1) = __float_as_uint(y.y);
+                            }
+                        } else {
+                            cap_in_tmem(t_s, to_u, from_u);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) tmem_ld32(t_s + 32 * i, s[i]);
+                            tc_wait_ld();
+                        }
+                    }
+                }
+                if constexpr (OWN_P) {                       // S may be overwritten from here on
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars[SB_READ + h]);
+                }
+                if constexpr (MODE == SA_ANY) {
+                    const float2 scale2 = capped ? pk2(1.f, 1.f) : pk2(raw_scale, raw_scale);
+                    // distances of the warp's rows in this tile: k0 - pos1 .. k0 + 127 - pos0
+                    const int near = k0 - pos1, far = k0 + SA_T - 1 - pos0;
+                    if (far <= 0 || near >= 0) {             // all behind or all ahead: -slope * |distance| is linear (0 without slopes)
+                        const float g = far <= 0 ? slope : -slope, at = g * static_cast<float>(k0 - pos);
+#pragma unroll
+                        for (int c = 0; c < SA_T; c += 2) {
+                            const float2 y = fma2(pk2(__uint_as_float(S_AT(c)), __uint_as_float(S_AT(c + 1))), scale2,
+                                                  fma2(pk2(g, g), pk2(static_cast<float>(c), static_cast<float>(c + 1)), pk2(at, at)));
+                            S_AT(c) = __float_as_uint(y.x);
+                            S_AT(c + 1) = __float_as_uint(y.y);
+                        }
+                    } else {
+                        const float away = static_cast<float>(k0 - pos);
+#pragma unroll
+                        for (int c = 0; c < SA_T; ++c)
+                            S_AT(c) = __float_as_uint(fmaf(__uint_as_float(S_AT(c)), scale2.x, -slope * fabsf(away + static_cast<float>(c))));
+                    }
+                    if (p.distance_bias != nullptr) {
+                        if (far <= -p.radius || near >= p.radius) {          // all of it beyond the table
+                            const float x = table[near >= p.radius ? 2 * p.radius + SA_PAD : SA_PAD];
+                            const float2 x2 = pk2(x, x);
+#pragma unroll
+                            for (int c = 0; c < SA_T; c += 2) {
+                                const float2 y = add2(pk2(__uint_as_float(S_AT(c)), __uint_as_float(S_AT(c + 1))), x2);
+                                S_AT(c) = __float_as_uint(y.x);
+                                S_AT(c + 1) = __float_as_uint(y.y);
+                            }
+                        } else {
+                            // (rows behind the last one are kept inside the table)
+                            const float* at = table + min(max(k0 - pos + p.radius + SA_PAD, 0), 2 * p.radius + 2 * SA_PAD - SA_T + 1);
+#pragma unroll
+                            for (int c = 0; c < SA_T; ++c) S_AT(c) = __float_as_uint(__uint_as_float(S_AT(c)) + at[c]);
+                        }
+                    }
+                }
+                if (!full || (mixed && !same_doc)) {
+                    const uint4 on = visible_keys(see_lo - k0, see_hi - k0, prefix - k0, k_end - k0, mixed && !same_doc ? key_docs[h][done & 1] : nullptr, my_doc);
+                    const uint32_t word[4] = {on.x, on.y, on.z, on.w};
+#pragma unroll
+                    for (int c = 0; c < SA_T; ++c)
+                        if ((word[c >> 5] & (1u << (c & 31))) == 0) S_AT(c) = 0xFF800000u;
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < SA_T; c += 8)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mx[i] = max3f(mx[i], __uint_as_float(S_AT(c + 2 * i)), __uint_as_float(S_AT(c + 2 * i + 1)));
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+                const bool need = top > m_ref + SA_RESCALE || (m_ref == -INFINITY && top > -INFINITY);
+                if (__any_sync(0xffffffffu, need)) {
+                    float alpha = 1.f;
+                    if (need) {
+                        // a whole number, for the polynomial exponential
+                        const float now = fminf(fmaxf(ceilf(top), -2097152.0f), 2097152.0f);
+                        alpha = m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - now);
+                        m_ref = now;
+                        l_sum *= alpha;
+                    }
+                    if (done > 0) {
+                        // Where P lies over S, S was issued behind the products before it and is there: so are they.  Else they have to
+                        // be waited for (SB_O counts them).
+                        if constexpr (OWN_P) {
+                            mbar_wait_addr(smem_u32(&bars[SB_O + h]), static_cast<uint32_t>((done - 1) & 1), wctx, SB_O + h);
+                            tc_fence_after();
+                        }
+                        rescale_o<D>(t_o, alpha);
+                    }
+                }
+                const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;
+                const float2 sc2 = pk2(sc, sc), negm2 = pk2(neg_m, neg_m), mm2 = pk2(12582912.0f + neg_m, 12582912.0f + neg_m);
+                const float lo = (-120.0f - neg_m) / sc;
+                float2 sum_a = pk2(0.f, 0.f), sum_b = pk2(0.f, 0.f);
+#pragma unroll
+                for (int part = 0; part < 2; ++part) {       // P goes to the issuer in two parts of 64 keys
+#pragma unroll
+                    for (int i = part * 32; i < part * 32 + 32; ++i) {
+                        const float s0 = __uint_as_float(S_AT(2 * i)), s1 = __uint_as_float(S_AT(2 * i + 1));
+                        float e0, e1;
+                        if (((i * SA_POLY_PAIRS) & 7) < SA_POLY_PAIRS) {
+                            exp2_poly_pair(s0, s1, lo, sc2, mm2, e0, e1);
+                        } else {
+                            const float2 x = fma2(pk2(s0, s1), sc2, negm2);
+                            e0 = fast_exp2(x.x);
+                            e1 = fast_exp2(x.y);
+                        }
+                        if (i & 1) sum_b = add2(sum_b, pk2(e0, e1));
+                        else sum_a = add2(sum_a, pk2(e0, e1));
+                        S_AT(i) = pack_pair<BF16>(e0, e1);   // the scores of pair i were used above
+                    }
+                    if constexpr (OWN_P) {
+                        // the products that read the P before this one have to be through: they are where O is complete
+                        if (part == 0 && done > 0) mbar_wait_addr(smem_u32(&bars[SB_O + h]), static_cast<uint32_t>((done - 1) & 1), wctx, SB_O + h);
+                    }
+                    tmem_st32(t_p + 32 * part, s[part]);
+                    tc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars[(part == 0 ? SB_P0 : SB_P1) + h]);
+                }
+                const float2 sum = add2(sum_a, sum_b);
+                l_sum += sum.x + sum.y;
+#undef S_AT
+                ++done;
+            }
+            // ---------------------------------------------------------------- O / l
+            if (done > 0) {
+                mbar_wait(&bars[SB_O + h], OWN_P ? static_cast<uint32_t>((done - 1) & 1) : 0u, wctx, SB_O + h);
+                tc_fence_after();
+            }
+            // a row that saw nothing has no maximum; where all it saw is NaN its sum says so
+            const bool any = done > 0 && (m_ref > -INFINITY || l_sum != l_sum);
+            const float inv = any ? 1.f / l_sum : 0.f;
+            uint16_t* dst = static_cast<uint16_t*>(p.out) + b * p.out_stride[0] + head * p.out_stride[1] + static_cast<long long>(row) * p.out_stride[2];
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                if (done > 0) {
+                    tmem_ld32(t_o + c, o);
+                    tc_wait_ld();
+                }
+                if (row < p.q_len) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        auto two = [&](int j) { return any ? pack_pair<BF16>(__uint_as_float(o[i + j]) * inv, __uint_as_float(o[i + j + 1]) * inv) : 0u; };
+                        *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(two(0), two(2), two(4), two(6));
+                    }
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == W_MMA) {
+        tc_fence_after();
+        tmem_dealloc(tmem, TMEM_COLS);
+    }
+}
+
+
+using ScoredMaps = CUtensorMap[3];
+// Launches the kernel for one head size (scored_attn_64.cu, scored_attn_128.cu: a translation unit each, they take long to compile)
+template <int D>
+int launch_scored(const ScoredMaps& maps, const ScoredParams& p, int halves, bool bf16, int mode, long long blocks, size_t smem, cudaStream_t stream);
+
+template <int D>
+int launch_scored_impl(const ScoredMaps& maps, const ScoredParams& p, int halves, bool bf16, int mode, long long blocks, size_t smem, cudaStream_t stream) {
+    auto launch = [&](auto kernel) -> int {
+        STOF_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+        LaunchConfig lc(dim3(static_cast<unsigned>(blocks)), static_cast<unsigned>(halves * 128 + 64), smem, stream);
+        STOF_CUDA(cudaLaunchKernelEx(&lc.cfg, kernel, maps[0], maps[1], maps[2], p));
+        return STOF_OK;
+    };
+    auto by_mode = [&](auto h, auto b) -> int {
+        constexpr int H = decltype(h)::value;
+        constexpr bool B = decltype(b)::value;
+        if (mode == SA_PLAIN) return launch(scored_attn_kernel<D, H, B, SA_PLAIN>);
+        if (mode == SA_CAP) return launch(scored_attn_kernel<D, H, B, SA_CAP>);
+        return launch(scored_attn_kernel<D, H, B, SA_ANY>);
+    };
+    using std::integral_constant;
+    if (halves == 2) return bf16 ? by_mode(integral_constant<int, 2>{}, std::true_type{}) : by_mode(integral_constant<int, 2>{}, std::false_type{});
+    return bf16 ? by_mode(integral_constant<int, 1>{}, std::true_type{}) : by_mode(integral_constant<int, 1>{}, std::false_type{});
+}
+
+}  // namespace stof
