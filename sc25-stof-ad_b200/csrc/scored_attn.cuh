@@ -75,8 +75,23 @@ static __device__ __forceinline__ float2 tanh_near(float2 u) {
 // tanh(u) = 1 - 2 / (1 + e^(2u)) for any u
 static __device__ __forceinline__ float tanh_any(float u) { return 1.f - 2.f * fast_reciprocal(1.f + fast_exp2(u * (2.f * SA_LOG2E))); }
 
+// The bounded wait without a call of a function (which does not go with moved registers)
+static __device__ __forceinline__ void wait_inline(uint32_t bar, uint32_t parity, const WaitCtx& ctx, int barrier_id) {
+    if (mbar_test_wait_addr(bar, parity)) return;
+    const long long t0 = clock64();
+#pragma unroll 1
+    while (!mbar_try_wait_addr(bar, parity)) {
+        if (*ctx.abort_smem) return;
+        if (clock64() - t0 > WAIT_BUDGET_CYCLES) {
+            *ctx.abort_smem = 1;
+            if (ctx.status_gmem) atomicCAS(ctx.status_gmem, 0, (barrier_id << 8) | STATUS_WAIT_TIMEOUT);
+            return;
+        }
+    }
+}
+
 // tanh of a whole row's scores in tensor memory that are not near enough for tanh_near: s = from_u * tanh(s * to_u), in place
-static __device__ __noinline__ void cap_in_tmem(uint32_t t_s, float to_u, float from_u) {
+static __device__ __forceinline__ void cap_in_tmem(uint32_t t_s, float to_u, float from_u) {
 #pragma unroll 1
     for (int c = 0; c < SA_T; c += 16) {
         uint32_t s[16];
@@ -91,7 +106,7 @@ static __device__ __noinline__ void cap_in_tmem(uint32_t t_s, float to_u, float 
 
 // Bits of the 128 keys of a tile that a row sees: those in [from, to] or in front of `front`, and in front of `end` (all relative to the
 // tile); and, with `stage`, those whose document is the row's.
-static __device__ __noinline__ uint4 visible_keys(int from, int to, int front, int end, const int* stage, int my_doc) {
+static __device__ __forceinline__ uint4 visible_keys(int from, int to, int front, int end, const int* stage, int my_doc) {
     // bits lo .. hi of word w
     auto bits = [](int lo, int hi, int w) -> uint32_t {
         lo -= 32 * w;
@@ -151,7 +166,7 @@ static __device__ __forceinline__ void mma_chain_ts(uint32_t d, uint32_t a, uint
 }
 
 template <int D>
-static __device__ __noinline__ void rescale_o(uint32_t t_o, float alpha) {
+static __device__ __forceinline__ void rescale_o(uint32_t t_o, float alpha) {
 #pragma unroll 1
     for (int c = 0; c < D; c += 16) {
         uint32_t o[16];
@@ -164,13 +179,19 @@ static __device__ __noinline__ void rescale_o(uint32_t t_o, float alpha) {
     tc_wait_st();
 }
 
+// Two halves: three warpgroups, the last one with two idle warps, so that registers can be moved from it to the softmax warps (setmaxnreg
+// is a whole warpgroup's): 384 x 168 at the launch, 256 x 224 + 128 x 56 afterwards, the same sum.
+constexpr int SA_REGS_SOFTMAX = 224, SA_REGS_OTHER = 56;
+static_assert(256 * SA_REGS_SOFTMAX + 128 * SA_REGS_OTHER <= 384 * 168, "more registers than the block was launched with would be waited for forever");
+constexpr int scored_threads(int halves) { return halves == 2 ? 384 : 192; }
+
 // What a stretch of rows sees: tiles [lo, hi) and [0, prefix), where documents agree
 struct Reach {
     int lo, hi, prefix, doc_min, doc_max;
 };
 
 template <int D, int HALVES, bool BF16, int MODE>
-__global__ void __launch_bounds__(HALVES * 128 + 64, HALVES == 1 && D == 64 ? 2 : 1) scored_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64 && MODE != SA_ANY ? 2 : 1) scored_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                                         const __grid_constant__ CUtensorMap map_v, const ScoredParams p) {
     constexpr int PANELS = D / 64;                           // 64-column panels of a tile, 128 rows of 128 swizzled bytes each
     constexpr int PANEL_BYTES = SA_T * 128, TILE_BYTES = PANELS * PANEL_BYTES;
@@ -255,7 +276,7 @@ __global__ void __launch_bounds__(HALVES * 128 + 64, HALVES == 1 && D == 64 ? 2 
     }
     int my_doc = 0;
     if (docs != nullptr) {
-        for (int t = t_begin + warp; t < t_end; t += HALVES * 4 + 2) {
+        for (int t = t_begin + warp; t < t_end; t += scored_threads(HALVES) / 32) {
             int lo = 0x7FFFFFFF, hi = -0x7FFFFFFF - 1;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -307,130 +328,9 @@ __global__ void __launch_bounds__(HALVES * 128 + 64, HALVES == 1 && D == 64 ? 2 
     // but zero times a NaN is none)
     const int fix_tile = k_end < p.k_len && k_end % SA_T != 0 ? k_end / SA_T : -1;
 
-    if (*abort_flag == 0) {
-        if (warp == W_LOAD) {
-            // ---------------------------------------------------------------- TMA producer
-            int fix_slot = -1;
-            uint32_t fix_phase = 0;
-            if (lane == 0) {
-                tma_prefetch_desc(&map_q);
-                tma_prefetch_desc(&map_k);
-                tma_prefetch_desc(&map_v);
-                // the n-th tile goes into slot n % 2 of its side, K a tile ahead of V
-                auto load = [&](int kind, int t, unsigned n) {
-                    const int s = static_cast<int>(n & 1);
-                    uint64_t *full = &bars[(kind == 0 ? SB_K_FULL : SB_V_FULL) + s], *empty = &bars[(kind == 0 ? SB_K_EMPTY : SB_V_EMPTY) + s];
-                    mbar_wait_addr(smem_u32(empty), ((n >> 1) & 1) ^ 1, wctx, (kind == 0 ? SB_K_EMPTY : SB_V_EMPTY) + s);
-                    mbar_arrive_expect_tx(full, TILE_BYTES);
-                    for (int c = 0; c < PANELS; ++c)
-                        load_tile(ring + (2 * kind + s) * TILE_BYTES + c * PANEL_BYTES, kind == 0 ? &map_k : &map_v, full, c * 64, t * SA_T, kv, b, p.slot_s[1 + kind],
-                                  p.slot_h[1 + kind]);
-                };
-                int t = next(t_begin);
-                if (t < t_end) {
-                    for (int h = 0; h < HALVES; ++h) {
-                        if (q0 + h * SA_T >= p.q_len) break;
-                        mbar_arrive_expect_tx(&bars[SB_Q + h], TILE_BYTES);
-                        for (int c = 0; c < PANELS; ++c)
-                            load_tile(q_smem + h * TILE_BYTES + c * PANEL_BYTES, &map_q, &bars[SB_Q + h], c * 64, q0 + h * SA_T, head, b, p.slot_s[0], p.slot_h[0]);
-                        if (h == 0) load(0, t, 0);
-                    }
-                }
-                for (unsigned n = 0; t < t_end; ++n) {
-                    const int tn = next(t + 1);
-                    if (tn < t_end) load(0, tn, n + 1);
-                    load(1, t, n);
-                    if (t == fix_tile) {
-                        fix_slot = static_cast<int>(n & 1);
-                        fix_phase = (n >> 1) & 1;
-                    }
-                    t = tn;
-                }
-            }
-            fix_slot = __shfl_sync(0xffffffffu, fix_slot, 0);
-            fix_phase = __shfl_sync(0xffffffffu, fix_phase, 0);
-            if (fix_slot >= 0) {                             // it is the last tile of all: nothing more goes into its slot
-                mbar_wait(&bars[SB_V_FULL + fix_slot], fix_phase, wctx, SB_V_FULL + fix_slot);
-                for (int i = (k_end % SA_T) * 8 + lane; i < SA_T * 8; i += 32)
-#pragma unroll
-                    for (int c = 0; c < PANELS; ++c)
-                        *reinterpret_cast<uint4*>(ring + (2 + fix_slot) * TILE_BYTES + c * PANEL_BYTES + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars[SB_FIX]);
-            }
-        } else if (warp == W_MMA) {
-            // ---------------------------------------------------------------- tcgen05 issuer
-            if (elect_one()) {
-                constexpr uint32_t type = BF16 ? (1u << 7) | (1u << 10) : 0u;
-                constexpr uint32_t idesc_qk = make_idesc_f16(SA_T, SA_T, false) | type, idesc_pv = make_idesc_f16(SA_T, D, true) | type;
-                const uint64_t q_desc = make_smem_desc_sw128(smem_u32(q_smem), 16, 1024);
-                const uint64_t k_desc = make_smem_desc_sw128(smem_u32(ring), 16, 1024);
-                const uint64_t v_desc = make_smem_desc_sw128(smem_u32(ring + 2 * TILE_BYTES), PANEL_BYTES, 1024);
-                const uint32_t bar0 = smem_u32(bars);
-                auto wait = [&](int bar, uint32_t parity) { mbar_wait_addr(bar0 + 8 * bar, parity, wctx, bar); };
-                int done[HALVES];                            // tiles whose PV has been issued
-#pragma unroll
-                for (int h = 0; h < HALVES; ++h) done[h] = 0;
-                auto qk = [&](int h, unsigned n) {           // S = Q K^T of the n-th tile
-                    if (done[h] == 0) wait(SB_Q + h, 0);
-                    tc_fence_after();
-                    mma_chain_ss<D / 16>(tmem + h * SA_T, q_desc + static_cast<uint64_t>(h * (TILE_BYTES >> 4)), k_desc + static_cast<uint64_t>((n & 1) * (TILE_BYTES >> 4)), idesc_qk);
-                    tc_commit_addr(bar0 + 8 * (SB_S + h));
-                };
-                auto pv = [&](int h, unsigned n) {           // O (+)= P V
-                    const uint64_t v = v_desc + static_cast<uint64_t>((n & 1) * (TILE_BYTES >> 4));
-                    const uint32_t parity = static_cast<uint32_t>(done[h] & 1), o = tmem + COL_O + h * D, q = tmem + COL_P + h * P_STEP;
-                    wait(SB_P0 + h, parity);
-                    tc_fence_after();
-                    mma_chain_ts(o, q, v, idesc_pv, done[h] > 0 ? 1u : 0u);
-                    wait(SB_P1 + h, parity);
-                    tc_fence_after();
-                    mma_chain_ts(o, q + 32, v + 512, idesc_pv, 1u);
-                    if constexpr (OWN_P) tc_commit_addr(bar0 + 8 * (SB_O + h));
-                    ++done[h];
-                };
-                int t = next(t_begin);
-                if (t < t_end) {
-                    wait(SB_K_FULL, 0);
-#pragma unroll
-                    for (int h = 0; h < HALVES; ++h)
-                        if (wanted(h, t)) qk(h, 0);
-                    tc_commit_addr(bar0 + 8 * SB_K_EMPTY);
-                }
-                for (unsigned n = 0; t < t_end; ++n) {
-                    const int tn = next(t + 1);
-                    const int ks = static_cast<int>((n + 1) & 1), vs = static_cast<int>(n & 1);
-                    if (tn < t_end) wait(SB_K_FULL + ks, ((n + 1) >> 1) & 1);
-                    if constexpr (OWN_P) {
-#pragma unroll
-                        for (int h = 0; h < HALVES; ++h) {
-                            if (tn < t_end && wanted(h, tn)) {
-                                if (wanted(h, t)) wait(SB_READ + h, static_cast<uint32_t>(done[h] & 1));     // S is in registers
-                                qk(h, n + 1);
-                            }
-                        }
-                        if (tn < t_end) tc_commit_addr(bar0 + 8 * (SB_K_EMPTY + ks));
-                    }
-                    wait(SB_V_FULL + vs, (n >> 1) & 1);
-                    if (t == fix_tile) wait(SB_FIX, 0);
-#pragma unroll
-                    for (int h = 0; h < HALVES; ++h) {
-                        if (wanted(h, t)) pv(h, n);
-                        if constexpr (!OWN_P)
-                            if (tn < t_end && wanted(h, tn)) qk(h, n + 1);
-                    }
-                    tc_commit_addr(bar0 + 8 * (SB_V_EMPTY + vs));
-                    if constexpr (!OWN_P)
-                        if (tn < t_end) tc_commit_addr(bar0 + 8 * (SB_K_EMPTY + ks));
-                    t = tn;
-                }
-                if constexpr (!OWN_P) {
-#pragma unroll
-                    for (int h = 0; h < HALVES; ++h) tc_commit_addr(bar0 + 8 * (SB_O + h));
-                }
-            }
-        } else {
+    if (warp < HALVES * 4) {
+        if constexpr (HALVES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SA_REGS_SOFTMAX));
+        if (*abort_flag == 0) {
             // ---------------------------------------------------------------- softmax: one row a thread
             const int h = HALVES == 2 ? warp >> 2 : 0, tid = threadIdx.x & 127;
             const Reach mine = h == 0 ? reach[0] : reach[HALVES - 1];
@@ -469,7 +369,7 @@ __global__ void __launch_bounds__(HALVES * 128 + 64, HALVES == 1 && D == 64 ? 2 
                         else asm volatile("bar.sync 2, 128;" ::: "memory");
                     }
                 }
-                mbar_wait_addr(s_bar, static_cast<uint32_t>(done & 1), wctx, SB_S + h);
+                wait_inline(s_bar, static_cast<uint32_t>(done & 1), wctx, SB_S + h);
                 tc_fence_after();
                 uint32_t s[4][32];
 #pragma unroll
@@ -566,7 +466,7 @@ __global__ void __launch_bounds__(HALVES * 128 + 64, HALVES == 1 && D == 64 ? 2 
                         // Where P lies over S, S was issued behind the products before it and is there: so are they.  Else they have to
                         // be waited for (SB_O counts them).
                         if constexpr (OWN_P) {
-                            mbar_wait_addr(smem_u32(&bars[SB_O + h]), static_cast<uint32_t>((done - 1) & 1), wctx, SB_O + h);
+                            wait_inline(smem_u32(&bars[SB_O + h]), static_cast<uint32_t>((done - 1) & 1), wctx, SB_O + h);
                             tc_fence_after();
                         }
                         rescale_o<D>(t_o, alpha);
@@ -595,7 +495,7 @@ __global__ void __launch_bounds__(HALVES * 128 + 64, HALVES == 1 && D == 64 ? 2 
                     }
                     if constexpr (OWN_P) {
                         // the products that read the P before this one have to be through: they are where O is complete
-                        if (part == 0 && done > 0) mbar_wait_addr(smem_u32(&bars[SB_O + h]), static_cast<uint32_t>((done - 1) & 1), wctx, SB_O + h);
+                        if (part == 0 && done > 0) wait_inline(smem_u32(&bars[SB_O + h]), static_cast<uint32_t>((done - 1) & 1), wctx, SB_O + h);
                     }
                     tmem_st32(t_p + 32 * part, s[part]);
                     tc_wait_st();
@@ -633,6 +533,131 @@ __global__ void __launch_bounds__(HALVES * 128 + 64, HALVES == 1 && D == 64 ? 2 
                 }
             }
         }
+    } else {
+        if constexpr (HALVES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SA_REGS_OTHER));
+        if (*abort_flag == 0 && warp == W_LOAD) {
+            // ---------------------------------------------------------------- TMA producer
+            int fix_slot = -1;
+            uint32_t fix_phase = 0;
+            if (lane == 0) {
+                tma_prefetch_desc(&map_q);
+                tma_prefetch_desc(&map_k);
+                tma_prefetch_desc(&map_v);
+                // the n-th tile goes into slot n % 2 of its side, K a tile ahead of V
+                auto load = [&](int kind, int t, unsigned n) {
+                    const int s = static_cast<int>(n & 1);
+                    uint64_t *full = &bars[(kind == 0 ? SB_K_FULL : SB_V_FULL) + s], *empty = &bars[(kind == 0 ? SB_K_EMPTY : SB_V_EMPTY) + s];
+                    wait_inline(smem_u32(empty), ((n >> 1) & 1) ^ 1, wctx, (kind == 0 ? SB_K_EMPTY : SB_V_EMPTY) + s);
+                    mbar_arrive_expect_tx(full, TILE_BYTES);
+                    for (int c = 0; c < PANELS; ++c)
+                        load_tile(ring + (2 * kind + s) * TILE_BYTES + c * PANEL_BYTES, kind == 0 ? &map_k : &map_v, full, c * 64, t * SA_T, kv, b, p.slot_s[1 + kind],
+                                  p.slot_h[1 + kind]);
+                };
+                int t = next(t_begin);
+                if (t < t_end) {
+                    for (int h = 0; h < HALVES; ++h) {
+                        if (q0 + h * SA_T >= p.q_len) break;
+                        mbar_arrive_expect_tx(&bars[SB_Q + h], TILE_BYTES);
+                        for (int c = 0; c < PANELS; ++c)
+                            load_tile(q_smem + h * TILE_BYTES + c * PANEL_BYTES, &map_q, &bars[SB_Q + h], c * 64, q0 + h * SA_T, head, b, p.slot_s[0], p.slot_h[0]);
+                        if (h == 0) load(0, t, 0);
+                    }
+                }
+                for (unsigned n = 0; t < t_end; ++n) {
+                    const int tn = next(t + 1);
+                    if (tn < t_end) load(0, tn, n + 1);
+                    load(1, t, n);
+                    if (t == fix_tile) {
+                        fix_slot = static_cast<int>(n & 1);
+                        fix_phase = (n >> 1) & 1;
+                    }
+                    t = tn;
+                }
+            }
+            fix_slot = __shfl_sync(0xffffffffu, fix_slot, 0);
+            fix_phase = __shfl_sync(0xffffffffu, fix_phase, 0);
+            if (fix_slot >= 0) {                             // it is the last tile of all: nothing more goes into its slot
+                mbar_wait(&bars[SB_V_FULL + fix_slot], fix_phase, wctx, SB_V_FULL + fix_slot);
+                for (int i = (k_end % SA_T) * 8 + lane; i < SA_T * 8; i += 32)
+#pragma unroll
+                    for (int c = 0; c < PANELS; ++c)
+                        *reinterpret_cast<uint4*>(ring + (2 + fix_slot) * TILE_BYTES + c * PANEL_BYTES + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars[SB_FIX]);
+            }
+        } else if (*abort_flag == 0 && warp == W_MMA) {
+            // ---------------------------------------------------------------- tcgen05 issuer
+            if (elect_one()) {
+                constexpr uint32_t type = BF16 ? (1u << 7) | (1u << 10) : 0u;
+                constexpr uint32_t idesc_qk = make_idesc_f16(SA_T, SA_T, false) | type, idesc_pv = make_idesc_f16(SA_T, D, true) | type;
+                const uint64_t q_desc = make_smem_desc_sw128(smem_u32(q_smem), 16, 1024);
+                const uint64_t k_desc = make_smem_desc_sw128(smem_u32(ring), 16, 1024);
+                const uint64_t v_desc = make_smem_desc_sw128(smem_u32(ring + 2 * TILE_BYTES), PANEL_BYTES, 1024);
+                const uint32_t bar0 = smem_u32(bars);
+                auto wait = [&](int bar, uint32_t parity) { wait_inline(bar0 + 8 * bar, parity, wctx, bar); };
+                int done[HALVES];                            // tiles whose PV has been issued
+#pragma unroll
+                for (int h = 0; h < HALVES; ++h) done[h] = 0;
+                auto qk = [&](int h, unsigned n) {           // S = Q K^T of the n-th tile
+                    if (done[h] == 0) wait(SB_Q + h, 0);
+                    tc_fence_after();
+                    mma_chain_ss<D / 16>(tmem + h * SA_T, q_desc + static_cast<uint64_t>(h * (TILE_BYTES >> 4)), k_desc + static_cast<uint64_t>((n & 1) * (TILE_BYTES >> 4)), idesc_qk);
+                    tc_commit_addr(bar0 + 8 * (SB_S + h));
+                };
+                auto pv = [&](int h, unsigned n) {           // O (+)= P V
+                    const uint64_t v = v_desc + static_cast<uint64_t>((n & 1) * (TILE_BYTES >> 4));
+                    const uint32_t parity = static_cast<uint32_t>(done[h] & 1), o = tmem + COL_O + h * D, q = tmem + COL_P + h * P_STEP;
+                    wait(SB_P0 + h, parity);
+                    tc_fence_after();
+                    mma_chain_ts(o, q, v, idesc_pv, done[h] > 0 ? 1u : 0u);
+                    wait(SB_P1 + h, parity);
+                    tc_fence_after();
+                    mma_chain_ts(o, q + 32, v + 512, idesc_pv, 1u);
+                    if constexpr (OWN_P) tc_commit_addr(bar0 + 8 * (SB_O + h));
+                    ++done[h];
+                };
+                int t = next(t_begin);
+                if (t < t_end) {
+                    wait(SB_K_FULL, 0);
+#pragma unroll
+                    for (int h = 0; h < HALVES; ++h)
+                        if (wanted(h, t)) qk(h, 0);
+                    tc_commit_addr(bar0 + 8 * SB_K_EMPTY);
+                }
+                for (unsigned n = 0; t < t_end; ++n) {
+                    const int tn = next(t + 1);
+                    const int ks = static_cast<int>((n + 1) & 1), vs = static_cast<int>(n & 1);
+                    if (tn < t_end) wait(SB_K_FULL + ks, ((n + 1) >> 1) & 1);
+                    if constexpr (OWN_P) {
+#pragma unroll
+                        for (int h = 0; h < HALVES; ++h) {
+                            if (tn < t_end && wanted(h, tn)) {
+                                if (wanted(h, t)) wait(SB_READ + h, static_cast<uint32_t>(done[h] & 1));     // S is in registers
+                                qk(h, n + 1);
+                            }
+                        }
+                        if (tn < t_end) tc_commit_addr(bar0 + 8 * (SB_K_EMPTY + ks));
+                    }
+                    wait(SB_V_FULL + vs, (n >> 1) & 1);
+                    if (t == fix_tile) wait(SB_FIX, 0);
+#pragma unroll
+                    for (int h = 0; h < HALVES; ++h) {
+                        if (wanted(h, t)) pv(h, n);
+                        if constexpr (!OWN_P)
+                            if (tn < t_end && wanted(h, tn)) qk(h, n + 1);
+                    }
+                    tc_commit_addr(bar0 + 8 * (SB_V_EMPTY + vs));
+                    if constexpr (!OWN_P)
+                        if (tn < t_end) tc_commit_addr(bar0 + 8 * (SB_K_EMPTY + ks));
+                    t = tn;
+                }
+                if constexpr (!OWN_P) {
+#pragma unroll
+                    for (int h = 0; h < HALVES; ++h) tc_commit_addr(bar0 + 8 * (SB_O + h));
+                }
+            }
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -652,7 +677,7 @@ template <int D>
 int launch_scored_impl(const ScoredMaps& maps, const ScoredParams& p, int halves, bool bf16, int mode, long long blocks, size_t smem, cudaStream_t stream) {
     auto launch = [&](auto kernel) -> int {
         STOF_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-        LaunchConfig lc(dim3(static_cast<unsigned>(blocks)), static_cast<unsigned>(halves * 128 + 64), smem, stream);
+        LaunchConfig lc(dim3(static_cast<unsigned>(blocks)), static_cast<unsigned>(scored_threads(halves)), smem, stream);
         STOF_CUDA(cudaLaunchKernelEx(&lc.cfg, kernel, maps[0], maps[1], maps[2], p));
         return STOF_OK;
     };
