@@ -25,9 +25,6 @@ constexpr int SA_T = 128;                    // rows of a half, keys of a tile
 constexpr int SA_PAD = 256;                  // the distance table in shared memory goes on for so long on both sides: a tile that meets the table needs no clamp
 constexpr float SA_RESCALE = 8.0f;           // log2 units by which a row's maximum may outgrow the reference of its P (P <= 2^8)
 constexpr float SA_LOG2E = 1.4426950408889634f;
-#ifndef SA_POLY_PAIRS
-#define SA_POLY_PAIRS 2                      // of every 8 pairs of exponentials, so many on the FMA pipe
-#endif
 enum { SA_PLAIN = 0, SA_CAP = 1, SA_ANY = 2 };       // what is done to scores: nothing, the cap alone, whatever the call asks for
 
 struct ScoredParams {
@@ -77,7 +74,7 @@ static __device__ __forceinline__ float tanh_any(float u) { return 1.f - 2.f * f
 
 // The bounded wait without a call of a function (which does not go with moved registers)
 static __device__ __forceinline__ void wait_inline(uint32_t bar, uint32_t parity, const WaitCtx& ctx, int barrier_id) {
-    if (mbar_test_wait_addr(bar, parity)) return;
+    if (__builtin_expect(mbar_test_wait_addr(bar, parity), 1)) return;
     const long long t0 = clock64();
 #pragma unroll 1
     while (!mbar_try_wait_addr(bar, parity)) {
@@ -309,13 +306,13 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
             reach[h].doc_max = max(max(row_docs[4 * h].y, row_docs[4 * h + 1].y), max(row_docs[4 * h + 2].y, row_docs[4 * h + 3].y));
         }
     }
-    auto wanted = [&](int h, int t) {
-        const Reach& r = reach[h];
+    auto wanted_by = [&](const Reach& r, int t) {
         if (t >= r.hi || (t < r.lo && t >= r.prefix)) return false;
         if (docs == nullptr) return true;
         const int2 d = range[t];
         return d.x <= r.doc_max && d.y >= r.doc_min;
     };
+    auto wanted = [&](int h, int t) { return wanted_by(reach[h], t); };     // (h known to the compiler: `reach` stays in registers)
     auto next = [&](int t) {                                 // first tile from t on that a half wants
         for (; t < t_end; ++t) {
             bool any = wanted(0, t);
@@ -333,7 +330,14 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
         if (*abort_flag == 0) {
             // ---------------------------------------------------------------- softmax: one row a thread
             const int h = HALVES == 2 ? warp >> 2 : 0, tid = threadIdx.x & 127;
-            const Reach mine = h == 0 ? reach[0] : reach[HALVES - 1];
+            Reach mine = reach_of(h);
+            if (docs != nullptr) {
+                for (int i = 0; i < 4; ++i) {
+                    const int2 d = row_docs[4 * h + i];
+                    mine.doc_min = i == 0 ? d.x : min(mine.doc_min, d.x);
+                    mine.doc_max = i == 0 ? d.y : max(mine.doc_max, d.y);
+                }
+            }
             const int row = q0 + h * SA_T + tid, pos = row + shift;
             const int warp_row = q0 + static_cast<int>(threadIdx.x & ~31u);
             const int pos0 = warp_row + shift, pos1 = min(warp_row + 31, p.q_len - 1) + shift;       // of the warp's first and last row
@@ -348,15 +352,22 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
             const float slope = p.slopes != nullptr ? __ldca(p.slopes + head) * SA_LOG2E : 0.f;
             const int2 warp_docs = docs != nullptr ? row_docs[warp] : make_int2(0, 0);
             const int see_lo = p.window > 0 ? pos - p.window + 1 : -0x40000000, see_hi = p.causal ? pos : p.window > 0 ? pos + p.window - 1 : 0x40000000;
+            // the tiles of which all is visible to all of the warp's rows (documents aside): [0, full_prefix) and [full_from, full_to)
+            const int full_prefix = prefix / SA_T, full_from = p.window > 0 ? max(pos1 - p.window + SA_T, 0) / SA_T : 0;
+            const int full_to = max(min(p.causal ? pos0 + 1 : p.window > 0 ? pos0 + p.window : p.k_len, k_end), 0) / SA_T;
             float m_ref = -INFINITY, l_sum = 0.f;
             int done = 0;
-            for (int t = t_begin; t < t_end; ++t) {
-                if (!wanted(h, t)) continue;
+            for (int t = mine.prefix > 0 ? 0 : mine.lo; t < mine.hi; ++t) {
+                if (t < mine.lo && t >= mine.prefix) {                       // from the prefix to the window
+                    t = mine.lo;
+                    if (t >= mine.hi) break;
+                }
+                if (docs != nullptr) {
+                    const int2 d = range[t];
+                    if (d.x > mine.doc_max || d.y < mine.doc_min) continue;
+                }
                 const int k0 = t * SA_T;
-                // all of the tile visible to all of the warp's rows?
-                const bool full = k0 + SA_T <= k_end &&
-                            (k0 + SA_T <= prefix || ((p.window == 0 || k0 >= pos1 - p.window + 1) &&
-                                                     (p.causal ? k0 + SA_T - 1 <= pos0 : p.window == 0 || k0 + SA_T - 1 <= pos0 + p.window - 1)));
+                const bool full = t < full_prefix || (t >= full_from && t < full_to);
                 bool same_doc = true, mixed = false;         // mixed: the half's rows or the tile's keys are of more than one document
                 if (docs != nullptr) {
                     const int2 d = range[t];
@@ -381,7 +392,7 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
                         float top = 0.f;
 #pragma unroll
                         for (int c = 0; c < SA_T; c += 2) top = max3f(top, fabsf(__uint_as_float(S_AT(c))), fabsf(__uint_as_float(S_AT(c + 1))));
-                        if (__all_sync(0xffffffffu, top * to_u <= 1.f)) {
+                        if (__builtin_expect(__all_sync(0xffffffffu, top * to_u <= 1.f), 1)) {
                             const float2 to2 = pk2(to_u, to_u), from2 = pk2(from_u, from_u);
 #pragma unroll
                             for (int c = 0; c < SA_T; c += 2) {
@@ -439,7 +450,7 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
                         }
                     }
                 }
-                if (!full || (mixed && !same_doc)) {
+                if (__builtin_expect(!full || (mixed && !same_doc), 0)) {
                     const uint4 on = visible_keys(see_lo - k0, see_hi - k0, prefix - k0, k_end - k0, mixed && !same_doc ? key_docs[h][done & 1] : nullptr, my_doc);
                     const uint32_t word[4] = {on.x, on.y, on.z, on.w};
 #pragma unroll
@@ -453,13 +464,11 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
                     for (int i = 0; i < 4; ++i) mx[i] = max3f(mx[i], __uint_as_float(S_AT(c + 2 * i)), __uint_as_float(S_AT(c + 2 * i + 1)));
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
                 const bool need = top > m_ref + SA_RESCALE || (m_ref == -INFINITY && top > -INFINITY);
-                if (__any_sync(0xffffffffu, need)) {
+                if (__builtin_expect(__any_sync(0xffffffffu, need), 0)) {
                     float alpha = 1.f;
                     if (need) {
-                        // a whole number, for the polynomial exponential
-                        const float now = fminf(fmaxf(ceilf(top), -2097152.0f), 2097152.0f);
-                        alpha = m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - now);
-                        m_ref = now;
+                        alpha = m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - top);
+                        m_ref = top;
                         l_sum *= alpha;
                     }
                     if (done > 0) {
@@ -473,22 +482,14 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
                     }
                 }
                 const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;
-                const float2 sc2 = pk2(sc, sc), negm2 = pk2(neg_m, neg_m), mm2 = pk2(12582912.0f + neg_m, 12582912.0f + neg_m);
-                const float lo = (-120.0f - neg_m) / sc;
+                const float2 sc2 = pk2(sc, sc), negm2 = pk2(neg_m, neg_m);
                 float2 sum_a = pk2(0.f, 0.f), sum_b = pk2(0.f, 0.f);
 #pragma unroll
                 for (int part = 0; part < 2; ++part) {       // P goes to the issuer in two parts of 64 keys
 #pragma unroll
                     for (int i = part * 32; i < part * 32 + 32; ++i) {
-                        const float s0 = __uint_as_float(S_AT(2 * i)), s1 = __uint_as_float(S_AT(2 * i + 1));
-                        float e0, e1;
-                        if (((i * SA_POLY_PAIRS) & 7) < SA_POLY_PAIRS) {
-                            exp2_poly_pair(s0, s1, lo, sc2, mm2, e0, e1);
-                        } else {
-                            const float2 x = fma2(pk2(s0, s1), sc2, negm2);
-                            e0 = fast_exp2(x.x);
-                            e1 = fast_exp2(x.y);
-                        }
+                        const float2 x = fma2(pk2(__uint_as_float(S_AT(2 * i)), __uint_as_float(S_AT(2 * i + 1))), sc2, negm2);
+                        const float e0 = fast_exp2(x.x), e1 = fast_exp2(x.y);
                         if (i & 1) sum_b = add2(sum_b, pk2(e0, e1));
                         else sum_a = add2(sum_a, pk2(e0, e1));
                         S_AT(i) = pack_pair<BF16>(e0, e1);   // the scores of pair i were used above
@@ -622,7 +623,12 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
                     wait(SB_K_FULL, 0);
 #pragma unroll
                     for (int h = 0; h < HALVES; ++h)
-                        if (wanted(h, t)) qk(h, 0);
+                        if (wanted(h, t)) {
+                            // the second half half a tile behind the first: in step, both would wait for the exponential unit at one time and leave
+                            // it idle at the other (heads of 64 835 -> 786 us over 8192 x 32 x 8192)
+                            if (OWN_P && h == 1 && wanted(0, t)) wait(SB_P0, 0);
+                            qk(h, 0);
+                        }
                     tc_commit_addr(bar0 + 8 * SB_K_EMPTY);
                 }
                 for (unsigned n = 0; t < t_end; ++n) {
