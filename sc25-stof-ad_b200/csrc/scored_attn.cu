@@ -9,8 +9,8 @@ int launch_scored<128>(const ScoredMaps&, const ScoredParams&, int, bool, int, l
 
 namespace {
 
-// A 4-D map of (batch, heads, rows, dim) with boxes of 128 rows x 64 columns; the outer dimensions in the order of their strides
-int make_map(CUtensorMap* map, const void* base, int batch, int heads, int rows, int dim, const long long st[3], int* slot_s, int* slot_h, int* slot_b) {
+// A 4-D map of (batch, heads, rows, dim) with boxes of box_rows x 64 columns; the outer dimensions in the order of their strides
+int make_map(CUtensorMap* map, const void* base, int batch, int heads, int rows, int dim, int box_rows, const long long st[3], int* slot_s, int* slot_h, int* slot_b) {
     struct Dim { uint64_t size; long long stride; int logical; } d[3] = {
         {static_cast<uint64_t>(rows), st[2], 0}, {static_cast<uint64_t>(heads), st[1], 1}, {static_cast<uint64_t>(batch), st[0], 2}};
     for (int i = 0; i < 3; ++i)
@@ -21,7 +21,7 @@ int make_map(CUtensorMap* map, const void* base, int batch, int heads, int rows,
     for (int i = 0; i < 3; ++i) {
         dims[i + 1] = d[i].size;
         strides[i] = static_cast<uint64_t>(d[i].stride) * 2;
-        if (d[i].logical == 0) { box[i + 1] = SA_T; *slot_s = i + 1; }
+        if (d[i].logical == 0) { box[i + 1] = static_cast<uint32_t>(box_rows); *slot_s = i + 1; }
         if (d[i].logical == 1) *slot_h = i + 1;
         if (d[i].logical == 2) *slot_b = i + 1;
     }
@@ -64,8 +64,6 @@ extern "C" int stof_scored_attn(const void* q, const void* k, const void* v, voi
     for (const long long* st : {q_strides, k_strides, v_strides, out_strides})
         for (int i = 0; i < 3; ++i) STOF_REQUIRE(st[i] > 0 && st[i] % 8 == 0, "scored_attn: strides must be positive multiples of 8 elements");
     ScoredParams p;
-    p.out = out;
-    for (int i = 0; i < 3; ++i) p.out_stride[i] = out_strides[i];
     p.slopes = rules->slopes; p.distance_bias = rules->distance_bias; p.documents = rules->documents; p.prefix_lens = rules->prefix_lens;
     p.key_lens = rules->key_lens; p.documents_stride = rules->documents_stride; p.status = status_dev;
     p.scale = rules->softmax_scale; p.softcap = rules->softcap; p.causal = rules->causal != 0; p.radius = rules->bias_radius;
@@ -74,16 +72,18 @@ extern "C" int stof_scored_attn(const void* q, const void* k, const void* v, voi
     p.table_bytes = rules->distance_bias != nullptr ? (2 * p.radius + 1 + 2 * SA_PAD) * 4 + 4 : 0;       // (an even number of words: pairs follow)
     p.range_bytes = rules->documents != nullptr ? (k_len + SA_T - 1) / SA_T * 8 : 0;
     ScoredMaps maps;
-    if (int rc = make_map(&maps[0], q, batch, heads, q_len, head_dim, q_strides, &p.slot_s[0], &p.slot_h[0], &p.slot_b[0])) return rc;
-    if (int rc = make_map(&maps[1], k, batch, kv_heads, k_len, head_dim, k_strides, &p.slot_s[1], &p.slot_h[1], &p.slot_b[1])) return rc;
-    if (int rc = make_map(&maps[2], v, batch, kv_heads, k_len, head_dim, v_strides, &p.slot_s[2], &p.slot_h[2], &p.slot_b[2])) return rc;
+    if (int rc = make_map(&maps[0], q, batch, heads, q_len, head_dim, SA_T, q_strides, &p.slot_s[0], &p.slot_h[0], &p.slot_b[0])) return rc;
+    if (int rc = make_map(&maps[1], k, batch, kv_heads, k_len, head_dim, SA_T, k_strides, &p.slot_s[1], &p.slot_h[1], &p.slot_b[1])) return rc;
+    if (int rc = make_map(&maps[2], v, batch, kv_heads, k_len, head_dim, SA_T, v_strides, &p.slot_s[2], &p.slot_h[2], &p.slot_b[2])) return rc;
+    if (int rc = make_map(&maps[3], out, batch, heads, q_len, head_dim, 32, out_strides, &p.slot_s[3], &p.slot_h[3], &p.slot_b[3])) return rc;
     // two halves to a block where that leaves a block for every multiprocessor
     const long long pairs = static_cast<long long>(batch) * heads;
     const int halves = pairs * ((q_len + 2 * SA_T - 1) / (2 * SA_T)) >= sm_count() ? 2 : 1;
     p.q_tiles = (q_len + halves * SA_T - 1) / (halves * SA_T);
     STOF_REQUIRE(pairs * p.q_tiles < (1ll << 31), "scored_attn: batch * heads * query tiles beyond 2^31");
     const size_t smem = 1024 + static_cast<size_t>(halves + 4) * SA_T * head_dim * 2 + p.table_bytes + p.range_bytes;
-    const int mode = p.slopes != nullptr || p.distance_bias != nullptr ? SA_ANY : p.softcap > 0.f ? SA_CAP : SA_PLAIN;
+    int mode = p.slopes != nullptr || p.distance_bias != nullptr ? SA_ANY : p.softcap > 0.f ? SA_CAP : SA_PLAIN;
+    if (p.documents != nullptr) mode = (mode == SA_PLAIN ? SA_PLAIN : SA_ANY) | SA_DOCS;
     const bool bf16 = dtype == STOF_DTYPE_BF16;
     return head_dim == 64 ? launch_scored<64>(maps, p, halves, bf16, mode, pairs * p.q_tiles, smem, stream)
                           : launch_scored<128>(maps, p, halves, bf16, mode, pairs * p.q_tiles, smem, stream);

@@ -25,11 +25,9 @@ constexpr int SA_T = 128;                    // rows of a half, keys of a tile
 constexpr int SA_PAD = 256;                  // the distance table in shared memory goes on for so long on both sides: a tile that meets the table needs no clamp
 constexpr float SA_RESCALE = 8.0f;           // log2 units by which a row's maximum may outgrow the reference of its P (P <= 2^8)
 constexpr float SA_LOG2E = 1.4426950408889634f;
-enum { SA_PLAIN = 0, SA_CAP = 1, SA_ANY = 2 };       // what is done to scores: nothing, the cap alone, whatever the call asks for
+enum { SA_PLAIN = 0, SA_CAP = 1, SA_ANY = 2, SA_DOCS = 4 };   // what is done to scores: nothing, the cap alone, whatever the call asks for; and documents
 
 struct ScoredParams {
-    void* out;
-    long long out_stride[3];
     const float *slopes, *distance_bias;
     const int *documents, *prefix_lens, *key_lens;
     long long documents_stride;
@@ -37,12 +35,12 @@ struct ScoredParams {
     float scale, softcap;
     int causal, window, radius;
     int batch, heads, group, q_len, k_len, q_tiles;
-    int slot_s[3], slot_h[3], slot_b[3];     // of q, k, v: which coordinate of the tensor map is the row, the head, the batch
+    int slot_s[4], slot_h[4], slot_b[4];     // of q, k, v, out: which coordinate of the tensor map is the row, the head, the batch
     int table_bytes, range_bytes;
 };
 
-// barriers, two of each (a half's, or a slot's): Q is there; S is there; parts 0 and 1 of P are there; S has been read; O is complete (OWN_P: up
-// to the last P, else the whole); slots
+// barriers, two of each (a half's, or a slot's): Q is there; S is there; parts 0 and 1 of P are there; S has been read; O is complete up
+// to the last P; slots
 enum { SB_Q = 0, SB_S = 2, SB_P0 = 4, SB_P1 = 6, SB_READ = 8, SB_O = 10, SB_FIX = 12, SB_K_FULL = 13, SB_K_EMPTY = 15, SB_V_FULL = 17, SB_V_EMPTY = 19, SB_COUNT = 21 };
 
 static __device__ __forceinline__ void load_tile(unsigned char* dst, const CUtensorMap* map, uint64_t* bar, int col, int row, int head, int batch, int slot_s, int slot_h) {
@@ -51,6 +49,13 @@ static __device__ __forceinline__ void load_tile(unsigned char* dst, const CUten
     const int c2 = slot_s == 2 ? row : slot_h == 2 ? head : batch;
     const int c3 = slot_s == 3 ? row : slot_h == 3 ? head : batch;
     tma_load_4d(dst, map, bar, col, c1, c2, c3);
+}
+
+static __device__ __forceinline__ void store_rows(const CUtensorMap* map, const unsigned char* src, int col, int row, int head, int batch, int slot_s, int slot_h) {
+    const int c1 = slot_s == 1 ? row : slot_h == 1 ? head : batch;
+    const int c2 = slot_s == 2 ? row : slot_h == 2 ? head : batch;
+    const int c3 = slot_s == 3 ? row : slot_h == 3 ? head : batch;
+    tma_store_4d(map, src, col, c1, c2, c3);
 }
 
 static __device__ __forceinline__ float max3f(float a, float b, float c) {
@@ -101,9 +106,8 @@ static __device__ __forceinline__ void cap_in_tmem(uint32_t t_s, float to_u, flo
     tc_wait_st();
 }
 
-// Bits of the 128 keys of a tile that a row sees: those in [from, to] or in front of `front`, and in front of `end` (all relative to the
-// tile); and, with `stage`, those whose document is the row's.
-static __device__ __forceinline__ uint4 visible_keys(int from, int to, int front, int end, const int* stage, int my_doc) {
+// Bits of the 128 keys of a tile that a row sees: those in [from, to] or in front of `front`, and in front of `end` (all relative to the tile).
+static __device__ __forceinline__ uint4 visible_keys(int from, int to, int front, int end) {
     // bits lo .. hi of word w
     auto bits = [](int lo, int hi, int w) -> uint32_t {
         lo -= 32 * w;
@@ -114,18 +118,7 @@ static __device__ __forceinline__ uint4 visible_keys(int from, int to, int front
     };
     uint32_t r[4];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        r[w] = (bits(from, to, w) | bits(0, front - 1, w)) & bits(0, end - 1, w);
-        if (stage != nullptr) {
-            uint32_t same = 0;
-#pragma unroll
-            for (int c = 0; c < 32; c += 4) {
-                const int4 k = *reinterpret_cast<const int4*>(stage + 32 * w + c);
-                same |= (k.x == my_doc ? 1u << c : 0u) | (k.y == my_doc ? 2u << c : 0u) | (k.z == my_doc ? 4u << c : 0u) | (k.w == my_doc ? 8u << c : 0u);
-            }
-            r[w] &= same;
-        }
-    }
+    for (int w = 0; w < 4; ++w) r[w] = (bits(from, to, w) | bits(0, front - 1, w)) & bits(0, end - 1, w);
     return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
@@ -187,9 +180,12 @@ struct Reach {
     int lo, hi, prefix, doc_min, doc_max;
 };
 
-template <int D, int HALVES, bool BF16, int MODE>
-__global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64 && MODE != SA_ANY ? 2 : 1) scored_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                                                                        const __grid_constant__ CUtensorMap map_v, const ScoredParams p) {
+template <int D, int HALVES, bool BF16, int WHAT>
+__global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64 && (WHAT & SA_ANY) == 0 ? 2 : 1) scored_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                                        const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_o,
+                                                                        const ScoredParams p) {
+    constexpr int MODE = WHAT & 3;
+    constexpr bool DOCS = (WHAT & SA_DOCS) != 0;
     constexpr int PANELS = D / 64;                           // 64-column panels of a tile, 128 rows of 128 swizzled bytes each
     constexpr int PANEL_BYTES = SA_T * 128, TILE_BYTES = PANELS * PANEL_BYTES;
     constexpr int W_LOAD = HALVES * 4, W_MMA = W_LOAD + 1;
@@ -211,7 +207,12 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int* abort_flag = &abort_word;
     const WaitCtx wctx{abort_flag, p.status};
-    if (threadIdx.x == 0) {
+    const bool loader = warp == W_LOAD && lane == 0;
+    if (loader) {
+        tma_prefetch_desc(&map_q);
+        tma_prefetch_desc(&map_k);
+        tma_prefetch_desc(&map_v);
+        tma_prefetch_desc(&map_o);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bars[SB_Q + i], 1);
             mbar_init(&bars[SB_S + i], 1);
@@ -235,7 +236,7 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
     }
     grid_dependency_wait();
     grid_launch_dependents();
-    if (threadIdx.x == 0) *abort_flag = failure_reported(p.status) ? 1 : 0;
+    if (loader) *abort_flag = failure_reported(p.status) ? 1 : 0;
 
     // the heaviest stretches first: with a causal mask those at the end of the sequence
     const int heads_all = p.batch * p.heads;
@@ -244,7 +245,7 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
     const int q0 = row_tile * (SA_T * HALVES), shift = p.k_len - p.q_len;
     const int k_end = p.key_lens != nullptr ? min(max(p.key_lens[b], 0), p.k_len) : p.k_len;
     const int prefix = p.prefix_lens != nullptr ? min(max(p.prefix_lens[b], 0), k_end) : 0;
-    const int* docs = p.documents != nullptr ? p.documents + b * p.documents_stride : nullptr;
+    const int* docs = DOCS ? p.documents + b * p.documents_stride : nullptr;
 
     auto reach_of = [&](int h) {
         Reach r = {0, 0, 0, 0, 0};
@@ -266,13 +267,48 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
         if (reach[h].hi > 0) t_begin = min(t_begin, reach[h].prefix > 0 ? 0 : reach[h].lo);
         t_end = max(t_end, reach[h].hi);
     }
+    auto wanted_by = [&](const Reach& r, int t) {
+        if (t >= r.hi || (t < r.lo && t >= r.prefix)) return false;
+        if (!DOCS) return true;
+        const int2 d = range[t];
+        return d.x <= r.doc_max && d.y >= r.doc_min;
+    };
+    auto wanted = [&](int h, int t) { return wanted_by(reach[h], t); };     // (h known to the compiler: `reach` stays in registers)
+    auto next = [&](int t) {                                 // first tile from t on that a half wants
+        for (; t < t_end; ++t) {
+            bool any = wanted(0, t);
+            if constexpr (HALVES == 2) any = any || wanted(1, t);
+            if (any) break;
+        }
+        return t;
+    };
+    // the n-th tile goes into slot n % 2 of its side, K a tile ahead of V
+    auto load = [&](int kind, int t, unsigned n) {
+        const int s = static_cast<int>(n & 1);
+        uint64_t *full = &bars[(kind == 0 ? SB_K_FULL : SB_V_FULL) + s], *empty = &bars[(kind == 0 ? SB_K_EMPTY : SB_V_EMPTY) + s];
+        wait_inline(smem_u32(empty), ((n >> 1) & 1) ^ 1, wctx, (kind == 0 ? SB_K_EMPTY : SB_V_EMPTY) + s);
+        mbar_arrive_expect_tx(full, TILE_BYTES);
+        for (int c = 0; c < PANELS; ++c)
+            load_tile(ring + (2 * kind + s) * TILE_BYTES + c * PANEL_BYTES, kind == 0 ? &map_k : &map_v, full, c * 64, t * SA_T, kv, b, p.slot_s[1 + kind],
+                      p.slot_h[1 + kind]);
+    };
+    // Q, and the first K where the rules alone say which that is, are on their way while the rest is set up
+    if (loader && *abort_flag == 0) {
+        for (int h = 0; h < HALVES; ++h) {
+            if (q0 + h * SA_T >= p.q_len) break;
+            mbar_arrive_expect_tx(&bars[SB_Q + h], TILE_BYTES);
+            for (int c = 0; c < PANELS; ++c)
+                load_tile(q_smem + h * TILE_BYTES + c * PANEL_BYTES, &map_q, &bars[SB_Q + h], c * 64, q0 + h * SA_T, head, b, p.slot_s[0], p.slot_h[0]);
+            if (h == 0 && !DOCS && next(t_begin) < t_end) load(0, next(t_begin), 0);
+        }
+    }
     // tables into shared memory
     if (p.distance_bias != nullptr) {
         const float* src = p.distance_bias + static_cast<size_t>(head) * (2 * p.radius + 1);
         for (int i = threadIdx.x; i < 2 * p.radius + 1 + 2 * SA_PAD; i += blockDim.x) table[i] = __ldca(src + min(max(i - SA_PAD, 0), 2 * p.radius)) * SA_LOG2E;
     }
     int my_doc = 0;
-    if (docs != nullptr) {
+    if (DOCS) {
         for (int t = t_begin + warp; t < t_end; t += scored_threads(HALVES) / 32) {
             int lo = 0x7FFFFFFF, hi = -0x7FFFFFFF - 1;
 #pragma unroll
@@ -299,28 +335,13 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    if (docs != nullptr) {
+    if (DOCS) {
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) {
             reach[h].doc_min = min(min(row_docs[4 * h].x, row_docs[4 * h + 1].x), min(row_docs[4 * h + 2].x, row_docs[4 * h + 3].x));
             reach[h].doc_max = max(max(row_docs[4 * h].y, row_docs[4 * h + 1].y), max(row_docs[4 * h + 2].y, row_docs[4 * h + 3].y));
         }
     }
-    auto wanted_by = [&](const Reach& r, int t) {
-        if (t >= r.hi || (t < r.lo && t >= r.prefix)) return false;
-        if (docs == nullptr) return true;
-        const int2 d = range[t];
-        return d.x <= r.doc_max && d.y >= r.doc_min;
-    };
-    auto wanted = [&](int h, int t) { return wanted_by(reach[h], t); };     // (h known to the compiler: `reach` stays in registers)
-    auto next = [&](int t) {                                 // first tile from t on that a half wants
-        for (; t < t_end; ++t) {
-            bool any = wanted(0, t);
-            if constexpr (HALVES == 2) any = any || wanted(1, t);
-            if (any) break;
-        }
-        return t;
-    };
     // the tile in which the keys end before the tensor does: what V holds there behind the last key is set to zero (P is zero there,
     // but zero times a NaN is none)
     const int fix_tile = k_end < p.k_len && k_end % SA_T != 0 ? k_end / SA_T : -1;
@@ -331,7 +352,7 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
             // ---------------------------------------------------------------- softmax: one row a thread
             const int h = HALVES == 2 ? warp >> 2 : 0, tid = threadIdx.x & 127;
             Reach mine = reach_of(h);
-            if (docs != nullptr) {
+            if (DOCS) {
                 for (int i = 0; i < 4; ++i) {
                     const int2 d = row_docs[4 * h + i];
                     mine.doc_min = i == 0 ? d.x : min(mine.doc_min, d.x);
@@ -350,32 +371,35 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
             const float raw_scale = p.scale * SA_LOG2E;      // of a score that nothing changes, to log2 units
             const float sc = changed ? 1.f : raw_scale;      // what is left to multiply by when the exponential is taken
             const float slope = p.slopes != nullptr ? __ldca(p.slopes + head) * SA_LOG2E : 0.f;
-            const int2 warp_docs = docs != nullptr ? row_docs[warp] : make_int2(0, 0);
+            const int2 warp_docs = DOCS ? row_docs[warp] : make_int2(0, 0);
             const int see_lo = p.window > 0 ? pos - p.window + 1 : -0x40000000, see_hi = p.causal ? pos : p.window > 0 ? pos + p.window - 1 : 0x40000000;
             // the tiles of which all is visible to all of the warp's rows (documents aside): [0, full_prefix) and [full_from, full_to)
             const int full_prefix = prefix / SA_T, full_from = p.window > 0 ? max(pos1 - p.window + SA_T, 0) / SA_T : 0;
             const int full_to = max(min(p.causal ? pos0 + 1 : p.window > 0 ? pos0 + p.window : p.k_len, k_end), 0) / SA_T;
             float m_ref = -INFINITY, l_sum = 0.f;
+            int doc_tile = -1, doc_ahead = 0;
             int done = 0;
             for (int t = mine.prefix > 0 ? 0 : mine.lo; t < mine.hi; ++t) {
                 if (t < mine.lo && t >= mine.prefix) {                       // from the prefix to the window
                     t = mine.lo;
                     if (t >= mine.hi) break;
                 }
-                if (docs != nullptr) {
+                if (DOCS) {
                     const int2 d = range[t];
                     if (d.x > mine.doc_max || d.y < mine.doc_min) continue;
                 }
                 const int k0 = t * SA_T;
                 const bool full = t < full_prefix || (t >= full_from && t < full_to);
                 bool same_doc = true, mixed = false;         // mixed: the half's rows or the tile's keys are of more than one document
-                if (docs != nullptr) {
+                if (DOCS) {
                     const int2 d = range[t];
                     same_doc = d.x == d.y && warp_docs.x == warp_docs.y && d.x == warp_docs.x;
                     mixed = d.x != d.y || mine.doc_min != mine.doc_max;
                     if (mixed) {                             // the keys' documents, 128 threads together: all warps of the half or none
                         int* stage = key_docs[h][done & 1];
-                        stage[tid] = k0 + tid < k_end ? __ldca(docs + k0 + tid) : 0;
+                        stage[tid] = t == doc_tile ? doc_ahead : k0 + tid < k_end ? __ldca(docs + k0 + tid) : 0;
+                        doc_tile = t + 1;                    // most likely the next one
+                        doc_ahead = k0 + SA_T + tid < k_end ? __ldca(docs + k0 + SA_T + tid) : 0;
                         if (HALVES == 1 || h == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
                         else asm volatile("bar.sync 2, 128;" ::: "memory");
                     }
@@ -414,31 +438,35 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
                     if (lane == 0) mbar_arrive(&bars[SB_READ + h]);
                 }
                 if constexpr (MODE == SA_ANY) {
-                    const float2 scale2 = capped ? pk2(1.f, 1.f) : pk2(raw_scale, raw_scale);
+                    float sc_now = capped ? 1.f : raw_scale;
                     // distances of the warp's rows in this tile: k0 - pos1 .. k0 + 127 - pos0
                     const int near = k0 - pos1, far = k0 + SA_T - 1 - pos0;
-                    if (far <= 0 || near >= 0) {             // all behind or all ahead: -slope * |distance| is linear (0 without slopes)
-                        const float g = far <= 0 ? slope : -slope, at = g * static_cast<float>(k0 - pos);
+                    if (p.slopes != nullptr) {
+                        if (far <= 0 || near >= 0) {         // all behind or all ahead: -slope * |distance| is linear
+                            const float g = far <= 0 ? slope : -slope, at = g * static_cast<float>(k0 - pos);
+                            const float2 now2 = pk2(sc_now, sc_now), g2 = pk2(g, g), at2 = pk2(at, at);
 #pragma unroll
-                        for (int c = 0; c < SA_T; c += 2) {
-                            const float2 y = fma2(pk2(__uint_as_float(S_AT(c)), __uint_as_float(S_AT(c + 1))), scale2,
-                                                  fma2(pk2(g, g), pk2(static_cast<float>(c), static_cast<float>(c + 1)), pk2(at, at)));
-                            S_AT(c) = __float_as_uint(y.x);
-                            S_AT(c + 1) = __float_as_uint(y.y);
+                            for (int c = 0; c < SA_T; c += 2) {
+                                const float2 y = fma2(pk2(__uint_as_float(S_AT(c)), __uint_as_float(S_AT(c + 1))), now2,
+                                                      fma2(g2, pk2(static_cast<float>(c), static_cast<float>(c + 1)), at2));
+                                S_AT(c) = __float_as_uint(y.x);
+                                S_AT(c + 1) = __float_as_uint(y.y);
+                            }
+                        } else {
+                            const float away = static_cast<float>(k0 - pos);
+#pragma unroll
+                            for (int c = 0; c < SA_T; ++c)
+                                S_AT(c) = __float_as_uint(fmaf(__uint_as_float(S_AT(c)), sc_now, -slope * fabsf(away + static_cast<float>(c))));
                         }
-                    } else {
-                        const float away = static_cast<float>(k0 - pos);
-#pragma unroll
-                        for (int c = 0; c < SA_T; ++c)
-                            S_AT(c) = __float_as_uint(fmaf(__uint_as_float(S_AT(c)), scale2.x, -slope * fabsf(away + static_cast<float>(c))));
+                        sc_now = 1.f;
                     }
                     if (p.distance_bias != nullptr) {
                         if (far <= -p.radius || near >= p.radius) {          // all of it beyond the table
                             const float x = table[near >= p.radius ? 2 * p.radius + SA_PAD : SA_PAD];
-                            const float2 x2 = pk2(x, x);
+                            const float2 x2 = pk2(x, x), now2 = pk2(sc_now, sc_now);
 #pragma unroll
                             for (int c = 0; c < SA_T; c += 2) {
-                                const float2 y = add2(pk2(__uint_as_float(S_AT(c)), __uint_as_float(S_AT(c + 1))), x2);
+                                const float2 y = fma2(pk2(__uint_as_float(S_AT(c)), __uint_as_float(S_AT(c + 1))), now2, x2);
                                 S_AT(c) = __float_as_uint(y.x);
                                 S_AT(c + 1) = __float_as_uint(y.y);
                             }
@@ -446,16 +474,27 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
                             // (rows behind the last one are kept inside the table)
                             const float* at = table + min(max(k0 - pos + p.radius + SA_PAD, 0), 2 * p.radius + 2 * SA_PAD - SA_T + 1);
 #pragma unroll
-                            for (int c = 0; c < SA_T; ++c) S_AT(c) = __float_as_uint(__uint_as_float(S_AT(c)) + at[c]);
+                            for (int c = 0; c < SA_T; ++c) S_AT(c) = __float_as_uint(fmaf(__uint_as_float(S_AT(c)), sc_now, at[c]));
                         }
                     }
                 }
-                if (__builtin_expect(!full || (mixed && !same_doc), 0)) {
-                    const uint4 on = visible_keys(see_lo - k0, see_hi - k0, prefix - k0, k_end - k0, mixed && !same_doc ? key_docs[h][done & 1] : nullptr, my_doc);
+                if (__builtin_expect(!full, 0)) {
+                    const uint4 on = visible_keys(see_lo - k0, see_hi - k0, prefix - k0, k_end - k0);
                     const uint32_t word[4] = {on.x, on.y, on.z, on.w};
 #pragma unroll
                     for (int c = 0; c < SA_T; ++c)
                         if ((word[c >> 5] & (1u << (c & 31))) == 0) S_AT(c) = 0xFF800000u;
+                }
+                if (__builtin_expect(mixed && !same_doc, 0)) {
+                    const int* stage = key_docs[h][done & 1];
+#pragma unroll
+                    for (int c = 0; c < SA_T; c += 4) {
+                        const int4 k = *reinterpret_cast<const int4*>(stage + c);
+                        S_AT(c) = k.x == my_doc ? S_AT(c) : 0xFF800000u;
+                        S_AT(c + 1) = k.y == my_doc ? S_AT(c + 1) : 0xFF800000u;
+                        S_AT(c + 2) = k.z == my_doc ? S_AT(c + 2) : 0xFF800000u;
+                        S_AT(c + 3) = k.w == my_doc ? S_AT(c + 3) : 0xFF800000u;
+                    }
                 }
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -510,28 +549,43 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
                 ++done;
             }
             // ---------------------------------------------------------------- O / l
+            // The rows leave through shared memory, 32 of a warp at a time, over the half's Q: every product that read it is complete.  (Stored
+            // from registers, each lane its row, they took 1200 cycles a warp for heads of 64 and up to 6000 for heads of 128.)
             if (done > 0) {
-                mbar_wait(&bars[SB_O + h], OWN_P ? static_cast<uint32_t>((done - 1) & 1) : 0u, wctx, SB_O + h);
+                wait_inline(smem_u32(&bars[SB_O + h]), static_cast<uint32_t>((done - 1) & 1), wctx, SB_O + h);
                 tc_fence_after();
+            } else if (q0 + h * SA_T < p.q_len) {
+                wait_inline(smem_u32(&bars[SB_Q + h]), 0, wctx, SB_Q + h);       // nobody used it: it may still be on its way
             }
             // a row that saw nothing has no maximum; where all it saw is NaN its sum says so
             const bool any = done > 0 && (m_ref > -INFINITY || l_sum != l_sum);
             const float inv = any ? 1.f / l_sum : 0.f;
-            uint16_t* dst = static_cast<uint16_t*>(p.out) + b * p.out_stride[0] + head * p.out_stride[1] + static_cast<long long>(row) * p.out_stride[2];
+            if (warp_row < p.q_len) {
 #pragma unroll
-            for (int c = 0; c < D; c += 32) {
-                uint32_t o[32];
-                if (done > 0) {
-                    tmem_ld32(t_o + c, o);
-                    tc_wait_ld();
-                }
-                if (row < p.q_len) {
+                for (int c = 0; c < PANELS; ++c) {
+                    unsigned char* slab = q_smem + h * TILE_BYTES + c * PANEL_BYTES + (warp & 3) * 4096;
+                    uint32_t o[2][32];
+                    if (done > 0) {
+                        tmem_ld32(t_o + 64 * c, o[0]);
+                        tmem_ld32(t_o + 64 * c + 32, o[1]);
+                        tc_wait_ld();
+                    }
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        auto two = [&](int j) { return any ? pack_pair<BF16>(__uint_as_float(o[i + j]) * inv, __uint_as_float(o[i + j + 1]) * inv) : 0u; };
-                        *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(two(0), two(2), two(4), two(6));
+                    for (int i = 0; i < 8; ++i) {
+                        auto two = [&](int j) {
+                            const int k = 8 * i + j;
+                            return any ? pack_pair<BF16>(__uint_as_float(o[k >> 5][k & 31]) * inv, __uint_as_float(o[k >> 5][(k & 31) + 1]) * inv) : 0u;
+                        };
+                        *reinterpret_cast<uint4*>(slab + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(two(0), two(2), two(4), two(6));
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        store_rows(&map_o, slab, 64 * c, warp_row, head, b, p.slot_s[3], p.slot_h[3]);
+                        tma_store_commit();
                     }
                 }
+                if (lane == 0) tma_store_wait_all();
             }
         }
     } else {
@@ -541,29 +595,8 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
             int fix_slot = -1;
             uint32_t fix_phase = 0;
             if (lane == 0) {
-                tma_prefetch_desc(&map_q);
-                tma_prefetch_desc(&map_k);
-                tma_prefetch_desc(&map_v);
-                // the n-th tile goes into slot n % 2 of its side, K a tile ahead of V
-                auto load = [&](int kind, int t, unsigned n) {
-                    const int s = static_cast<int>(n & 1);
-                    uint64_t *full = &bars[(kind == 0 ? SB_K_FULL : SB_V_FULL) + s], *empty = &bars[(kind == 0 ? SB_K_EMPTY : SB_V_EMPTY) + s];
-                    wait_inline(smem_u32(empty), ((n >> 1) & 1) ^ 1, wctx, (kind == 0 ? SB_K_EMPTY : SB_V_EMPTY) + s);
-                    mbar_arrive_expect_tx(full, TILE_BYTES);
-                    for (int c = 0; c < PANELS; ++c)
-                        load_tile(ring + (2 * kind + s) * TILE_BYTES + c * PANEL_BYTES, kind == 0 ? &map_k : &map_v, full, c * 64, t * SA_T, kv, b, p.slot_s[1 + kind],
-                                  p.slot_h[1 + kind]);
-                };
                 int t = next(t_begin);
-                if (t < t_end) {
-                    for (int h = 0; h < HALVES; ++h) {
-                        if (q0 + h * SA_T >= p.q_len) break;
-                        mbar_arrive_expect_tx(&bars[SB_Q + h], TILE_BYTES);
-                        for (int c = 0; c < PANELS; ++c)
-                            load_tile(q_smem + h * TILE_BYTES + c * PANEL_BYTES, &map_q, &bars[SB_Q + h], c * 64, q0 + h * SA_T, head, b, p.slot_s[0], p.slot_h[0]);
-                        if (h == 0) load(0, t, 0);
-                    }
-                }
+                if (DOCS && t < t_end) load(0, t, 0);
                 for (unsigned n = 0; t < t_end; ++n) {
                     const int tn = next(t + 1);
                     if (tn < t_end) load(0, tn, n + 1);
@@ -615,7 +648,7 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
                     wait(SB_P1 + h, parity);
                     tc_fence_after();
                     mma_chain_ts(o, q + 32, v + 512, idesc_pv, 1u);
-                    if constexpr (OWN_P) tc_commit_addr(bar0 + 8 * (SB_O + h));
+                    tc_commit_addr(bar0 + 8 * (SB_O + h));
                     ++done[h];
                 };
                 int t = next(t_begin);
@@ -658,10 +691,6 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
                         if (tn < t_end) tc_commit_addr(bar0 + 8 * (SB_K_EMPTY + ks));
                     t = tn;
                 }
-                if constexpr (!OWN_P) {
-#pragma unroll
-                    for (int h = 0; h < HALVES; ++h) tc_commit_addr(bar0 + 8 * (SB_O + h));
-                }
             }
         }
     }
@@ -674,7 +703,7 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
 }
 
 
-using ScoredMaps = CUtensorMap[3];
+using ScoredMaps = CUtensorMap[4];             // q, k, v, out
 // Launches the kernel for one head size (scored_attn_64.cu, scored_attn_128.cu: a translation unit each, they take long to compile)
 template <int D>
 int launch_scored(const ScoredMaps& maps, const ScoredParams& p, int halves, bool bf16, int mode, long long blocks, size_t smem, cudaStream_t stream);
@@ -684,15 +713,19 @@ int launch_scored_impl(const ScoredMaps& maps, const ScoredParams& p, int halves
     auto launch = [&](auto kernel) -> int {
         STOF_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
         LaunchConfig lc(dim3(static_cast<unsigned>(blocks)), static_cast<unsigned>(scored_threads(halves)), smem, stream);
-        STOF_CUDA(cudaLaunchKernelEx(&lc.cfg, kernel, maps[0], maps[1], maps[2], p));
+        STOF_CUDA(cudaLaunchKernelEx(&lc.cfg, kernel, maps[0], maps[1], maps[2], maps[3], p));
         return STOF_OK;
     };
     auto by_mode = [&](auto h, auto b) -> int {
         constexpr int H = decltype(h)::value;
         constexpr bool B = decltype(b)::value;
-        if (mode == SA_PLAIN) return launch(scored_attn_kernel<D, H, B, SA_PLAIN>);
-        if (mode == SA_CAP) return launch(scored_attn_kernel<D, H, B, SA_CAP>);
-        return launch(scored_attn_kernel<D, H, B, SA_ANY>);
+        switch (mode) {
+            case SA_PLAIN: return launch(scored_attn_kernel<D, H, B, SA_PLAIN>);
+            case SA_CAP: return launch(scored_attn_kernel<D, H, B, SA_CAP>);
+            case SA_ANY: return launch(scored_attn_kernel<D, H, B, SA_ANY>);
+            case SA_PLAIN | SA_DOCS: return launch(scored_attn_kernel<D, H, B, SA_PLAIN | SA_DOCS>);
+            default: return launch(scored_attn_kernel<D, H, B, SA_ANY | SA_DOCS>);
+        }
     };
     using std::integral_constant;
     if (halves == 2) return bf16 ? by_mode(integral_constant<int, 2>{}, std::true_type{}) : by_mode(integral_constant<int, 2>{}, std::false_type{});
