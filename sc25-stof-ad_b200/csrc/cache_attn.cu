@@ -657,6 +657,16 @@ Shape shape_of(int requests, int tokens, int heads, int kv_heads, int page_size,
     return s;
 }
 
+template <int NT, int D, bool E4M3>
+int launch(const CacheAttnParams& p, const Shape& s, cudaStream_t stream) {
+    if (int rc = allow_shared_memory<cache_attn_kernel<NT, D, E4M3>>()) return rc;
+    LaunchConfig lc(dim3(static_cast<unsigned>(s.blocks)), CT_THREADS, CT_WARPS * Ring<D>::BYTES, stream);
+    STOF_CUDA(cudaLaunchKernelEx(&lc.cfg, cache_attn_kernel<NT, D, E4M3>, p));
+    LaunchConfig lj(dim3(static_cast<unsigned>(s.joins), static_cast<unsigned>(s.rows < 8 * NT ? s.rows : 8 * NT)), CT_THREADS, 0, stream);
+    STOF_CUDA(cudaLaunchKernelEx(&lj.cfg, cache_attn_join_kernel<NT, D>, p));
+    return STOF_OK;
+}
+
 }  // namespace
 }  // namespace stof
 
@@ -717,20 +727,11 @@ extern "C" int stof_cache_attn(const void* q, void* out, int dtype, const long l
     p.table_width = table_width; p.page_count = pages; p.bf16 = dtype == STOF_DTYPE_BF16;
     p.page_shift = 0;
     while ((1 << p.page_shift) < page_size) ++p.page_shift;
-    auto launch = [&](auto kernel, auto join) -> int {
-        const int smem = CT_WARPS * (head_dim == 64 ? Ring<64>::BYTES : Ring<128>::BYTES);
-        STOF_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        LaunchConfig lc(dim3(static_cast<unsigned>(s.blocks)), CT_THREADS, static_cast<size_t>(smem), stream);
-        STOF_CUDA(cudaLaunchKernelEx(&lc.cfg, kernel, p));
-        LaunchConfig lj(dim3(static_cast<unsigned>(s.joins), static_cast<unsigned>(s.rows < 8 * s.nt ? s.rows : 8 * s.nt)), CT_THREADS, 0, stream);
-        STOF_CUDA(cudaLaunchKernelEx(&lj.cfg, join, p));
-        return STOF_OK;
-    };
     const bool e4m3 = cache_dtype == STOF_DTYPE_E4M3;
     if (head_dim == 64) {
-        if (s.nt == 1) return e4m3 ? launch(cache_attn_kernel<1, 64, true>, cache_attn_join_kernel<1, 64>) : launch(cache_attn_kernel<1, 64, false>, cache_attn_join_kernel<1, 64>);
-        return e4m3 ? launch(cache_attn_kernel<2, 64, true>, cache_attn_join_kernel<2, 64>) : launch(cache_attn_kernel<2, 64, false>, cache_attn_join_kernel<2, 64>);
+        if (s.nt == 1) return e4m3 ? launch<1, 64, true>(p, s, stream) : launch<1, 64, false>(p, s, stream);
+        return e4m3 ? launch<2, 64, true>(p, s, stream) : launch<2, 64, false>(p, s, stream);
     }
-    if (s.nt == 1) return e4m3 ? launch(cache_attn_kernel<1, 128, true>, cache_attn_join_kernel<1, 128>) : launch(cache_attn_kernel<1, 128, false>, cache_attn_join_kernel<1, 128>);
-    return e4m3 ? launch(cache_attn_kernel<2, 128, true>, cache_attn_join_kernel<2, 128>) : launch(cache_attn_kernel<2, 128, false>, cache_attn_join_kernel<2, 128>);
+    if (s.nt == 1) return e4m3 ? launch<1, 128, true>(p, s, stream) : launch<1, 128, false>(p, s, stream);
+    return e4m3 ? launch<2, 128, true>(p, s, stream) : launch<2, 128, false>(p, s, stream);
 }

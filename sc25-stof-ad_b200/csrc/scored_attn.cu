@@ -76,12 +76,18 @@ extern "C" int stof_scored_attn(const void* q, const void* k, const void* v, voi
     if (int rc = make_map(&maps[1], k, batch, kv_heads, k_len, head_dim, SA_T, k_strides, &p.slot_s[1], &p.slot_h[1], &p.slot_b[1])) return rc;
     if (int rc = make_map(&maps[2], v, batch, kv_heads, k_len, head_dim, SA_T, v_strides, &p.slot_s[2], &p.slot_h[2], &p.slot_b[2])) return rc;
     if (int rc = make_map(&maps[3], out, batch, heads, q_len, head_dim, 32, out_strides, &p.slot_s[3], &p.slot_h[3], &p.slot_b[3])) return rc;
-    // two halves to a block where that leaves a block for every multiprocessor
     const long long pairs = static_cast<long long>(batch) * heads;
-    const int halves = pairs * ((q_len + 2 * SA_T - 1) / (2 * SA_T)) >= sm_count() ? 2 : 1;
+    // Heads of 64: one half, two blocks on an SM, which cover each other's beginnings and ends (8192 x 32 x 8192: causal 375 us against
+    // 388 with two halves, 8 x 1001 with a table 79 against 83).  Heads of 128: two halves share their tiles (859 us against 949), in
+    // whole rounds of blocks, though; single halves go round in blocks half as long, of which the last run alone on their SM (2 x 32 x
+    // 2048 queries, 3.46 rounds: 128 us against 139).  Costs in rounds of two halves:
+    const long long sms = sm_count(), single = pairs * ((q_len + SA_T - 1) / SA_T), doubled = pairs * ((q_len + 2 * SA_T - 1) / (2 * SA_T));
+    const long long over = single % (2 * sms);
+    const double rounds1 = static_cast<double>(single / (2 * sms)) + (over == 0 ? 0.0 : over <= sms ? 0.62 : 1.0);
+    const int halves = head_dim == 64 || 1.07 * rounds1 < static_cast<double>((doubled + sms - 1) / sms) ? 1 : 2;
     p.q_tiles = (q_len + halves * SA_T - 1) / (halves * SA_T);
     STOF_REQUIRE(pairs * p.q_tiles < (1ll << 31), "scored_attn: batch * heads * query tiles beyond 2^31");
-    const size_t smem = 1024 + static_cast<size_t>(halves + 4) * SA_T * head_dim * 2 + p.table_bytes + p.range_bytes;
+    const size_t smem = 1024 + static_cast<size_t>(halves + 2 * scored_slots(head_dim, halves)) * SA_T * head_dim * 2 + p.table_bytes + p.range_bytes;
     int mode = p.slopes != nullptr || p.distance_bias != nullptr ? SA_ANY : p.softcap > 0.f ? SA_CAP : SA_PLAIN;
     if (p.documents != nullptr) mode = (mode == SA_PLAIN ? SA_PLAIN : SA_ANY) | SA_DOCS;
     const bool bf16 = dtype == STOF_DTYPE_BF16;

@@ -13,7 +13,6 @@
 // A tile is classified per warp (32 rows): nothing to mask, or masked by 128 bits a row.
 // What a call does not use is not in its kernel's loop (MODE): the loop a warp spends its time in has to fit the instruction caches.
 #pragma once
-#include <type_traits>
 
 #include "cache_common.cuh"
 #include "stof_host.h"
@@ -22,7 +21,7 @@
 namespace stof {
 
 constexpr int SA_T = 128;                    // rows of a half, keys of a tile
-constexpr int SA_PAD = 256;                  // the distance table in shared memory goes on for so long on both sides: a tile that meets the table needs no clamp
+constexpr int SA_PAD = 160;                  // the distance table in shared memory goes on for so long on both sides: a tile that meets the table needs no clamp
 constexpr float SA_RESCALE = 8.0f;           // log2 units by which a row's maximum may outgrow the reference of its P (P <= 2^8)
 constexpr float SA_LOG2E = 1.4426950408889634f;
 enum { SA_PLAIN = 0, SA_CAP = 1, SA_ANY = 2, SA_DOCS = 4 };   // what is done to scores: nothing, the cap alone, whatever the call asks for; and documents
@@ -169,11 +168,18 @@ static __device__ __forceinline__ void rescale_o(uint32_t t_o, float alpha) {
     tc_wait_st();
 }
 
-// Two halves: three warpgroups, the last one with two idle warps, so that registers can be moved from it to the softmax warps (setmaxnreg
-// is a whole warpgroup's): 384 x 168 at the launch, 256 x 224 + 128 x 56 afterwards, the same sum.
-constexpr int SA_REGS_SOFTMAX = 224, SA_REGS_OTHER = 56;
-static_assert(256 * SA_REGS_SOFTMAX + 128 * SA_REGS_OTHER <= 384 * 168, "more registers than the block was launched with would be waited for forever");
-constexpr int scored_threads(int halves) { return halves == 2 ? 384 : 192; }
+// Registers are moved to the softmax warps from the others (setmaxnreg, which is a whole warpgroup's: two of the others' four warps are
+// idle).  Two halves: 384 x 168 at the launch, 256 x R + 128 x r afterwards.  One half of D = 64, two blocks on an SM: 256 x 128, then
+// 128 x R + 128 x r.  One half of D = 128 has the SM to itself and 255 each.
+constexpr int SA_R2 = 224, SA_R1 = 208;      // (216 and 232, 200 and 216: up to 3 % slower)
+constexpr int scored_threads(int halves) { return halves == 2 ? 384 : 256; }
+constexpr int scored_per_sm(int dim, int halves) { return halves == 1 ? 2 : 1; }
+constexpr int scored_slots(int dim, int halves) { return dim == 128 && halves == 1 ? 1 : 2; }
+constexpr bool scored_moves(int dim, int halves) { return halves == 2 || scored_per_sm(dim, halves) == 2; }
+constexpr int scored_regs_softmax(int halves) { return halves == 2 ? SA_R2 : SA_R1; }
+constexpr int scored_regs_other(int halves) { return halves == 2 ? (384 * 168 - 256 * SA_R2) / 128 : (256 * 128 - 128 * SA_R1) / 128; }
+static_assert(256 * SA_R2 + 128 * scored_regs_other(2) <= 384 * 168 && 128 * SA_R1 + 128 * scored_regs_other(1) <= 256 * 128 && SA_R1 % 8 == 0 && SA_R2 % 8 == 0 &&
+                  scored_regs_other(1) % 8 == 0 && scored_regs_other(2) % 8 == 0, "more registers than the block was launched with would be waited for forever");
 
 // What a stretch of rows sees: tiles [lo, hi) and [0, prefix), where documents agree
 struct Reach {
@@ -181,7 +187,7 @@ struct Reach {
 };
 
 template <int D, int HALVES, bool BF16, int WHAT>
-__global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64 && (WHAT & SA_ANY) == 0 ? 2 : 1) scored_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(D, HALVES)) scored_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_o,
                                                                         const ScoredParams p) {
     constexpr int MODE = WHAT & 3;
@@ -189,14 +195,15 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
     constexpr int PANELS = D / 64;                           // 64-column panels of a tile, 128 rows of 128 swizzled bytes each
     constexpr int PANEL_BYTES = SA_T * 128, TILE_BYTES = PANELS * PANEL_BYTES;
     constexpr int W_LOAD = HALVES * 4, W_MMA = W_LOAD + 1;
-    constexpr bool OWN_P = HALVES * (SA_T + SA_T / 2 + D) <= 512;
+    constexpr bool OWN_P = scored_per_sm(D, HALVES) * HALVES * (SA_T + SA_T / 2 + D) <= 512;
+    constexpr unsigned SLOTS = scored_slots(D, HALVES);     // of K, and of V
     constexpr int COL_O = HALVES * SA_T, COL_P = OWN_P ? COL_O + HALVES * D : 0, P_STEP = OWN_P ? SA_T / 2 : SA_T;
     constexpr int TMEM_COLS = (OWN_P ? COL_P + HALVES * SA_T / 2 : COL_O + HALVES * D) > 256 ? 512 : 256;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     unsigned char* q_smem = smem;
     unsigned char* ring = q_smem + HALVES * TILE_BYTES;
-    float* table = reinterpret_cast<float*>(ring + 4 * TILE_BYTES);      // (two slots of K, two of V)
+    float* table = reinterpret_cast<float*>(ring + 2 * SLOTS * TILE_BYTES);
     int2* range = reinterpret_cast<int2*>(reinterpret_cast<unsigned char*>(table) + p.table_bytes);
     __shared__ __align__(8) uint64_t bars[SB_COUNT];
     __shared__ uint32_t tmem_slot;
@@ -284,12 +291,12 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
     };
     // the n-th tile goes into slot n % 2 of its side, K a tile ahead of V
     auto load = [&](int kind, int t, unsigned n) {
-        const int s = static_cast<int>(n & 1);
+        const int s = static_cast<int>(n % SLOTS);
         uint64_t *full = &bars[(kind == 0 ? SB_K_FULL : SB_V_FULL) + s], *empty = &bars[(kind == 0 ? SB_K_EMPTY : SB_V_EMPTY) + s];
-        wait_inline(smem_u32(empty), ((n >> 1) & 1) ^ 1, wctx, (kind == 0 ? SB_K_EMPTY : SB_V_EMPTY) + s);
+        wait_inline(smem_u32(empty), ((n / SLOTS) & 1) ^ 1, wctx, (kind == 0 ? SB_K_EMPTY : SB_V_EMPTY) + s);
         mbar_arrive_expect_tx(full, TILE_BYTES);
         for (int c = 0; c < PANELS; ++c)
-            load_tile(ring + (2 * kind + s) * TILE_BYTES + c * PANEL_BYTES, kind == 0 ? &map_k : &map_v, full, c * 64, t * SA_T, kv, b, p.slot_s[1 + kind],
+            load_tile(ring + (SLOTS * kind + s) * TILE_BYTES + c * PANEL_BYTES, kind == 0 ? &map_k : &map_v, full, c * 64, t * SA_T, kv, b, p.slot_s[1 + kind],
                       p.slot_h[1 + kind]);
     };
     // Q, and the first K where the rules alone say which that is, are on their way while the rest is set up
@@ -347,7 +354,7 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
     const int fix_tile = k_end < p.k_len && k_end % SA_T != 0 ? k_end / SA_T : -1;
 
     if (warp < HALVES * 4) {
-        if constexpr (HALVES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SA_REGS_SOFTMAX));
+        if constexpr (scored_moves(D, HALVES)) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(scored_regs_softmax(HALVES)));
         if (*abort_flag == 0) {
             // ---------------------------------------------------------------- softmax: one row a thread
             const int h = HALVES == 2 ? warp >> 2 : 0, tid = threadIdx.x & 127;
@@ -535,7 +542,10 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
                     }
                     if constexpr (OWN_P) {
                         // the products that read the P before this one have to be through: they are where O is complete
-                        if (part == 0 && done > 0) wait_inline(smem_u32(&bars[SB_O + h]), static_cast<uint32_t>((done - 1) & 1), wctx, SB_O + h);
+                        if (part == 0 && done > 0) {
+                            wait_inline(smem_u32(&bars[SB_O + h]), static_cast<uint32_t>((done - 1) & 1), wctx, SB_O + h);
+                            tc_fence_after();
+                        }
                     }
                     tmem_st32(t_p + 32 * part, s[part]);
                     tc_wait_st();
@@ -589,7 +599,7 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
             }
         }
     } else {
-        if constexpr (HALVES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SA_REGS_OTHER));
+        if constexpr (scored_moves(D, HALVES)) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(scored_regs_other(HALVES)));
         if (*abort_flag == 0 && warp == W_LOAD) {
             // ---------------------------------------------------------------- TMA producer
             int fix_slot = -1;
@@ -599,11 +609,13 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
                 if (DOCS && t < t_end) load(0, t, 0);
                 for (unsigned n = 0; t < t_end; ++n) {
                     const int tn = next(t + 1);
+                    // (the one slot of K is free later than the one of V)
+                    if (SLOTS == 1) load(1, t, n);
                     if (tn < t_end) load(0, tn, n + 1);
-                    load(1, t, n);
+                    if (SLOTS > 1) load(1, t, n);
                     if (t == fix_tile) {
-                        fix_slot = static_cast<int>(n & 1);
-                        fix_phase = (n >> 1) & 1;
+                        fix_slot = static_cast<int>(n % SLOTS);
+                        fix_phase = (n / SLOTS) & 1;
                     }
                     t = tn;
                 }
@@ -615,7 +627,7 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
                 for (int i = (k_end % SA_T) * 8 + lane; i < SA_T * 8; i += 32)
 #pragma unroll
                     for (int c = 0; c < PANELS; ++c)
-                        *reinterpret_cast<uint4*>(ring + (2 + fix_slot) * TILE_BYTES + c * PANEL_BYTES + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        *reinterpret_cast<uint4*>(ring + (SLOTS + fix_slot) * TILE_BYTES + c * PANEL_BYTES + i * 16) = make_uint4(0u, 0u, 0u, 0u);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars[SB_FIX]);
@@ -627,7 +639,7 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
                 constexpr uint32_t idesc_qk = make_idesc_f16(SA_T, SA_T, false) | type, idesc_pv = make_idesc_f16(SA_T, D, true) | type;
                 const uint64_t q_desc = make_smem_desc_sw128(smem_u32(q_smem), 16, 1024);
                 const uint64_t k_desc = make_smem_desc_sw128(smem_u32(ring), 16, 1024);
-                const uint64_t v_desc = make_smem_desc_sw128(smem_u32(ring + 2 * TILE_BYTES), PANEL_BYTES, 1024);
+                const uint64_t v_desc = make_smem_desc_sw128(smem_u32(ring + SLOTS * TILE_BYTES), PANEL_BYTES, 1024);
                 const uint32_t bar0 = smem_u32(bars);
                 auto wait = [&](int bar, uint32_t parity) { wait_inline(bar0 + 8 * bar, parity, wctx, bar); };
                 int done[HALVES];                            // tiles whose PV has been issued
@@ -636,11 +648,11 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
                 auto qk = [&](int h, unsigned n) {           // S = Q K^T of the n-th tile
                     if (done[h] == 0) wait(SB_Q + h, 0);
                     tc_fence_after();
-                    mma_chain_ss<D / 16>(tmem + h * SA_T, q_desc + static_cast<uint64_t>(h * (TILE_BYTES >> 4)), k_desc + static_cast<uint64_t>((n & 1) * (TILE_BYTES >> 4)), idesc_qk);
+                    mma_chain_ss<D / 16>(tmem + h * SA_T, q_desc + static_cast<uint64_t>(h * (TILE_BYTES >> 4)), k_desc + static_cast<uint64_t>((n % SLOTS) * (TILE_BYTES >> 4)), idesc_qk);
                     tc_commit_addr(bar0 + 8 * (SB_S + h));
                 };
                 auto pv = [&](int h, unsigned n) {           // O (+)= P V
-                    const uint64_t v = v_desc + static_cast<uint64_t>((n & 1) * (TILE_BYTES >> 4));
+                    const uint64_t v = v_desc + static_cast<uint64_t>((n % SLOTS) * (TILE_BYTES >> 4));
                     const uint32_t parity = static_cast<uint32_t>(done[h] & 1), o = tmem + COL_O + h * D, q = tmem + COL_P + h * P_STEP;
                     wait(SB_P0 + h, parity);
                     tc_fence_after();
@@ -666,9 +678,10 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
                 }
                 for (unsigned n = 0; t < t_end; ++n) {
                     const int tn = next(t + 1);
-                    const int ks = static_cast<int>((n + 1) & 1), vs = static_cast<int>(n & 1);
-                    if (tn < t_end) wait(SB_K_FULL + ks, ((n + 1) >> 1) & 1);
+                    const int ks = static_cast<int>((n + 1) % SLOTS), vs = static_cast<int>(n % SLOTS);
+                    auto k_there = [&] { wait(SB_K_FULL + ks, ((n + 1) / SLOTS) & 1); };
                     if constexpr (OWN_P) {
+                        if (tn < t_end) k_there();
 #pragma unroll
                         for (int h = 0; h < HALVES; ++h) {
                             if (tn < t_end && wanted(h, tn)) {
@@ -678,13 +691,16 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
                         }
                         if (tn < t_end) tc_commit_addr(bar0 + 8 * (SB_K_EMPTY + ks));
                     }
-                    wait(SB_V_FULL + vs, (n >> 1) & 1);
+                    wait(SB_V_FULL + vs, (n / SLOTS) & 1);
                     if (t == fix_tile) wait(SB_FIX, 0);
 #pragma unroll
                     for (int h = 0; h < HALVES; ++h) {
                         if (wanted(h, t)) pv(h, n);
                         if constexpr (!OWN_P)
-                            if (tn < t_end && wanted(h, tn)) qk(h, n + 1);
+                            if (tn < t_end && wanted(h, tn)) {
+                                k_there();
+                                qk(h, n + 1);
+                            }
                     }
                     tc_commit_addr(bar0 + 8 * (SB_V_EMPTY + vs));
                     if constexpr (!OWN_P)
@@ -706,30 +722,30 @@ __global__ void __launch_bounds__(scored_threads(HALVES), HALVES == 1 && D == 64
 using ScoredMaps = CUtensorMap[4];             // q, k, v, out
 // Launches the kernel for one head size (scored_attn_64.cu, scored_attn_128.cu: a translation unit each, they take long to compile)
 template <int D>
-int launch_scored(const ScoredMaps& maps, const ScoredParams& p, int halves, bool bf16, int mode, long long blocks, size_t smem, cudaStream_t stream);
+int launch_scored(const ScoredMaps& maps, const ScoredParams& p, int halves, bool bf16, int what, long long blocks, size_t smem, cudaStream_t stream);
 
+template <int D, int HALVES, bool BF16, int WHAT>
+int launch_one(const ScoredMaps& maps, const ScoredParams& p, long long blocks, size_t smem, cudaStream_t stream) {
+    if (int rc = allow_shared_memory<scored_attn_kernel<D, HALVES, BF16, WHAT>>()) return rc;
+    LaunchConfig lc(dim3(static_cast<unsigned>(blocks)), static_cast<unsigned>(scored_threads(HALVES)), smem, stream);
+    STOF_CUDA(cudaLaunchKernelEx(&lc.cfg, scored_attn_kernel<D, HALVES, BF16, WHAT>, maps[0], maps[1], maps[2], maps[3], p));
+    return STOF_OK;
+}
+template <int D, int HALVES, bool BF16>
+int launch_what(const ScoredMaps& maps, const ScoredParams& p, int what, long long blocks, size_t smem, cudaStream_t stream) {
+    switch (what) {
+        case SA_PLAIN: return launch_one<D, HALVES, BF16, SA_PLAIN>(maps, p, blocks, smem, stream);
+        case SA_CAP: return launch_one<D, HALVES, BF16, SA_CAP>(maps, p, blocks, smem, stream);
+        case SA_ANY: return launch_one<D, HALVES, BF16, SA_ANY>(maps, p, blocks, smem, stream);
+        case SA_PLAIN | SA_DOCS: return launch_one<D, HALVES, BF16, SA_PLAIN | SA_DOCS>(maps, p, blocks, smem, stream);
+        default: return launch_one<D, HALVES, BF16, SA_ANY | SA_DOCS>(maps, p, blocks, smem, stream);
+    }
+}
 template <int D>
-int launch_scored_impl(const ScoredMaps& maps, const ScoredParams& p, int halves, bool bf16, int mode, long long blocks, size_t smem, cudaStream_t stream) {
-    auto launch = [&](auto kernel) -> int {
-        STOF_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-        LaunchConfig lc(dim3(static_cast<unsigned>(blocks)), static_cast<unsigned>(scored_threads(halves)), smem, stream);
-        STOF_CUDA(cudaLaunchKernelEx(&lc.cfg, kernel, maps[0], maps[1], maps[2], maps[3], p));
-        return STOF_OK;
-    };
-    auto by_mode = [&](auto h, auto b) -> int {
-        constexpr int H = decltype(h)::value;
-        constexpr bool B = decltype(b)::value;
-        switch (mode) {
-            case SA_PLAIN: return launch(scored_attn_kernel<D, H, B, SA_PLAIN>);
-            case SA_CAP: return launch(scored_attn_kernel<D, H, B, SA_CAP>);
-            case SA_ANY: return launch(scored_attn_kernel<D, H, B, SA_ANY>);
-            case SA_PLAIN | SA_DOCS: return launch(scored_attn_kernel<D, H, B, SA_PLAIN | SA_DOCS>);
-            default: return launch(scored_attn_kernel<D, H, B, SA_ANY | SA_DOCS>);
-        }
-    };
-    using std::integral_constant;
-    if (halves == 2) return bf16 ? by_mode(integral_constant<int, 2>{}, std::true_type{}) : by_mode(integral_constant<int, 2>{}, std::false_type{});
-    return bf16 ? by_mode(integral_constant<int, 1>{}, std::true_type{}) : by_mode(integral_constant<int, 1>{}, std::false_type{});
+int launch_scored_impl(const ScoredMaps& maps, const ScoredParams& p, int halves, bool bf16, int what, long long blocks, size_t smem, cudaStream_t stream) {
+    if constexpr (D == 128)                                  // (heads of 64: one half, see the caller)
+        if (halves == 2) return bf16 ? launch_what<D, 2, true>(maps, p, what, blocks, smem, stream) : launch_what<D, 2, false>(maps, p, what, blocks, smem, stream);
+    return bf16 ? launch_what<D, 1, true>(maps, p, what, blocks, smem, stream) : launch_what<D, 1, false>(maps, p, what, blocks, smem, stream);
 }
 
 }  // namespace stof

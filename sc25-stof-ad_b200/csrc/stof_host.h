@@ -8,6 +8,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <atomic>
+
 #include "../../include/stof_b200.h"
 
 namespace stof {
@@ -58,6 +60,21 @@ struct LaunchConfig {
         cfg.numAttrs = cluster > 1 ? 2 : 1;
     }
 };
+
+// Lets a kernel use as much dynamic shared memory as a block may have, once per device and kernel (KERNEL names the kernel: one flag array
+// each; host threads that race here store the same)
+template <auto KERNEL>
+int allow_shared_memory() {
+    static std::atomic<bool> allowed[64];
+    int dev = 0;
+    STOF_CUDA(cudaGetDevice(&dev));
+    if (dev >= 0 && dev < 64 && allowed[dev]) return STOF_OK;
+    cudaFuncAttributes a;
+    STOF_CUDA(cudaFuncGetAttributes(&a, KERNEL));
+    STOF_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - static_cast<int>(a.sharedSizeBytes)));
+    if (dev >= 0 && dev < 64) allowed[dev] = true;
+    return STOF_OK;
+}
 
 int sm_count();   // multiprocessors of the current device (cached per device)
 
