@@ -24,8 +24,8 @@ namespace {
 constexpr int CT_WARPS = 4, CT_THREADS = CT_WARPS * 32;
 constexpr int CT_TILES = 2;                  // tiles of 16 keys that a warp takes at a time: independent chains of products, and half the work around them
 constexpr int CT_STEP = 16 * CT_TILES, CT_UNIT = CT_STEP * CT_WARPS;     // keys of a warp's step, of a block's: the unit
-#ifndef CT_STAGES
-#define CT_STAGES 2
+#ifndef CT_STAGES64
+#define CT_STAGES64 3
 #endif
 #ifndef CT_LONG
 #define CT_LONG 16
@@ -33,9 +33,10 @@ constexpr int CT_STEP = 16 * CT_TILES, CT_UNIT = CT_STEP * CT_WARPS;     // keys
 #ifndef CT_WAVES
 #define CT_WAVES 4
 #endif
-#ifndef CT_BLOCKS
-#define CT_BLOCKS 3
+#ifndef CT_BLOCKS64
+#define CT_BLOCKS64 4
 #endif
+constexpr int ct_blocks(int nt, int dim) { return nt == 2 ? 2 : dim == 64 ? CT_BLOCKS64 : 3; }   // on an SM
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct CacheAttnParams {
@@ -63,8 +64,7 @@ struct CacheAttnParams {
 // keys [first, first + 128 * units) cover what the request's tokens see
 struct Span { int length, first, units; };
 __device__ __forceinline__ Span span_of(const CacheAttnParams& p, int b) {
-    const long long most = static_cast<long long>(p.table_width) << p.page_shift;
-    const int length = static_cast<int>(min(static_cast<long long>(max(p.lengths[b], 0)), most));
+    const int length = min(max(p.lengths[b], 0), p.table_width << p.page_shift);     // (at most 2^30)
     int first = 0;
     if (p.window > 0) first = max(length - p.tokens - p.window + 1, 0) & ~(CT_UNIT - 1);
     return {length, first, (length - first + CT_UNIT - 1) / CT_UNIT};
@@ -95,7 +95,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 // once meet all banks.
 template <int D>
 struct Ring {
-    static constexpr int STAGES = CT_STAGES;
+    static constexpr int STAGES = D == 64 ? CT_STAGES64 : 2;
     static constexpr int SIDE = 16 * D, TILE = 2 * SIDE + 16, STAGE = CT_TILES * TILE;       // of a tile: K, V, {k scale, v scale, valid, -}
     static constexpr int BYTES = STAGES * STAGE;
     static constexpr int CHUNKS = D / 16, LOADS = CHUNKS / 2;                // of a row; copies of a lane per side
@@ -116,7 +116,7 @@ __device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
 }
 
 template <int NT, int D, bool E4M3>
-__global__ void __launch_bounds__(CT_THREADS, NT == 1 ? CT_BLOCKS : 2) cache_attn_kernel(const CacheAttnParams p) {
+__global__ void __launch_bounds__(CT_THREADS, ct_blocks(NT, D)) cache_attn_kernel(const CacheAttnParams p) {
     constexpr int CH = D / 64, KS = D / 16, MT = D / 16, ROWS = NT * 8;
     constexpr int V_BYTES = D / 8;           // of a row, per lane
     using R = Ring<D>;
@@ -129,14 +129,15 @@ __global__ void __launch_bounds__(CT_THREADS, NT == 1 ? CT_BLOCKS : 2) cache_att
     const uint32_t ring_addr = smem_u32(ring);
     grid_dependency_wait();
     grid_launch_dependents();
-    if (__syncthreads_or(failure_reported(p.status))) return;
+    const bool muted = failure_reported(p.status);           // asked for now, looked at when there is something to write
     // which piece is this block's?  Every warp finds out for itself, a lane a request (no barrier, the lengths are in the cache)
     const unsigned pairs = static_cast<unsigned>(p.kv_heads * p.row_groups);     // of a request
+    Span span = {0, 0, 0};                                   // of the lane's request: the first 32 stay in registers
     unsigned total = 0, some = 0;
-    for (int i = lane; i < p.requests; i += 32) {
-        const int units = span_of(p, i).units;
-        total += static_cast<unsigned>(units);
-        some += units > 0 ? 1u : 0u;
+    for (int i = p.requests - 1 - (p.requests - 1 - lane & 31); i >= 0; i -= 32) {       // the last of lane, lane + 32, .. to the first
+        span = span_of(p, i);
+        total += static_cast<unsigned>(span.units);
+        some += span.units > 0 ? 1u : 0u;
     }
     total = __reduce_add_sync(0xffffffffu, total) * pairs;
     some = __reduce_add_sync(0xffffffffu, some) * pairs;
@@ -144,8 +145,8 @@ __global__ void __launch_bounds__(CT_THREADS, NT == 1 ? CT_BLOCKS : 2) cache_att
     int b = -1;
     unsigned base = 0;
     for (int b0 = 0; b0 < p.requests; b0 += 32) {
-        const unsigned units = b0 + lane < p.requests ? static_cast<unsigned>(span_of(p, b0 + lane).units) : 0u;
-        const unsigned mine = (units + length_each - 1) / length_each * pairs;
+        if (b0 > 0) span = b0 + lane < p.requests ? span_of(p, b0 + lane) : Span{0, 0, 0};
+        const unsigned mine = (static_cast<unsigned>(span.units) + length_each - 1) / length_each * pairs;
         unsigned upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -157,12 +158,12 @@ __global__ void __launch_bounds__(CT_THREADS, NT == 1 ? CT_BLOCKS : 2) cache_att
             const int at = __ffs(here) - 1;
             b = b0 + at;
             base += __shfl_sync(0xffffffffu, upto - mine, at);
+            span = {__shfl_sync(0xffffffffu, span.length, at), __shfl_sync(0xffffffffu, span.first, at), __shfl_sync(0xffffffffu, span.units, at)};
             break;
         }
         base += __shfl_sync(0xffffffffu, upto, 31);
     }
     if (b < 0) return;
-    const Span span = span_of(p, b);
     const unsigned pieces = (static_cast<unsigned>(span.units) + length_each - 1) / length_each;
     const unsigned pair = (blockIdx.x - base) / pieces, piece = (blockIdx.x - base) - pair * pieces;
     const unsigned each = static_cast<unsigned>(span.units) / pieces, extra = static_cast<unsigned>(span.units) - each * pieces;
@@ -484,7 +485,7 @@ __global__ void __launch_bounds__(CT_THREADS, NT == 1 ? CT_BLOCKS : 2) cache_att
             stage = stage + 1 == R::STAGES ? 0 : stage + 1;
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
-        __syncthreads();                                     // merge_o lies over the rings
+        if (__syncthreads_or(muted)) return;                 // merge_o lies over the rings
 
         // ---- the four warps' results are added in smem, in their order
 #pragma unroll
@@ -588,29 +589,24 @@ __global__ void __launch_bounds__(CT_THREADS) cache_attn_join_kernel(const Cache
     for (int i0 = warp; i0 < count; i0 += CT_WARPS * AHEAD) {
         float m[AHEAD], l[AHEAD], x[AHEAD][EACH];
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-            const int i = i0 + j * CT_WARPS;
-            m[j] = -INFINITY;
-            l[j] = 0.f;
-#pragma unroll
-            for (int e = 0; e < EACH; ++e) x[j][e] = 0.f;
-            if (i < count) {
-                const float* at = part(i);
-                m[j] = __ldca(at + r);
-                l[j] = __ldca(at + ROWS + r);
-                at += 2 * ROWS + r * D + lane * EACH;
-                if constexpr (EACH == 4) {
-                    const float4 v = __ldca(reinterpret_cast<const float4*>(at));
-                    x[j][0] = v.x; x[j][1] = v.y; x[j][2] = v.z; x[j][3] = v.w;
-                } else {
-                    const float2 v = __ldca(reinterpret_cast<const float2*>(at));
-                    x[j][0] = v.x; x[j][1] = v.y;
-                }
+        for (int j = 0; j < AHEAD; ++j) {                    // no branches: all loads are on their way together
+            const float* at = part(min(i0 + j * CT_WARPS, count - 1));
+            m[j] = __ldca(at + r);
+            l[j] = __ldca(at + ROWS + r);
+            at += 2 * ROWS + r * D + lane * EACH;
+            if constexpr (EACH == 4) {
+                const float4 v = __ldca(reinterpret_cast<const float4*>(at));
+                x[j][0] = v.x; x[j][1] = v.y; x[j][2] = v.z; x[j][3] = v.w;
+            } else {
+                const float2 v = __ldca(reinterpret_cast<const float2*>(at));
+                x[j][0] = v.x; x[j][1] = v.y;
             }
         }
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
-            const float f = m[j] > -INFINITY ? fast_exp2(m[j] - top) : 1.f;  // (a part that saw nothing is 0, or NaN)
+            // (a part that saw nothing is 0, or NaN)
+            const float f = i0 + j * CT_WARPS >= count ? 0.f : m[j] > -INFINITY ? fast_exp2(m[j] - top) : 1.f;
+            if (f == 0.f) continue;                          // (nothing of a part that is there twice, nor zero times an infinity)
             sum += l[j] * f;
 #pragma unroll
             for (int e = 0; e < EACH; ++e) o[e] += x[j][e] * f;
@@ -641,14 +637,14 @@ struct Shape {
     long long blocks, joins, units;          // joins: (request, K/V head, row group)s; units: at most
 };
 // row tiles of 8: one up to 8 rows, else two at a time; blocks: as many as there may be pieces (piece_units)
-Shape shape_of(int requests, int tokens, int heads, int kv_heads, int page_size, int table_width) {
+Shape shape_of(int requests, int tokens, int heads, int kv_heads, int head_dim, int page_size, int table_width) {
     Shape s;
     s.rows = tokens * (heads / kv_heads);
     s.nt = s.rows <= 8 ? 1 : 2;
     s.row_groups = (s.rows + 8 * s.nt - 1) / (8 * s.nt);
     s.joins = static_cast<long long>(requests) * kv_heads * s.row_groups;
     s.units = s.joins * ((static_cast<long long>(table_width) * page_size + CT_UNIT - 1) / CT_UNIT);
-    s.resident = sm_count() * (s.nt == 1 ? CT_BLOCKS : 2);
+    s.resident = sm_count() * ct_blocks(s.nt, head_dim);
     long long pieces = s.units / CT_LONG;
     if (pieces > static_cast<long long>(s.resident) * CT_WAVES) pieces = static_cast<long long>(s.resident) * CT_WAVES;
     if (pieces < s.resident) pieces = s.resident;
@@ -674,7 +670,7 @@ using namespace stof;
 
 extern "C" size_t stof_cache_attn_workspace_bytes(int requests, int tokens, int heads, int kv_heads, int head_dim, int page_size, int table_width) {
     if (requests <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || page_size <= 0 || table_width < 0) return 0;
-    const Shape s = shape_of(requests, tokens, heads, kv_heads, page_size, table_width);
+    const Shape s = shape_of(requests, tokens, heads, kv_heads, head_dim, page_size, table_width);
     return (static_cast<size_t>(s.joins) * sizeof(int2) + 15) / 16 * 16 + static_cast<size_t>(s.blocks) * (8 * s.nt) * (static_cast<size_t>(head_dim) + 2) * sizeof(float);
 }
 
@@ -703,7 +699,7 @@ extern "C" int stof_cache_attn(const void* q, void* out, int dtype, const long l
     STOF_REQUIRE(aligned16(q) && aligned16(out) && aligned16(k_pages) && aligned16(v_pages) && aligned16(workspace), "cache_attn: pointers must be 16-byte aligned");
     for (int i = 0; i < 3; ++i)
         STOF_REQUIRE(q_strides[i] % 8 == 0 && out_strides[i] % 8 == 0, "cache_attn: strides must be multiples of 8 elements");
-    const Shape s = shape_of(requests, tokens, heads, kv_heads, page_size, table_width);
+    const Shape s = shape_of(requests, tokens, heads, kv_heads, head_dim, page_size, table_width);
     const size_t need = stof_cache_attn_workspace_bytes(requests, tokens, heads, kv_heads, head_dim, page_size, table_width);
     if (workspace == nullptr || workspace_bytes < need) {
         set_error("cache_attn: workspace of %zu bytes, need %zu", workspace == nullptr ? static_cast<size_t>(0) : workspace_bytes, need);
