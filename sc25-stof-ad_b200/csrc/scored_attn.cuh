@@ -63,17 +63,36 @@ static __device__ __forceinline__ float max3f(float a, float b, float c) {
     return d;
 }
 
-// tanh of a pair, |u| <= 1: odd polynomial, relative error below 7e-6 (a weighted least-squares fit moved towards the minimax one).
-// A score of 40 is then off by 3e-4, less than P's rounding to fp16 makes of it.
-static __device__ __forceinline__ float2 tanh_near(float2 u) {
-    const float2 w = mul2(u, u);
-    float2 p = fma2(w, pk2(0.009036419913172722f, 0.009036419913172722f), pk2(-0.044817544519901276f, -0.044817544519901276f));
-    p = fma2(p, w, pk2(0.13036811351776123f, 0.13036811351776123f));
-    p = fma2(p, w, pk2(-0.3329806625843048f, -0.3329806625843048f));
-    p = fma2(p, w, pk2(0.999993085861206f, 0.999993085861206f));
-    return mul2(p, u);
+// from_u * tanh(s * to_u) near zero: an odd polynomial of s, the factors in its coefficients.  Relative errors of the fits (weighted least
+// squares moved towards the minimax one): 2.9e-6 of three terms up to |u| = 0.35, 7e-6 of five up to 1; a score of 40 is then off by
+// 3e-4 at most, less than P's rounding to fp16 makes of it.
+struct NearTanh {
+    float near[3], far[5];                   // of s, s^3, s^5, ..
+    float near_end, far_end;                 // up to which |s| they are used: 0 where powers of to_u leave fp32's range
+    __device__ __forceinline__ NearTanh() : near{}, far{}, near_end(0.f), far_end(0.f) {}
+    __device__ __forceinline__ NearTanh(float to_u, float from_u) {
+        const float w = to_u * to_u, a = to_u * from_u;
+        near_end = to_u < 1e8f ? 0.35f / to_u : 0.f;         // (below 1e-10 the higher terms vanish, and so do they in the sum)
+        far_end = to_u > 2e-4f && to_u < 5e3f ? 1.f / to_u : 0.f;
+        near[0] = a * 0.9999971389770508f;
+        near[1] = a * w * -0.33290955424308777f;
+        near[2] = a * w * w * 0.1239503026008606f;
+        far[0] = a * 0.999993085861206f;
+        far[1] = a * w * -0.3329806625843048f;
+        far[2] = a * w * w * 0.13036811351776123f;
+        far[3] = a * w * w * w * -0.044817544519901276f;
+        far[4] = a * w * w * w * w * 0.009036419913172722f;
+    }
+};
+template <int N>
+static __device__ __forceinline__ float2 odd_polynomial(float2 s, const float (&c)[N]) {
+    const float2 w = mul2(s, s);
+    float2 q = pk2(c[N - 1], c[N - 1]);
+#pragma unroll
+    for (int i = N - 2; i >= 0; --i) q = fma2(q, w, pk2(c[i], c[i]));
+    return mul2(q, s);
 }
-// tanh(u) = 1 - 2 / (1 + e^(2u)) for any u
+// tanh(u) = 1 - 2 / (1 + e^(2u)): off by 1e-7, where it is not near zero
 static __device__ __forceinline__ float tanh_any(float u) { return 1.f - 2.f * fast_reciprocal(1.f + fast_exp2(u * (2.f * SA_LOG2E))); }
 
 // The bounded wait without a call of a function (which does not go with moved registers)
@@ -91,7 +110,7 @@ static __device__ __forceinline__ void wait_inline(uint32_t bar, uint32_t parity
     }
 }
 
-// tanh of a whole row's scores in tensor memory that are not near enough for tanh_near: s = from_u * tanh(s * to_u), in place
+// tanh of a whole row's scores in tensor memory that are not near enough to zero for a polynomial: s = from_u * tanh(s * to_u), in place
 static __device__ __forceinline__ void cap_in_tmem(uint32_t t_s, float to_u, float from_u) {
 #pragma unroll 1
     for (int c = 0; c < SA_T; c += 16) {
@@ -375,6 +394,8 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(D, HALVE
             const bool capped = MODE == SA_CAP || (MODE == SA_ANY && p.softcap > 0.f);
             const float to_u = capped ? p.scale / p.softcap : 0.f, from_u = p.softcap * SA_LOG2E;
             const uint32_t s_bar = smem_u32(&bars[SB_S + h]);
+            NearTanh tanh_near;
+            if (capped) tanh_near = NearTanh(to_u, from_u);
             const float raw_scale = p.scale * SA_LOG2E;      // of a score that nothing changes, to log2 units
             const float sc = changed ? 1.f : raw_scale;      // what is left to multiply by when the exponential is taken
             const float slope = p.slopes != nullptr ? __ldca(p.slopes + head) * SA_LOG2E : 0.f;
@@ -423,11 +444,17 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(D, HALVE
                         float top = 0.f;
 #pragma unroll
                         for (int c = 0; c < SA_T; c += 2) top = max3f(top, fabsf(__uint_as_float(S_AT(c))), fabsf(__uint_as_float(S_AT(c + 1))));
-                        if (__builtin_expect(__all_sync(0xffffffffu, top * to_u <= 1.f), 1)) {
-                            const float2 to2 = pk2(to_u, to_u), from2 = pk2(from_u, from_u);
+                        if (__builtin_expect(__all_sync(0xffffffffu, top <= tanh_near.near_end), 1)) {
 #pragma unroll
                             for (int c = 0; c < SA_T; c += 2) {
-                                const float2 y = mul2(tanh_near(mul2(pk2(__uint_as_float(S_AT(c)), __uint_as_float(S_AT(c + 1))), to2)), from2);
+                                const float2 y = odd_polynomial(pk2(__uint_as_float(S_AT(c)), __uint_as_float(S_AT(c + 1))), tanh_near.near);
+                                S_AT(c) = __float_as_uint(y.x);
+                                S_AT(c + 1) = __float_as_uint(y.y);
+                            }
+                        } else if (__all_sync(0xffffffffu, top <= tanh_near.far_end)) {
+#pragma unroll
+                            for (int c = 0; c < SA_T; c += 2) {
+                                const float2 y = odd_polynomial(pk2(__uint_as_float(S_AT(c)), __uint_as_float(S_AT(c + 1))), tanh_near.far);
                                 S_AT(c) = __float_as_uint(y.x);
                                 S_AT(c + 1) = __float_as_uint(y.y);
                             }

@@ -74,7 +74,7 @@ def _rules(name, B, H, Sk):
     g = torch.Generator().manual_seed(7)
     docs = torch.randint(1, 90, (B, Sk), generator=g).cumsum(1) // 1500
     return {
-        "cap": dict(softcap=30.0), "cap far": dict(softcap=1.5), "slopes": dict(slopes=torch.rand(H, generator=g)),
+        "cap": dict(softcap=30.0), "cap far": dict(softcap=1.5), "cap middle": dict(softcap=14.0), "cap tiny": dict(softcap=1e-3), "cap huge": dict(softcap=1e6), "slopes": dict(slopes=torch.rand(H, generator=g)),
         "slopes causal": dict(slopes=torch.rand(H, generator=g), causal=True), "table": dict(distance_bias=_table(H, 20, 5)),
         "table 0": dict(distance_bias=_table(H, 0, 5)), "table wide causal": dict(distance_bias=_table(H, 2048, 6), causal=True),
         "everything": dict(softcap=20.0, slopes=torch.rand(H, generator=g), distance_bias=_table(H, 33, 8), causal=True, window=150,
@@ -91,7 +91,7 @@ def _rules(name, B, H, Sk):
     }[name]
 
 
-ALL_RULES = ["cap", "cap far", "slopes", "slopes causal", "table", "table 0", "table wide causal", "everything", "window", "window causal", "window 1", "window wide",
+ALL_RULES = ["cap", "cap far", "cap middle", "cap tiny", "cap huge", "slopes", "slopes causal", "table", "table 0", "table wide causal", "everything", "window", "window causal", "window 1", "window wide",
              "prefix", "prefix past the keys", "window prefix", "documents", "documents causal", "documents shuffled", "one document", "padded",
              "padded to nothing", "padded beyond", "padded causal"]
 
@@ -252,7 +252,7 @@ def test_cache_attention(dim, entry, page, heads, kv_heads, tokens, dtype):
     _both_cache(_rand((len(lengths), tokens, heads, dim), 71, 2.0, TYPES[dtype]), _cache(lengths, kv_heads, page, dim, entry, 72))
 
 
-@pytest.mark.parametrize("rules", [dict(softcap=3.0), dict(softcap=50.0), dict(window=1), dict(window=70), dict(slopes=torch.tensor([0.5, 0.01, 0.2, 0.0])),
+@pytest.mark.parametrize("rules", [dict(softcap=3.0), dict(softcap=50.0), dict(softcap=1e6), dict(softcap=1e-3), dict(window=1), dict(window=70), dict(slopes=torch.tensor([0.5, 0.01, 0.2, 0.0])),
                                    dict(distance_bias=_table(4, 30, 5)), dict(distance_bias=_table(4, 0, 5)), dict(softmax_scale=0.3),
                                    dict(softcap=20.0, window=200, slopes=torch.tensor([0.5, 0.01, 0.2, 0.0]), distance_bias=_table(4, 128, 6))])
 @pytest.mark.parametrize("tokens", [1, 3])
