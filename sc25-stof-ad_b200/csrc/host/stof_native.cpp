@@ -1013,6 +1013,14 @@ PyObject* py_cache_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// `size` elements of a vector from `offset` on, without the dispatcher's round
+at::Tensor part_of(const at::Tensor& base, int64_t offset, int64_t size) {
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(base.storage()), base.key_set(), base.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(offset);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({size});
+    return t;
+}
+
 // page_tables(lengths, held, block_table, free_pages, free_count, page_size, new_tokens) -> (slots, starts, free_count, missing)
 PyObject* py_page_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
@@ -1033,8 +1041,10 @@ PyObject* py_page_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
         at::Tensor keep[2];
         const int* len = int_vector(&lengths, B, lengths, keep[0], op, "lengths");
         const int* held = int_vector(&tensor_needed(a[1], op), B, lengths, keep[1], op, "held");
-        const at::Tensor slots = make({fresh}, at::kInt, lengths), starts = make({B + 1}, at::kInt, lengths), left = make({1}, at::kInt, lengths),
-                         missing = make({1}, at::kInt, lengths);
+        // one allocation for the four of them (what the call costs is mostly this)
+        const int64_t room = (fresh + 3) / 4 * 4;
+        const at::Tensor all = make({room + B + 3}, at::kInt, lengths);
+        const at::Tensor slots = part_of(all, 0, fresh), starts = part_of(all, room, B + 1), left = part_of(all, room + B + 1, 1), missing = part_of(all, room + B + 2, 1);
         call("stof_page_tables", api.page_tables, len, held, as_int(B, "requests"), static_cast<int*>(table.data_ptr()),
              static_cast<long long>(B > 1 ? table.stride(0) : table.size(1)), as_int(table.size(1), "width of the block table"), static_cast<int*>(stack.data_ptr()),
              as_int(stack.size(0), "free pages"), static_cast<const int*>(count.data_ptr()), as_int(page, "page size"), static_cast<int*>(slots.data_ptr()),

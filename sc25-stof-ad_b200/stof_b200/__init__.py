@@ -16,4 +16,5 @@ from .rowwise import rowwise_attn_full, rowwise_attn_sliding, rowwise_attn_mask 
 from .fused import (gemm_bias, gemm_bias_gelu, gemm_bias_relu, gemm_bias_act, gemm_bias_residual, gemm_bias_residual_layernorm, gemm_bias_residual_then_layernorm, bias_residual_layernorm,  # noqa: F401
                     matmul_bias_layernorm, matmul_gelu_matmul, batched_bias_layernorm)
 from .scored import scored_attention, cache_attention, cache_append, page_tables  # noqa: F401
+from .generation import GenerationCache  # noqa: F401
 from .encoder import BertEncoder, EncoderWeights, T5Decoder, T5DecoderWeights, gpt2_stack, t5_encoder_stack  # noqa: F401

@@ -9,8 +9,9 @@ from typing import List
 import torch
 
 from . import _lib
-from .fused import EPILOGUES
+from .fused import EPILOGUES, gemm_bias, gemm_bias_act, gemm_bias_residual_layernorm
 from .masks import get_sparse_storage
+from .scored import scored_attention
 
 
 @dataclass
@@ -100,6 +101,63 @@ class BertEncoder:
         return self._run(hidden, False)
 
     __call__ = forward
+
+    # ---- generation: the same layers with a causal mask, over a cache (no mask or index is needed)
+    def _fits(self, hidden, cache, dims):
+        if hidden.dim() != dims or hidden.shape[-1] != cache.heads * cache.head_dim or cache.heads != self.head_num or cache.layers != len(self.layers):
+            raise _lib.StofError(f"generation: {dims} dimensions, the last of {cache.heads * cache.head_dim}, and a cache of {len(self.layers)} layers with "
+                                 f"{self.head_num} heads expected")
+
+    def _generate(self, x, cache, slots, attend):
+        """x (T, hidden) through all layers: new keys and values go to the cache, `attend(layer, q, k, v)` gives (T, hidden)."""
+        for i, w in enumerate(self.layers):
+            q, k, v = gemm_bias(x, w.Wqkv, w.bqkv).view(-1, 3, cache.heads, cache.head_dim).unbind(1)
+            cache.append(i, k, v, slots)
+            x = gemm_bias_residual_layernorm(attend(i, q, k, v), w.Wo, w.bo, x, w.g1, w.b1, self.eps)
+            inner = gemm_bias_act(x, w.W1, w.bi1, {"erf": "gelu_erf", "tanh": "gelu_tanh", "relu": "relu"}[self.gelu])
+            x = gemm_bias_residual_layernorm(inner, w.W2, w.bi2, x, w.g2, w.b2, self.eps)
+        return x
+
+    def prefill(self, hidden: torch.Tensor, cache, lengths: torch.Tensor, **rules) -> torch.Tensor:
+        """Prompts into a `GenerationCache`: hidden (T, hidden), the prompts of the requests that come in back to back in the order of the
+        requests; lengths (max_requests) int32: what every request holds afterwards (requests that are in the cache already keep
+        theirs, or are let go with 0; their tokens come by `step`, not here).  Returns (T, hidden).  The prompts attend to themselves causally as they are, the cache holds
+        them in 8 bits for the steps to come.  `rules`: softcap, slopes, distance_bias, window, softmax_scale of `scored_attention`."""
+        self._fits(hidden, cache, 2)
+        T = hidden.shape[0]
+        came = (lengths - cache.lengths).clamp(min=0)
+        # tokens behind the last prompt, and all of them where pages are missing, are nobody's: a document of their own
+        ends = came.cumsum(0)
+        documents = torch.searchsorted(ends, torch.arange(T, device=hidden.device), right=True, out_int32=True).view(1, T)
+        slots, _ = cache.resize(lengths, T)
+
+        def attend(layer, q, k, v):
+            q, k, v = (t.transpose(0, 1).unsqueeze(0) for t in (q, k, v))
+            out = torch.empty(1, T, self.head_num, cache.head_dim, dtype=hidden.dtype, device=hidden.device)
+            scored_attention(q, k, v, causal=True, documents=documents, out=out.transpose(1, 2), **rules)
+            return out.view(T, -1)
+
+        return self._generate(hidden, cache, slots, attend)
+
+    def step(self, hidden: torch.Tensor, cache, active: torch.Tensor = None, **rules) -> torch.Tensor:
+        """The next n tokens of every request: hidden (max_requests, n, hidden) -> the same shape.  `active` (max_requests) int32 of 1
+        and 0 says which requests take them (default: those that hold tokens); the rows of the others give nothing of use.  Everything
+        stays on the GPU; a captured step can be replayed."""
+        self._fits(hidden, cache, 3)
+        R, n, hid = hidden.shape
+        if R != cache.lengths.shape[0]:
+            raise _lib.StofError(f"generation: tokens of {R} requests, the cache is for {cache.lengths.shape[0]}")
+        if active is None:
+            active = (cache.lengths > 0).int()
+        # tokens of requests that take none have no slot: the slots of those that do, put to their rows
+        slots, starts = cache.resize(cache.lengths + active * n, R * n)
+        at = starts[:-1].unsqueeze(1) + torch.arange(n, dtype=torch.int32, device=hidden.device)
+        slots = torch.where(active.unsqueeze(1) > 0, slots[at.clamp(max=R * n - 1).long()], -1).view(-1)
+
+        def attend(layer, q, k, v):
+            return cache.attention(layer, q.unflatten(0, (R, n)), **rules).view(R * n, -1)
+
+        return self._generate(hidden.reshape(R * n, hid), cache, slots, attend).view(R, n, hid)
 
     def capture(self, hidden: torch.Tensor):
         """Records one forward pass on `hidden` (a tensor the caller keeps and refills in place) into a CUDA graph and returns
