@@ -247,7 +247,9 @@ extern "C" int stof_page_tables(const int* lengths, const int* held, int request
     // slots of many tokens: a kernel of their own, which stores 16 bytes at a time
     const bool apart = slot_count >= PT_MANY && aligned16(slots);
     if (apart) p.slots = nullptr;
-    const int cluster = requests > 4 * PT_WARPS || (!apart && slot_count >= PT_MANY) ? PT_MAX_CLUSTER : 1;
+    // A step (a token or two for each request) is done by the requests' own threads: one block, which also starts faster than a cluster.
+    // Else warps see to prompts and to requests that leave, and there are more of them in a cluster.
+    const int cluster = requests <= PT_THREADS && slot_count <= 2 * requests ? 1 : requests > 4 * PT_WARPS || (!apart && slot_count >= PT_MANY) ? PT_MAX_CLUSTER : 1;
     LaunchConfig lc(dim3(static_cast<unsigned>(cluster)), PT_THREADS, 0, stream, static_cast<unsigned>(cluster));
     STOF_CUDA(cudaLaunchKernelEx(&lc.cfg, page_tables_kernel, p));
     if (apart) {
