@@ -14,6 +14,11 @@
 // Work is counted in units of 128 keys (32 for each of a block's four warps).  The units of a (request, K/V head, row group) are cut into
 // pieces of about the same length everywhere, a piece a block, whatever the lengths of the requests (which only the device knows).
 // What one block covers is written at once, the rest in parts that cache_attn_join_kernel adds in the order of the blocks.
+//
+// Measured (int8 or e4m3 alike, pages of 16 to 128 alike): 96 requests of up to 16000 tokens, 32 heads on 8 of 128 (1.78 GB), 297 us = 6.0 TB/s,
+// bound by memory; 48 of up to 8000, 32 heads on 8 of 64 (0.22 GB), 76 us = 2.9 TB/s, bound by the instructions of a key, of which a row of 64
+// has almost as many as one of 128 for half the bytes (issue slots 60 % taken); one request of 4000 tokens 10 us, where the chain launch -
+// lengths - pages' numbers - entries - parts - joining launch is all there is.
 #include "cache_common.cuh"
 #include "stof_host.h"
 #include "stof_ptx.cuh"
@@ -24,19 +29,11 @@ namespace {
 constexpr int CT_WARPS = 4, CT_THREADS = CT_WARPS * 32;
 constexpr int CT_TILES = 2;                  // tiles of 16 keys that a warp takes at a time: independent chains of products, and half the work around them
 constexpr int CT_STEP = 16 * CT_TILES, CT_UNIT = CT_STEP * CT_WARPS;     // keys of a warp's step, of a block's: the unit
-#ifndef CT_STAGES64
-#define CT_STAGES64 3
-#endif
-#ifndef CT_LONG
-#define CT_LONG 16
-#endif
-#ifndef CT_WAVES
-#define CT_WAVES 4
-#endif
-#ifndef CT_BLOCKS64
-#define CT_BLOCKS64 4
-#endif
-constexpr int ct_blocks(int nt, int dim) { return nt == 2 ? 2 : dim == 64 ? CT_BLOCKS64 : 3; }   // on an SM
+constexpr int CT_STAGES = 2;                 // of a warp's ring: one step on its way while one is used (three: the same times, and less on an SM)
+constexpr unsigned CT_LONG = 16, CT_WAVES = 4;                           // see piece_units
+// Blocks on an SM: as many as registers (and for D = 128 shared memory) hold without spills.  D = 64, 16 requests of 12 heads: 22.0 us with
+// four, 25.7 with three, 22.0 to 22.8 with five and six that spill a little.
+constexpr int ct_blocks(int nt, int dim) { return nt == 2 ? 2 : dim == 64 ? 4 : 3; }
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct CacheAttnParams {
@@ -72,8 +69,9 @@ __device__ __forceinline__ Span span_of(const CacheAttnParams& p, int b) {
 
 // How long the pieces are that the (request, K/V head, row group)s are cut into, in units, for `total` units in `pairs` of them: such that
 // there are about as many pieces as blocks that the GPU holds at once (a piece too many would wait for a whole round: every pair rounds
-// up, by half a piece on average), or more of CT_LONG units where there is work for more, so that blocks that get on faster take over
-// from the others towards the end.
+// up, by half a piece on average), or more of CT_LONG units where there is work for more, up to CT_WAVES times as many, so that blocks that
+// get on faster take over from the others towards the end (96 requests of up to 16000 tokens: 297 us; once as many 355, twice 312, eight
+// times 302; pieces of 8 or 32 units at least make no difference).
 __device__ __forceinline__ unsigned piece_units(unsigned total, unsigned pairs, unsigned resident) {
     const unsigned at_once = pairs < resident ? resident - pairs / 2 : resident;
     const unsigned target = max(at_once, min(total / CT_LONG, resident * CT_WAVES));
@@ -95,7 +93,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 // once meet all banks.
 template <int D>
 struct Ring {
-    static constexpr int STAGES = D == 64 ? CT_STAGES64 : 2;
+    static constexpr int STAGES = CT_STAGES;
     static constexpr int SIDE = 16 * D, TILE = 2 * SIDE + 16, STAGE = CT_TILES * TILE;       // of a tile: K, V, {k scale, v scale, valid, -}
     static constexpr int BYTES = STAGES * STAGE;
     static constexpr int CHUNKS = D / 16, LOADS = CHUNKS / 2;                // of a row; copies of a lane per side

@@ -6,12 +6,20 @@
 // thread - and its own list of tiles: those that the rules leave anything of.  While one half's warps work on their scores the tensor
 // core serves the other half.
 //   warps 0..3 (and 4..7)   softmax of the half
-//   next warp               TMA producer: Q, then K and V tiles through a ring of two slots each
+//   next warp               TMA producer: Q, then K and V tiles through rings of slots (scored_slots)
 //   last warp               tcgen05 issuer
-// Where tensor memory has room (OWN_P: all but two halves of D = 128) P lies beside S, and S = Q K^T of the next tile is issued as soon
-// as S has been read into registers; else P lies over S and the next product waits for O += P V.  P is handed over in two parts.
+// Where tensor memory has room (OWN_P: D = 64) P lies beside S, and S = Q K^T of the next tile is issued as soon as S has been read into
+// registers; else P lies over S and the next product waits for O += P V.  P is handed over in two parts.
 // A tile is classified per warp (32 rows): nothing to mask, or masked by 128 bits a row.
-// What a call does not use is not in its kernel's loop (MODE): the loop a warp spends its time in has to fit the instruction caches.
+// What a call does not use is not in its kernel's loop (WHAT): the loop a warp spends its time in has to fit the instruction caches.
+//
+// What bounds it: long sequences the softmax warps.  A tile of 2 x 128 rows costs the tensor core 1024 cycles (D = 128) and the
+// exponentials 2048 (16 a cycle and scheduler quarter); with the loads from tensor memory, the maxima and the packing a warp comes to
+// about 3300 between two tiles of its own: 8192 x 8192, 32 heads on 8 of 128: 860 us = 1278 TFLOP/s, causal 450, causal with cap and prefix
+// 565; heads of 64, where the exponentials stand against half the products: 730 us = 753 TFLOP/s.  Short ones a block's beginning and end (the chain
+// launch - Q, K - S - softmax - O - store, 4 to 6 us, half of it hidden by the other block on the SM).  Measured and slower: a persistent grid
+// (1.8 us less per block, more per tile: 4 x 12 x 1120 with documents 35 us against 29, 2 x 32 x 2048 queries with a window 145 against
+// 138); part of the exponentials as polynomials (plain 3 % faster, with a cap slower, and a NaN is lost); eight chains of maxima.
 #pragma once
 
 #include "cache_common.cuh"
@@ -23,6 +31,7 @@ namespace stof {
 constexpr int SA_T = 128;                    // rows of a half, keys of a tile
 constexpr int SA_PAD = 160;                  // the distance table in shared memory goes on for so long on both sides: a tile that meets the table needs no clamp
 constexpr float SA_RESCALE = 8.0f;           // log2 units by which a row's maximum may outgrow the reference of its P (P <= 2^8)
+constexpr long long SA_DRAIN_CYCLES = 1 << 17;
 constexpr float SA_LOG2E = 1.4426950408889634f;
 enum { SA_PLAIN = 0, SA_CAP = 1, SA_ANY = 2, SA_DOCS = 4 };   // what is done to scores: nothing, the cap alone, whatever the call asks for; and documents
 
@@ -188,13 +197,11 @@ static __device__ __forceinline__ void rescale_o(uint32_t t_o, float alpha) {
 }
 
 // Registers are moved to the softmax warps from the others (setmaxnreg, which is a whole warpgroup's: two of the others' four warps are
-// idle).  Two halves: 384 x 168 at the launch, 256 x R + 128 x r afterwards.  One half of D = 64, two blocks on an SM: 256 x 128, then
-// 128 x R + 128 x r.  One half of D = 128 has the SM to itself and 255 each.
+// idle).  Two halves: 384 x 168 at the launch, 256 x R + 128 x r afterwards.  One half, two blocks on an SM: 256 x 128, then 128 x R + 128 x r.
 constexpr int SA_R2 = 224, SA_R1 = 208;      // (216 and 232, 200 and 216: up to 3 % slower)
 constexpr int scored_threads(int halves) { return halves == 2 ? 384 : 256; }
-constexpr int scored_per_sm(int dim, int halves) { return halves == 1 ? 2 : 1; }
-constexpr int scored_slots(int dim, int halves) { return dim == 128 && halves == 1 ? 1 : 2; }
-constexpr bool scored_moves(int dim, int halves) { return halves == 2 || scored_per_sm(dim, halves) == 2; }
+constexpr int scored_per_sm(int halves) { return halves == 1 ? 2 : 1; }
+constexpr int scored_slots(int dim, int halves) { return dim == 128 && halves == 1 ? 1 : 2; }       // as many as shared memory holds
 constexpr int scored_regs_softmax(int halves) { return halves == 2 ? SA_R2 : SA_R1; }
 constexpr int scored_regs_other(int halves) { return halves == 2 ? (384 * 168 - 256 * SA_R2) / 128 : (256 * 128 - 128 * SA_R1) / 128; }
 static_assert(256 * SA_R2 + 128 * scored_regs_other(2) <= 384 * 168 && 128 * SA_R1 + 128 * scored_regs_other(1) <= 256 * 128 && SA_R1 % 8 == 0 && SA_R2 % 8 == 0 &&
@@ -206,7 +213,7 @@ struct Reach {
 };
 
 template <int D, int HALVES, bool BF16, int WHAT>
-__global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(D, HALVES)) scored_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(HALVES)) scored_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_o,
                                                                         const ScoredParams p) {
     constexpr int MODE = WHAT & 3;
@@ -214,7 +221,7 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(D, HALVE
     constexpr int PANELS = D / 64;                           // 64-column panels of a tile, 128 rows of 128 swizzled bytes each
     constexpr int PANEL_BYTES = SA_T * 128, TILE_BYTES = PANELS * PANEL_BYTES;
     constexpr int W_LOAD = HALVES * 4, W_MMA = W_LOAD + 1;
-    constexpr bool OWN_P = scored_per_sm(D, HALVES) * HALVES * (SA_T + SA_T / 2 + D) <= 512;
+    constexpr bool OWN_P = scored_per_sm(HALVES) * HALVES * (SA_T + SA_T / 2 + D) <= 512;
     constexpr unsigned SLOTS = scored_slots(D, HALVES);     // of K, and of V
     constexpr int COL_O = HALVES * SA_T, COL_P = OWN_P ? COL_O + HALVES * D : 0, P_STEP = OWN_P ? SA_T / 2 : SA_T;
     constexpr int TMEM_COLS = (OWN_P ? COL_P + HALVES * SA_T / 2 : COL_O + HALVES * D) > 256 ? 512 : 256;
@@ -308,7 +315,7 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(D, HALVE
         }
         return t;
     };
-    // the n-th tile goes into slot n % 2 of its side, K a tile ahead of V
+    // the n-th tile goes into slot n % SLOTS of its side, K a tile ahead of V
     auto load = [&](int kind, int t, unsigned n) {
         const int s = static_cast<int>(n % SLOTS);
         uint64_t *full = &bars[(kind == 0 ? SB_K_FULL : SB_V_FULL) + s], *empty = &bars[(kind == 0 ? SB_K_EMPTY : SB_V_EMPTY) + s];
@@ -373,7 +380,7 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(D, HALVE
     const int fix_tile = k_end < p.k_len && k_end % SA_T != 0 ? k_end / SA_T : -1;
 
     if (warp < HALVES * 4) {
-        if constexpr (scored_moves(D, HALVES)) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(scored_regs_softmax(HALVES)));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(scored_regs_softmax(HALVES)));
         if (*abort_flag == 0) {
             // ---------------------------------------------------------------- softmax: one row a thread
             const int h = HALVES == 2 ? warp >> 2 : 0, tid = threadIdx.x & 127;
@@ -626,7 +633,7 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(D, HALVE
             }
         }
     } else {
-        if constexpr (scored_moves(D, HALVES)) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(scored_regs_other(HALVES)));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(scored_regs_other(HALVES)));
         if (*abort_flag == 0 && warp == W_LOAD) {
             // ---------------------------------------------------------------- TMA producer
             int fix_slot = -1;
@@ -695,12 +702,7 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(D, HALVE
                     wait(SB_K_FULL, 0);
 #pragma unroll
                     for (int h = 0; h < HALVES; ++h)
-                        if (wanted(h, t)) {
-                            // the second half half a tile behind the first: in step, both would wait for the exponential unit at one time and leave
-                            // it idle at the other (heads of 64 835 -> 786 us over 8192 x 32 x 8192)
-                            if (OWN_P && h == 1 && wanted(0, t)) wait(SB_P0, 0);
-                            qk(h, 0);
-                        }
+                        if (wanted(h, t)) qk(h, 0);
                     tc_commit_addr(bar0 + 8 * SB_K_EMPTY);
                 }
                 for (unsigned n = 0; t < t_end; ++n) {
@@ -741,6 +743,8 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(D, HALVE
     __syncthreads();
     if (warp == W_MMA) {
         tc_fence_after();
+        if (*abort_flag != 0)                                // a wait ran out: copies and products in flight end before their memory is given back
+            for (const long long t0 = clock64(); clock64() - t0 < SA_DRAIN_CYCLES;) {}
         tmem_dealloc(tmem, TMEM_COLS);
     }
 }

@@ -13,6 +13,8 @@ from .fused import EPILOGUES, gemm_bias, gemm_bias_act, gemm_bias_residual_layer
 from .masks import get_sparse_storage
 from .scored import scored_attention
 
+MAX_PROMPT_TOKENS = 131072                   # what `scored_attention` takes of keys with documents
+
 
 @dataclass
 class EncoderWeights:
@@ -107,6 +109,8 @@ class BertEncoder:
         if hidden.dim() != dims or hidden.shape[-1] != cache.heads * cache.head_dim or cache.heads != self.head_num or cache.layers != len(self.layers):
             raise _lib.StofError(f"generation: {dims} dimensions, the last of {cache.heads * cache.head_dim}, and a cache of {len(self.layers)} layers with "
                                  f"{self.head_num} heads expected")
+        if hidden.dtype != torch.float16:                    # (before anything has been done to the cache)
+            raise _lib.StofError(f"generation: float16 expected, got {hidden.dtype}")
 
     def _generate(self, x, cache, slots, attend):
         """x (T, hidden) through all layers: new keys and values go to the cache, `attend(layer, q, k, v)` gives (T, hidden)."""
@@ -119,12 +123,15 @@ class BertEncoder:
         return x
 
     def prefill(self, hidden: torch.Tensor, cache, lengths: torch.Tensor, **rules) -> torch.Tensor:
-        """Prompts into a `GenerationCache`: hidden (T, hidden), the prompts of the requests that come in back to back in the order of the
-        requests; lengths (max_requests) int32: what every request holds afterwards (requests that are in the cache already keep
-        theirs, or are let go with 0; their tokens come by `step`, not here).  Returns (T, hidden).  The prompts attend to themselves causally as they are, the cache holds
-        them in 8 bits for the steps to come.  `rules`: softcap, slopes, distance_bias, window, softmax_scale of `scored_attention`."""
+        """Prompts into a `GenerationCache`: hidden (T, hidden), T at most 131072, the prompts of the requests that come in back to back in the
+        order of the requests; lengths (max_requests) int32: what every request holds afterwards (requests that are in the cache
+        already keep theirs, or are let go with 0; their tokens come by `step`, not here).  Returns (T, hidden).  The prompts attend
+        to themselves causally as they are, the cache holds them in 8 bits for the steps to come.  `rules`: softcap, slopes,
+        distance_bias, window, softmax_scale of `scored_attention`."""
         self._fits(hidden, cache, 2)
         T = hidden.shape[0]
+        if T > MAX_PROMPT_TOKENS:
+            raise _lib.StofError(f"generation: {T} tokens of prompts in one call, beyond the maximum of {MAX_PROMPT_TOKENS}")
         came = (lengths - cache.lengths).clamp(min=0)
         # tokens behind the last prompt, and all of them where pages are missing, are nobody's: a document of their own
         ends = came.cumsum(0)

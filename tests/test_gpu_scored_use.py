@@ -243,3 +243,18 @@ def test_a_reported_failure_mutes_the_operators():
     torch.cuda.synchronize()
     word.zero_()
     assert bool((out == 3.0).all()) and bool((one == 3.0).all()) and all(torch.equal(a, b) for a, b in zip(before, cache[:4]))
+
+
+def test_generation_refuses_before_it_changes_the_cache():
+    import stof_b200
+    from test_gpu_generation import HEADS, HID, _weights
+    enc = stof_b200.gpt2_stack([stof_b200.EncoderWeights.from_dict(w, "cuda") for w in _weights(1)], HEADS)
+    cache = stof_b200.GenerationCache(1, HEADS, 2, 300000)
+    lengths = torch.tensor([5, 0], dtype=torch.int32, device="cuda")
+    for x, match in ((torch.zeros(5, HID, dtype=torch.bfloat16, device="cuda"), "float16"), (torch.zeros(131073, HID, dtype=torch.float16, device="cuda"), "131072")):
+        with pytest.raises(stof_b200.StofError, match=match):
+            enc.prefill(x, cache, lengths)
+    with pytest.raises(stof_b200.StofError, match="float16"):
+        enc.step(torch.zeros(2, 1, HID, device="cuda"), cache)
+    cache.check()
+    assert cache.lengths.tolist() == [0, 0]
