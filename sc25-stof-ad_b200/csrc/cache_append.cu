@@ -43,11 +43,7 @@ struct Rows {
         return fmaxf(fmaxf(pair(u.x), pair(u.y)), fmaxf(pair(u.z), pair(u.w)));
     }
     static __device__ __forceinline__ uint2 entries(const uint4& u, float inv) {
-        auto four = [&](uint32_t a, uint32_t b) {
-            const float2 f = unpack_pair<BF16>(a), g = unpack_pair<BF16>(b);
-            return quantise2<E4M3>(f.x, f.y, inv) | (quantise2<E4M3>(g.x, g.y, inv) << 16);
-        };
-        return make_uint2(four(u.x, u.y), four(u.z, u.w));
+        return make_uint2(quantise4<E4M3>(unpack_pair<BF16>(u.x), unpack_pair<BF16>(u.y), inv), quantise4<E4M3>(unpack_pair<BF16>(u.z), unpack_pair<BF16>(u.w), inv));
     }
 };
 
@@ -136,7 +132,7 @@ __device__ __forceinline__ void write_run(const AppendParams& p, int head, int t
                 uint32_t lo, hi;
                 entries_to_half<E4M3>(w, lo, hi);
                 const float2 a = unpack_pair<false>(lo), b = unpack_pair<false>(hi);
-                return quantise2<E4M3>(a.x, a.y, ratio[side]) | (quantise2<E4M3>(b.x, b.y, ratio[side]) << 16);
+                return quantise4<E4M3>(a, b, ratio[side]);
             };
             front[i] = make_uint4(round_again(u.x), round_again(u.y), round_again(u.z), round_again(u.w));
         }

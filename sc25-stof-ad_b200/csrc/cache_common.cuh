@@ -2,7 +2,6 @@
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 #include <stdint.h>
 
 namespace stof {
@@ -33,17 +32,22 @@ __device__ __forceinline__ float fast_reciprocal(float x) {
 template <bool E4M3>
 constexpr float entry_max() { return E4M3 ? 448.0f : 127.0f; }
 
-// round(a * inv), round(b * inv) as two entries in the low 16 bits
+// round(x * inv) of four numbers as entries
 template <bool E4M3>
-__device__ __forceinline__ uint32_t quantise2(float a, float b, float inv) {
-    const float most = entry_max<E4M3>();
-    a *= inv;
-    b *= inv;
+__device__ __forceinline__ uint32_t quantise4(float2 x, float2 y, float inv) {
+    x.x *= inv;
+    x.y *= inv;
+    y.x *= inv;
+    y.y *= inv;
     if constexpr (E4M3) {
-        return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+        uint32_t w;
+        asm("{\n\t.reg .b16 a, b;\n\tcvt.rn.satfinite.e4m3x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 b, %4, %3;\n\tmov.b32 %0, {a, b};\n\t}"
+            : "=r"(w) : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
+        return w;
     } else {
-        const int x = __float2int_rn(fminf(fmaxf(a, -most), most)), y = __float2int_rn(fminf(fmaxf(b, -most), most));
-        return (static_cast<uint32_t>(x) & 0xFFu) | ((static_cast<uint32_t>(y) & 0xFFu) << 8);
+        // next to 1.5 * 2^23 the numbers are integers: the sum is rounded to one, its low byte is the entry (a conversion takes four times as long)
+        auto whole = [](float v) { return __float_as_uint(fminf(fmaxf(v, -127.f), 127.f) + 12582912.f); };
+        return __byte_perm(__byte_perm(whole(x.x), whole(x.y), 0x0040), __byte_perm(whole(y.x), whole(y.y), 0x0040), 0x5410);
     }
 }
 
