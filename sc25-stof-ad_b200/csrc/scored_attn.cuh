@@ -71,6 +71,11 @@ static __device__ __forceinline__ float max3f(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
+static __device__ __forceinline__ float min3f(float a, float b, float c) {
+    float d;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 
 // from_u * tanh(s * to_u) near zero: an odd polynomial of s, the factors in its coefficients.  Relative errors of the fits (weighted least
 // squares moved towards the minimax one): 2.9e-6 of three terms up to |u| = 0.35, 7e-6 of five up to 1; a score of 40 is then off by
@@ -91,6 +96,9 @@ struct NearTanh {
         far[2] = a * w * w * 0.13036811351776123f;
         far[3] = a * w * w * w * -0.044817544519901276f;
         far[4] = a * w * w * w * w * 0.009036419913172722f;
+        // (never 0: minus infinity, a masked score, stays what it is)
+        near[2] = fmaxf(near[2], 1e-45f);
+        far[4] = fmaxf(far[4], 1e-45f);
     }
 };
 template <int N>
@@ -100,6 +108,14 @@ static __device__ __forceinline__ float2 odd_polynomial(float2 s, const float (&
 #pragma unroll
     for (int i = N - 2; i >= 0; --i) q = fma2(q, w, pk2(c[i], c[i]));
     return mul2(q, s);
+}
+template <int N>
+static __device__ __forceinline__ float2 odd_polynomial_plus(float2 s, const float (&c)[N], float2 added) {
+    const float2 w = mul2(s, s);
+    float2 q = pk2(c[N - 1], c[N - 1]);
+#pragma unroll
+    for (int i = N - 2; i >= 0; --i) q = fma2(q, w, pk2(c[i], c[i]));
+    return fma2(q, s, added);
 }
 // tanh(u) = 1 - 2 / (1 + e^(2u)): off by 1e-7, where it is not near zero
 static __device__ __forceinline__ float tanh_any(float u) { return 1.f - 2.f * fast_reciprocal(1.f + fast_exp2(u * (2.f * SA_LOG2E))); }
@@ -446,19 +462,49 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(HALVES))
                 for (int i = 0; i < 4; ++i) tmem_ld32(t_s + 32 * i, s[i]);
                 tc_wait_ld();
 #define S_AT(c) s[(c) >> 5][(c) & 31]
-                if constexpr (MODE != SA_PLAIN) {
-                    if (capped) {
-                        float top = 0.f;
+                // The cap alone: a row's largest score is its largest raw one, capped, so that the polynomial can go into the loop of
+                // exponentials, whose unit is busy all along while the others idle (in_loop 1, 2: which; 0: the scores are final)
+                int in_loop = 0;
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                auto largest = [&] {
 #pragma unroll
-                        for (int c = 0; c < SA_T; c += 2) top = max3f(top, fabsf(__uint_as_float(S_AT(c))), fabsf(__uint_as_float(S_AT(c + 1))));
-                        if (__builtin_expect(__all_sync(0xffffffffu, top <= tanh_near.near_end), 1)) {
+                    for (int c = 0; c < SA_T; c += 8)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) mx[i] = max3f(mx[i], __uint_as_float(S_AT(c + 2 * i)), __uint_as_float(S_AT(c + 2 * i + 1)));
+                    return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                };
+                auto cap_exactly = [&] {
+                    cap_in_tmem(t_s, to_u, from_u);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) tmem_ld32(t_s + 32 * i, s[i]);
+                    tc_wait_ld();
+                };
+                float top = -INFINITY;
+                if constexpr (MODE == SA_CAP) {
+                    float mn[4] = {INFINITY, INFINITY, INFINITY, INFINITY};
+                    top = largest();
+#pragma unroll
+                    for (int c = 0; c < SA_T; c += 8)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) mn[i] = min3f(mn[i], __uint_as_float(S_AT(c + 2 * i)), __uint_as_float(S_AT(c + 2 * i + 1)));
+                    const float reached = fmaxf(top, -fminf(fminf(mn[0], mn[1]), fminf(mn[2], mn[3])));
+                    if (__builtin_expect(__all_sync(0xffffffffu, reached <= tanh_near.near_end), 1)) in_loop = 1;
+                    else if (__all_sync(0xffffffffu, reached <= tanh_near.far_end)) in_loop = 2;
+                    else cap_exactly();
+                }
+                if constexpr (MODE == SA_ANY) {
+                    if (capped) {
+                        float reached = 0.f;
+#pragma unroll
+                        for (int c = 0; c < SA_T; c += 2) reached = max3f(reached, fabsf(__uint_as_float(S_AT(c))), fabsf(__uint_as_float(S_AT(c + 1))));
+                        if (__builtin_expect(__all_sync(0xffffffffu, reached <= tanh_near.near_end), 1)) {
 #pragma unroll
                             for (int c = 0; c < SA_T; c += 2) {
                                 const float2 y = odd_polynomial(pk2(__uint_as_float(S_AT(c)), __uint_as_float(S_AT(c + 1))), tanh_near.near);
                                 S_AT(c) = __float_as_uint(y.x);
                                 S_AT(c + 1) = __float_as_uint(y.y);
                             }
-                        } else if (__all_sync(0xffffffffu, top <= tanh_near.far_end)) {
+                        } else if (__all_sync(0xffffffffu, reached <= tanh_near.far_end)) {
 #pragma unroll
                             for (int c = 0; c < SA_T; c += 2) {
                                 const float2 y = odd_polynomial(pk2(__uint_as_float(S_AT(c)), __uint_as_float(S_AT(c + 1))), tanh_near.far);
@@ -466,10 +512,7 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(HALVES))
                                 S_AT(c + 1) = __float_as_uint(y.y);
                             }
                         } else {
-                            cap_in_tmem(t_s, to_u, from_u);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) tmem_ld32(t_s + 32 * i, s[i]);
-                            tc_wait_ld();
+                            cap_exactly();
                         }
                     }
                 }
@@ -537,12 +580,13 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(HALVES))
                         S_AT(c + 3) = k.w == my_doc ? S_AT(c + 3) : 0xFF800000u;
                     }
                 }
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int c = 0; c < SA_T; c += 8)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) mx[i] = max3f(mx[i], __uint_as_float(S_AT(c + 2 * i)), __uint_as_float(S_AT(c + 2 * i + 1)));
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+                if (in_loop == 0 || !full) {
+                    mx[0] = mx[1] = mx[2] = mx[3] = -INFINITY;
+                    top = largest();
+                }
+                if (in_loop == 1 && top > -INFINITY) top = odd_polynomial(pk2(top, top), tanh_near.near).x;
+                if (in_loop == 2 && top > -INFINITY) top = odd_polynomial(pk2(top, top), tanh_near.far).x;
+                top *= sc;
                 const bool need = top > m_ref + SA_RESCALE || (m_ref == -INFINITY && top > -INFINITY);
                 if (__builtin_expect(__any_sync(0xffffffffu, need), 0)) {
                     float alpha = 1.f;
@@ -564,29 +608,34 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(HALVES))
                 const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;
                 const float2 sc2 = pk2(sc, sc), negm2 = pk2(neg_m, neg_m);
                 float2 sum_a = pk2(0.f, 0.f), sum_b = pk2(0.f, 0.f);
+                auto exponentials = [&](auto&& less_reference) {
 #pragma unroll
-                for (int part = 0; part < 2; ++part) {       // P goes to the issuer in two parts of 64 keys
+                    for (int part = 0; part < 2; ++part) {       // P goes to the issuer in two parts of 64 keys
 #pragma unroll
-                    for (int i = part * 32; i < part * 32 + 32; ++i) {
-                        const float2 x = fma2(pk2(__uint_as_float(S_AT(2 * i)), __uint_as_float(S_AT(2 * i + 1))), sc2, negm2);
-                        const float e0 = fast_exp2(x.x), e1 = fast_exp2(x.y);
-                        if (i & 1) sum_b = add2(sum_b, pk2(e0, e1));
-                        else sum_a = add2(sum_a, pk2(e0, e1));
-                        S_AT(i) = pack_pair<BF16>(e0, e1);   // the scores of pair i were used above
-                    }
-                    if constexpr (OWN_P) {
-                        // the products that read the P before this one have to be through: they are where O is complete
-                        if (part == 0 && done > 0) {
-                            wait_inline(smem_u32(&bars[SB_O + h]), static_cast<uint32_t>((done - 1) & 1), wctx, SB_O + h);
-                            tc_fence_after();
+                        for (int i = part * 32; i < part * 32 + 32; ++i) {
+                            const float2 x = less_reference(pk2(__uint_as_float(S_AT(2 * i)), __uint_as_float(S_AT(2 * i + 1))));
+                            const float e0 = fast_exp2(x.x), e1 = fast_exp2(x.y);
+                            if (i & 1) sum_b = add2(sum_b, pk2(e0, e1));
+                            else sum_a = add2(sum_a, pk2(e0, e1));
+                            S_AT(i) = pack_pair<BF16>(e0, e1);   // the scores of pair i were used above
                         }
+                        if constexpr (OWN_P) {
+                            // the products that read the P before this one have to be through: they are where O is complete
+                            if (part == 0 && done > 0) {
+                                wait_inline(smem_u32(&bars[SB_O + h]), static_cast<uint32_t>((done - 1) & 1), wctx, SB_O + h);
+                                tc_fence_after();
+                            }
+                        }
+                        tmem_st32(t_p + 32 * part, s[part]);
+                        tc_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&bars[(part == 0 ? SB_P0 : SB_P1) + h]);
                     }
-                    tmem_st32(t_p + 32 * part, s[part]);
-                    tc_wait_st();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&bars[(part == 0 ? SB_P0 : SB_P1) + h]);
-                }
+                };
+                if (in_loop == 1) exponentials([&](float2 v) { return odd_polynomial_plus(v, tanh_near.near, negm2); });
+                else if (in_loop == 2) exponentials([&](float2 v) { return odd_polynomial_plus(v, tanh_near.far, negm2); });
+                else exponentials([&](float2 v) { return fma2(v, sc2, negm2); });
                 const float2 sum = add2(sum_a, sum_b);
                 l_sum += sum.x + sum.y;
 #undef S_AT
