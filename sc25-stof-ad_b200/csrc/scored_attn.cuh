@@ -285,16 +285,47 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(HALVES))
     }
     grid_dependency_wait();
     grid_launch_dependents();
-    if (loader) *abort_flag = failure_reported(p.status) ? 1 : 0;
 
     // the heaviest stretches first: with a causal mask those at the end of the sequence
     const int heads_all = p.batch * p.heads;
     const int row_tile = p.q_tiles - 1 - static_cast<int>(blockIdx.x / heads_all), bh = static_cast<int>(blockIdx.x % heads_all);
     const int b = bh / p.heads, head = bh % p.heads, kv = head / p.group;
     const int q0 = row_tile * (SA_T * HALVES), shift = p.k_len - p.q_len;
-    const int k_end = p.key_lens != nullptr ? min(max(p.key_lens[b], 0), p.k_len) : p.k_len;
-    const int prefix = p.prefix_lens != nullptr ? min(max(p.prefix_lens[b], 0), k_end) : 0;
     const int* docs = DOCS ? p.documents + b * p.documents_stride : nullptr;
+    // what a block waits for before its first tile are loads of a word or a few, so all are asked for before any is used
+    const int key_len = p.key_lens != nullptr ? __ldca(p.key_lens + b) : p.k_len, prefix_len = p.prefix_lens != nullptr ? __ldca(p.prefix_lens + b) : 0;
+    const bool muted = loader && failure_reported(p.status);
+    const int my_row = q0 + static_cast<int>(threadIdx.x);
+    int my_doc = 0;
+    if (DOCS && warp < HALVES * 4) my_doc = __ldca(docs + min(my_row, p.q_len - 1) + shift);
+    // (the loading warp has Q and K to see to)
+    const int helper = static_cast<int>(threadIdx.x) - (warp > W_LOAD ? 32 : 0), helpers = scored_threads(HALVES) - 32;
+    if (p.distance_bias != nullptr && warp != W_LOAD) {
+        const float* src = p.distance_bias + static_cast<size_t>(head) * (2 * p.radius + 1);
+        const int count = 2 * p.radius + 1 + 2 * SA_PAD;
+        for (int i0 = helper; i0 < count; i0 += 4 * helpers) {
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = __ldca(src + min(max(i0 + j * helpers - SA_PAD, 0), 2 * p.radius));
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (i0 + j * helpers < count) table[i0 + j * helpers] = v[j] * SA_LOG2E;
+        }
+    }
+    // the documents of the tiles that the rules may want, whatever the lengths are
+    constexpr int DOC_WARPS = scored_threads(HALVES) / 32 - 1;
+    const int r_last = min(q0 + SA_T * HALVES, p.q_len) - 1 + shift;
+    const int doc_from = p.window > 0 && p.prefix_lens == nullptr ? max(q0 + shift - p.window + 1, 0) / SA_T : 0;
+    const int doc_to = (max(min(p.prefix_lens != nullptr ? p.k_len : p.causal ? r_last + 1 : p.window > 0 ? r_last + p.window : p.k_len, p.k_len), 0) + SA_T - 1) / SA_T;
+    int doc_ids[2][4];
+    auto ask_docs = [&](int t) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) doc_ids[n][i] = __ldca(docs + min((t + n * DOC_WARPS) * SA_T + 32 * i + lane, p.k_len - 1));
+    };
+    if (DOCS && warp != W_LOAD) ask_docs(doc_from + helper / 32);
+    const int k_end = min(max(key_len, 0), p.k_len), prefix = min(max(prefix_len, 0), k_end);
 
     auto reach_of = [&](int h) {
         Reach r = {0, 0, 0, 0, 0};
@@ -342,7 +373,8 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(HALVES))
                       p.slot_h[1 + kind]);
     };
     // Q, and the first K where the rules alone say which that is, are on their way while the rest is set up
-    if (loader && *abort_flag == 0) {
+    if (loader) *abort_flag = muted ? 1 : 0;
+    if (loader && !muted) {
         for (int h = 0; h < HALVES; ++h) {
             if (q0 + h * SA_T >= p.q_len) break;
             mbar_arrive_expect_tx(&bars[SB_Q + h], TILE_BYTES);
@@ -351,32 +383,27 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(HALVES))
             if (h == 0 && !DOCS && next(t_begin) < t_end) load(0, next(t_begin), 0);
         }
     }
-    // tables into shared memory
-    if (p.distance_bias != nullptr) {
-        const float* src = p.distance_bias + static_cast<size_t>(head) * (2 * p.radius + 1);
-        for (int i = threadIdx.x; i < 2 * p.radius + 1 + 2 * SA_PAD; i += blockDim.x) table[i] = __ldca(src + min(max(i - SA_PAD, 0), 2 * p.radius)) * SA_LOG2E;
-    }
-    int my_doc = 0;
     if (DOCS) {
-        for (int t = t_begin + warp; t < t_end; t += scored_threads(HALVES) / 32) {
-            int lo = 0x7FFFFFFF, hi = -0x7FFFFFFF - 1;
+        if (warp != W_LOAD)
+            for (int t = doc_from + helper / 32; t < doc_to; t += 2 * DOC_WARPS) {
+                if (t >= doc_from + 2 * DOC_WARPS) ask_docs(t);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int j = t * SA_T + 32 * i + lane;
-                if (j < k_end) {
-                    const int d = __ldca(docs + j);
-                    lo = min(lo, d);
-                    hi = max(hi, d);
+                for (int n = 0; n < 2; ++n) {
+                    int lo = 0x7FFFFFFF, hi = -0x7FFFFFFF - 1;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if ((t + n * DOC_WARPS) * SA_T + 32 * i + lane < k_end) {
+                            lo = min(lo, doc_ids[n][i]);
+                            hi = max(hi, doc_ids[n][i]);
+                        }
+                    lo = __reduce_min_sync(0xffffffffu, lo);
+                    hi = __reduce_max_sync(0xffffffffu, hi);
+                    if (lane == 0 && t + n * DOC_WARPS < doc_to) range[t + n * DOC_WARPS] = make_int2(lo, hi);
                 }
             }
-            lo = __reduce_min_sync(0xffffffffu, lo);
-            hi = __reduce_max_sync(0xffffffffu, hi);
-            if (lane == 0) range[t] = make_int2(lo, hi);
-        }
         if (warp < HALVES * 4) {
-            const int row = q0 + static_cast<int>(threadIdx.x);
-            if (row < p.q_len) my_doc = __ldca(docs + row + shift);
-            const int lo = __reduce_min_sync(0xffffffffu, row < p.q_len ? my_doc : 0x7FFFFFFF), hi = __reduce_max_sync(0xffffffffu, row < p.q_len ? my_doc : -0x7FFFFFFF - 1);
+            const bool there = my_row < p.q_len;
+            const int lo = __reduce_min_sync(0xffffffffu, there ? my_doc : 0x7FFFFFFF), hi = __reduce_max_sync(0xffffffffu, there ? my_doc : -0x7FFFFFFF - 1);
             if (lane == 0) row_docs[warp] = make_int2(lo, hi);
         }
     }
