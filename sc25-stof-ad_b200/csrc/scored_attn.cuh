@@ -555,13 +555,18 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(HALVES))
                     if (p.slopes != nullptr) {
                         if (far <= 0 || near >= 0) {         // all behind or all ahead: -slope * |distance| is linear
                             const float g = far <= 0 ? slope : -slope, at = g * static_cast<float>(k0 - pos);
-                            const float2 now2 = pk2(sc_now, sc_now), g2 = pk2(g, g), at2 = pk2(at, at);
+                            const float2 now2 = pk2(sc_now, sc_now);
+                            const float2 step[4] = {pk2(0.f, g), pk2(2.f * g, 3.f * g), pk2(4.f * g, 5.f * g), pk2(6.f * g, 7.f * g)};
 #pragma unroll
-                            for (int c = 0; c < SA_T; c += 2) {
-                                const float2 y = fma2(pk2(__uint_as_float(S_AT(c)), __uint_as_float(S_AT(c + 1))), now2,
-                                                      fma2(g2, pk2(static_cast<float>(c), static_cast<float>(c + 1)), at2));
-                                S_AT(c) = __float_as_uint(y.x);
-                                S_AT(c + 1) = __float_as_uint(y.y);
+                            for (int c = 0; c < SA_T; c += 8) {
+                                const float from = fmaf(g, static_cast<float>(c), at);
+                                const float2 from2 = pk2(from, from);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const float2 y = fma2(pk2(__uint_as_float(S_AT(c + 2 * i)), __uint_as_float(S_AT(c + 2 * i + 1))), now2, add2(from2, step[i]));
+                                    S_AT(c + 2 * i) = __float_as_uint(y.x);
+                                    S_AT(c + 2 * i + 1) = __float_as_uint(y.y);
+                                }
                             }
                         } else {
                             const float away = static_cast<float>(k0 - pos);
