@@ -590,7 +590,11 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(HALVES))
                             // (rows behind the last one are kept inside the table)
                             const float* at = table + min(max(k0 - pos + p.radius + SA_PAD, 0), 2 * p.radius + 2 * SA_PAD - SA_T + 1);
 #pragma unroll
-                            for (int c = 0; c < SA_T; ++c) S_AT(c) = __float_as_uint(fmaf(__uint_as_float(S_AT(c)), sc_now, at[c]));
+                            for (int c = 0; c < SA_T; c += 2) {
+                                const float2 y = fma2(pk2(__uint_as_float(S_AT(c)), __uint_as_float(S_AT(c + 1))), pk2(sc_now, sc_now), pk2(at[c], at[c + 1]));
+                                S_AT(c) = __float_as_uint(y.x);
+                                S_AT(c + 1) = __float_as_uint(y.y);
+                            }
                         }
                     }
                 }
