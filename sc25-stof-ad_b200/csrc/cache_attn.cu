@@ -287,8 +287,9 @@ __global__ void __launch_bounds__(CT_THREADS, ct_blocks(NT, D)) cache_attn_kerne
         }
 
         auto word = [](const uint4& u, int i) { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; };
-        // up to here every row of the block sees all keys, where no rule hides any
-        const int all_see = p.slopes == nullptr && p.distance_bias == nullptr && p.window == 0 ? span.length - p.tokens + row0 / p.group : -1;
+        // keys [see_from, see_to] are visible to every row of the block (none where a table has to be read for each)
+        const int first_pos = span.length - p.tokens + row0 / p.group, last_pos = span.length - p.tokens + min(row0 + ROWS - 1, p.rows - 1) / p.group;
+        const int see_from = p.window > 0 ? last_pos - p.window + 1 : 0, see_to = p.distance_bias == nullptr ? first_pos : -1;
         auto compute = [&](int key, const unsigned char* tiles) {
             float k_scale[CT_TILES], v_scale[CT_TILES];
             int left[CT_TILES];                              // keys of the tile that exist; what lies behind them may be anything
@@ -370,13 +371,18 @@ __global__ void __launch_bounds__(CT_THREADS, ct_blocks(NT, D)) cache_attn_kerne
 #pragma unroll
                         for (int e = 0; e < 4; ++e) s[t][nt][e] *= k_scale[t] * row_scale[nt][e & 1];
             }
-            if (key + CT_STEP - 1 <= all_see && left[0] > 0 && left[CT_TILES - 1] > 0) {
+            if (key >= see_from && key + CT_STEP - 1 <= see_to && left[0] > 0 && left[CT_TILES - 1] > 0) {
 #pragma unroll
-                for (int t = 0; t < CT_TILES; ++t)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                    for (int e = 0; e < 2; ++e) {
+                        const float away = static_cast<float>(key + g - pos[nt][e]), less = fmaf(slope[nt][e], away, -m[nt][e]);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) s[t][nt][e] -= m[nt][e & 1];
+                        for (int t = 0; t < CT_TILES; ++t) {
+                            s[t][nt][e] += fmaf(slope[nt][e], static_cast<float>(16 * t), less);
+                            s[t][nt][2 + e] += fmaf(slope[nt][e], static_cast<float>(16 * t + 8), less);
+                        }
+                    }
             } else {
 #pragma unroll
                 for (int t = 0; t < CT_TILES; ++t)
