@@ -32,7 +32,7 @@ constexpr int CT_STEP = 16 * CT_TILES, CT_UNIT = CT_STEP * CT_WARPS;     // keys
 constexpr int CT_STAGES = 2;                 // of a warp's ring: one step on its way while one is used (three: the same times, and less on an SM)
 constexpr unsigned CT_LONG = 16, CT_WAVES = 4;                           // see piece_units
 // Blocks on an SM: as many as registers (and for D = 128 shared memory) hold without spills.  D = 64, 16 requests of 12 heads: 22.0 us with
-// four, 25.7 with three, 22.0 to 22.8 with five and six that spill a little.
+// four, 25.7 with three, 22.0 to 22.8 with five and six that spill a little (before slopes had a path without tests: 19.0 now).
 constexpr int ct_blocks(int nt, int dim) { return nt == 2 ? 2 : dim == 64 ? 4 : 3; }
 constexpr float LOG2E = 1.4426950408889634f;
 
