@@ -743,7 +743,7 @@ extern "C" int stof_cache_attn(const void* q, void* out, int dtype, const long l
     p.slopes = rules->slopes; p.distance_bias = rules->distance_bias; p.radius = rules->bias_radius;
     p.parts = static_cast<int2*>(workspace);
     p.workspace = reinterpret_cast<float*>(static_cast<char*>(workspace) + (static_cast<size_t>(s.joins) * sizeof(int2) + 15) / 16 * 16); p.status = status_dev;
-    p.scale = rules->softmax_scale; p.softcap = rules->softcap; p.window = rules->window;
+    p.scale = rules->softmax_scale; p.softcap = usable_cap(rules->softcap); p.window = rules->window;
     p.requests = requests; p.tokens = tokens; p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads;
     p.rows = s.rows; p.row_groups = s.row_groups; p.resident = s.resident;
     p.table_width = table_width; p.page_count = pages; p.bf16 = dtype == STOF_DTYPE_BF16;

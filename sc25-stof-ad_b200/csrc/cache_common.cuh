@@ -22,6 +22,9 @@ __device__ __forceinline__ void entries_to_half(uint32_t w, uint32_t& lo, uint32
     }
 }
 
+// A cap whose inverse and multiples stay inside fp32: scores capped to 1e-30 are all alike, and 1e30 caps none that are told apart
+inline float usable_cap(float cap) { return cap > 0.f ? (cap < 1e-30f ? 1e-30f : cap > 1e30f ? 1e30f : cap) : 0.f; }
+
 // 1 / x to a unit in the last place
 __device__ __forceinline__ float fast_reciprocal(float x) {
     float y;

@@ -992,6 +992,7 @@ PyObject* py_cache_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const char* op = "cache_append";
         need_args(n, 7, op);
         const Cache c = cache_args(a, op);
+        if (c.pages > 0 && (c.k == c.v || c.k_scales == c.v_scales)) fail("%s: keys and values need pages and scales of their own", op);
         const at::Tensor &pages = tensor_needed(a[0], op), &k = tensor_needed(a[4], op), &v = tensor_needed(a[5], op);
         for (const at::Tensor* t : {&k, &v}) need_same_device(pages, t, op);
         const int type = half_type(k, op);

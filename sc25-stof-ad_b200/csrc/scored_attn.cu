@@ -66,7 +66,7 @@ extern "C" int stof_scored_attn(const void* q, const void* k, const void* v, voi
     ScoredParams p;
     p.slopes = rules->slopes; p.distance_bias = rules->distance_bias; p.documents = rules->documents; p.prefix_lens = rules->prefix_lens;
     p.key_lens = rules->key_lens; p.documents_stride = rules->documents_stride; p.status = status_dev;
-    p.scale = rules->softmax_scale; p.softcap = rules->softcap; p.causal = rules->causal != 0; p.radius = rules->bias_radius;
+    p.scale = rules->softmax_scale; p.softcap = usable_cap(rules->softcap); p.causal = rules->causal != 0; p.radius = rules->bias_radius;
     p.window = rules->window > q_len + k_len ? q_len + k_len : rules->window;
     p.batch = batch; p.heads = heads; p.group = heads / kv_heads; p.q_len = q_len; p.k_len = k_len;
     p.table_bytes = rules->distance_bias != nullptr ? (2 * p.radius + 1 + 2 * SA_PAD) * 4 + 4 : 0;       // (an even number of words: pairs follow)

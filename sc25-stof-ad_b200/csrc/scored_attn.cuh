@@ -84,12 +84,12 @@ static __device__ __forceinline__ float min3f(float a, float b, float c) {
 // 3e-4 at most, less than P's rounding to fp16 makes of it.
 struct NearTanh {
     float near[3], far[5];                   // of s, s^3, s^5, ..
-    float near_end, far_end;                 // up to which |s| they are used: 0 where powers of to_u leave fp32's range
-    __device__ __forceinline__ NearTanh() : near{}, far{}, near_end(0.f), far_end(0.f) {}
+    float near_end, far_end;                 // up to which |s| they are used: -1, not even for 0, where powers of to_u leave fp32's range
+    __device__ __forceinline__ NearTanh() : near{}, far{}, near_end(-1.f), far_end(-1.f) {}
     __device__ __forceinline__ NearTanh(float to_u, float from_u) {
         const float w = to_u * to_u, a = to_u * from_u;
-        near_end = to_u < 1e8f ? 0.35f / to_u : 0.f;         // (below 1e-10 the higher terms vanish, and so do they in the sum)
-        far_end = to_u > 2e-4f && to_u < 5e3f ? 1.f / to_u : 0.f;
+        near_end = to_u < 1e8f ? 0.35f / to_u : -1.f;         // (below 1e-10 the higher terms vanish, and so do they in the sum)
+        far_end = to_u > 2e-4f && to_u < 5e3f ? 1.f / to_u : -1.f;
         near[0] = a * 0.9999971389770508f;
         near[1] = a * w * -0.33290955424308777f;
         near[2] = a * w * w * 0.1239503026008606f;
@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(HALVES))
             const uint32_t t_s = t_lane + h * SA_T, t_o = t_lane + COL_O + h * D, t_p = t_lane + COL_P + h * P_STEP;
             constexpr bool changed = MODE != SA_PLAIN;
             const bool capped = MODE == SA_CAP || (MODE == SA_ANY && p.softcap > 0.f);
-            const float to_u = capped ? p.scale / p.softcap : 0.f, from_u = p.softcap * SA_LOG2E;
+            const float to_u = capped ? fminf(p.scale / p.softcap, 1e38f) : 0.f, from_u = p.softcap * SA_LOG2E;
             const uint32_t s_bar = smem_u32(&bars[SB_S + h]);
             NearTanh tanh_near;
             if (capped) tanh_near = NearTanh(to_u, from_u);

@@ -258,3 +258,75 @@ def test_generation_refuses_before_it_changes_the_cache():
         enc.step(torch.zeros(2, 1, HID, device="cuda"), cache)
     cache.check()
     assert cache.lengths.tolist() == [0, 0]
+
+
+MASKS = {"causal": dict(causal=True), "window": dict(window=40), "window causal": dict(window=70, causal=True),
+         "prefix": dict(causal=True, prefix_lens=torch.tensor([77, 0], dtype=torch.int32)), "padded": dict(key_lens=torch.tensor([100, 301], dtype=torch.int32)),
+         "padded to nothing": dict(causal=True, key_lens=torch.tensor([0, 33], dtype=torch.int32))}
+
+
+@pytest.mark.parametrize("mask", MASKS)
+@pytest.mark.parametrize("cap", [1e-38, 1e-3, 1.5, 6.0, 14.0, 50.0, 1e6, 3e38])
+@pytest.mark.parametrize("dim,dtype,q_len,k_len", [(64, "fp16", 333, 333), (128, "bf16", 300, 400), (64, "bf16", 400, 301)])
+def test_the_cap_alone_under_masks(mask, cap, dim, dtype, q_len, k_len):
+    """From scores near zero to far behind the cap in one tensor: the polynomials and the exact form, with scores that the mask takes."""
+    from test_gpu_scored import _both
+    t = TYPES[dtype]
+    q, k, v = _rand((2, 2, q_len, dim), 31, 2.0, t), _rand((2, 1, k_len, dim), 32, 1.0, t), _rand((2, 1, k_len, dim), 33, 1.0, t)
+    q[:, 1] *= 0.01
+    q[:, :, 64:128] = 0                                  # whole warps of rows that score zero everywhere
+    _both(q, k, v, t, softcap=cap, **MASKS[mask])
+
+
+@pytest.mark.parametrize("junk", [float("nan"), float("inf"), -float("inf"), 6e4])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_the_cap_alone_over_junk_behind_the_keys(junk, dim):
+    from test_gpu_scored import _both
+    q, k, v = _rand((2, 2, 260, dim), 34, 2.0), _rand((2, 2, 260, dim), 35), _rand((2, 2, 260, dim), 36)
+    clean = [x.clone() for x in (k, v)]
+    for x in (k, v):
+        x[0, :, 130:] = junk
+        x[1, :, 7:] = junk
+    lens = torch.tensor([130, 7], dtype=torch.int32)
+    for x in clean:
+        x[0, :, 130:] = 0
+        x[1, :, 7:] = 0
+    import stof_b200
+    got = stof_b200.scored_attention(q.cuda(), k.cuda(), v.cuda(), softcap=30.0, key_lens=lens.cuda())
+    _status()
+    _check(got, os_.scored_attention(q, *clean, softcap=30.0, key_lens=lens), clean[1].double(), torch.float16)
+
+
+@pytest.mark.parametrize("rules", [{}, dict(causal=True), dict(window=30), dict(causal=True, softcap=9.0), dict(causal=True, slopes=torch.tensor([0.5, 0.01])),
+                                   dict(window=200, distance_bias=torch.linspace(-1, 1, 2 * 17).view(2, 17)), dict(causal=True, prefix_lens=torch.tensor([50, 1], dtype=torch.int32))])
+@pytest.mark.parametrize("dim,dtype", [(64, "bf16"), (128, "fp16")])
+def test_more_queries_than_keys(rules, dim, dtype):
+    """The first queries sit in front of the first key."""
+    from test_gpu_scored import _both
+    t = TYPES[dtype]
+    _both(_rand((2, 2, 401, dim), 41, 2.0, t), _rand((2, 2, 170, dim), 42, 1.0, t), _rand((2, 2, 170, dim), 43, 1.0, t), t, **rules)
+
+
+def test_append_refuses_one_page_for_keys_and_values():
+    import stof_b200
+    k, _, ks, vs = [x.cuda() for x in _cache([40], 2, 16, 64, torch.int8, 1)][:4]
+    x, slots = _rand((5, 2, 64), 1).cuda(), torch.arange(5, dtype=torch.int32, device="cuda")
+    with pytest.raises(stof_b200.StofError, match="of their own"):
+        stof_b200.cache_append(k, k, ks, vs, x, x, slots)
+    with pytest.raises(stof_b200.StofError, match="of their own"):
+        stof_b200.cache_append(k, k.clone(), ks, ks, x, x, slots)
+
+
+@pytest.mark.parametrize("cap", [1e-38, 1e-3, 1.5, 14.0, 3e38])
+@pytest.mark.parametrize("rules", [{}, dict(window=33), dict(slopes=torch.tensor([0.5, 0.0, 0.1, 2.0])), dict(window=60, slopes=torch.tensor([0.5, 0.0, 0.1, 2.0]))])
+def test_cache_caps_windows_and_slopes_together(cap, rules):
+    import stof_b200
+    cache = _cache([300, 3, 40, 0], 2, 32, 64, torch.int8, 5)
+    for tokens in (1, 5):
+        q = _rand((4, tokens, 4, 64), 6, 2.0)
+        dev = {n: (x.cuda() if isinstance(x, torch.Tensor) else x) for n, x in rules.items()}
+        got = stof_b200.cache_attention(q.cuda(), *(x.cuda() for x in cache), softcap=cap, **dev)
+        _status()
+        want = os_.cache_attention(q, *cache, softcap=cap, **rules)
+        v_max = (cache[1].double().abs() * cache[3].double()[:, :, None, None]).max()
+        _check(got, want, v_max.view(1), torch.float16)
