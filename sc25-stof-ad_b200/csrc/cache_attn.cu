@@ -597,23 +597,18 @@ __global__ void __launch_bounds__(CT_THREADS) cache_attn_join_kernel(const Cache
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     grid_dependency_wait();
     grid_launch_dependents();
-    if (__syncthreads_or(failure_reported(p.status))) return;
     const int pairs = p.kv_heads * p.row_groups;
     const int b = blockIdx.x / pairs, pair = blockIdx.x % pairs, kv = pair / p.row_groups, row = (pair % p.row_groups) * ROWS + blockIdx.y;
     if (row >= p.rows) return;
+    // what the launch costs is its loads one after the other: status, parts and length together, then the first parts and all maxima
     const int2 parts = __ldca(p.parts + blockIdx.x);
+    const bool muted = failure_reported(p.status);
     const bool empty = span_of(p, b).units == 0;             // (its entry was not written)
-    if (!empty && parts.y == 1) return;                      // one block had all of it
+    if (__syncthreads_or(muted) || (!empty && parts.y == 1)) return;         // (one block had all of it)
     const int count = empty ? 0 : parts.y, r = blockIdx.y;
     auto part = [&](int i) { return p.workspace + static_cast<size_t>(parts.x + i) * (ROWS * (D + 2)); };
-    float top = -INFINITY, sum = 0.f, o[EACH];
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) o[e] = 0.f;
-    for (int i = lane; i < count; i += 32) top = fmaxf(top, __ldca(part(i) + r));
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    for (int i0 = warp; i0 < count; i0 += CT_WARPS * AHEAD) {
-        float m[AHEAD], l[AHEAD], x[AHEAD][EACH];
+    float m[AHEAD], l[AHEAD], x[AHEAD][EACH];
+    auto load = [&](int i0) {
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {                    // no branches: all loads are on their way together
             const float* at = part(min(i0 + j * CT_WARPS, count - 1));
@@ -628,6 +623,19 @@ __global__ void __launch_bounds__(CT_THREADS) cache_attn_join_kernel(const Cache
                 x[j][0] = v.x; x[j][1] = v.y;
             }
         }
+    };
+    float top = -INFINITY, sum = 0.f, o[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) o[e] = 0.f;
+    float own = -INFINITY;
+    if (lane < count) own = __ldca(part(lane) + r);
+    if (warp < count) load(warp);
+    top = own;
+    for (int i = lane + 32; i < count; i += 32) top = fmaxf(top, __ldca(part(i) + r));
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    for (int i0 = warp; i0 < count; i0 += CT_WARPS * AHEAD) {
+        if (i0 != warp) load(i0);
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
             // (a part that saw nothing is 0, or NaN)
