@@ -17,7 +17,7 @@
 //
 // Measured (int8 or e4m3 alike, pages of 16 to 128 alike): 96 requests of up to 16000 tokens, 32 heads on 8 of 128 (1.78 GB), 297 us = 6.0 TB/s,
 // bound by memory; 48 of up to 8000, 32 heads on 8 of 64 (0.22 GB), 76 us = 2.9 TB/s, bound by the instructions of a key, of which a row of 64
-// has almost as many as one of 128 for half the bytes (issue slots 60 % taken); one request of 4000 tokens 10 us, where the chain launch -
+// has almost as many as one of 128 for half the bytes (issue slots 60 % taken); one request of 4000 tokens 9.5 us, where the chain launch -
 // lengths - pages' numbers - entries - parts - joining launch is all there is.
 #include "cache_common.cuh"
 #include "stof_host.h"
