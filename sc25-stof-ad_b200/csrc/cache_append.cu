@@ -217,6 +217,7 @@ extern "C" int stof_cache_append(void* k_pages, void* v_pages, float* k_scales, 
     STOF_REQUIRE(aligned16(k_pages) && aligned16(v_pages) && aligned16(k) && aligned16(v), "cache_append: pointers must be 16-byte aligned");
     for (int i = 0; i < 2; ++i)
         STOF_REQUIRE(k_strides[i] % 8 == 0 && v_strides[i] % 8 == 0, "cache_append: strides must be multiples of 8 elements");
+    STOF_REQUIRE(k_pages != v_pages && k_scales != v_scales, "cache_append: keys and values need pages and scales of their own");
     AppendParams p;
     p.pages[0] = k_pages; p.pages[1] = v_pages; p.scales[0] = k_scales; p.scales[1] = v_scales; p.x[0] = k; p.x[1] = v;
     p.token_stride[0] = k_strides[0]; p.head_stride[0] = k_strides[1]; p.token_stride[1] = v_strides[0]; p.head_stride[1] = v_strides[1];

@@ -47,8 +47,8 @@ def cache_append(k_pages, v_pages, k_scales, v_scales, k, v, slots) -> None:
     that is there and, where the scale grows, the entries in front of the run are rounded again to it.  entry = round(x * (1 / scale)).
 
     A page may hold one run of a call only: with two runs in one page - the same slot twice, say - its contents and scales are
-    undefined.  Slots behind the cache are reported through the status word and not written.  An infinity in k or v makes its page's
-    scale infinite."""
+    undefined.  Keys and values have pages and scales of their own.  Slots behind the cache are reported through the status word and
+    not written.  An infinity in k or v makes its page's scale infinite."""
     (_lib._native or _lib.native()).cache_append(k_pages, v_pages, k_scales, v_scales, k, v, slots)
 
 

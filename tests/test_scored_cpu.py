@@ -99,6 +99,10 @@ def test_cache_append_refusals(lib, kw, text):
     assert _append(lib, **kw) == -1 and text in lib.stof_last_error()
 
 
+def test_cache_append_refuses_one_page_for_keys_and_values(lib):
+    assert _append(lib) == -1 and b"of their own" in lib.stof_last_error()
+
+
 def test_cache_append_of_nothing(lib):
     assert _append(lib, tokens=0) == 0
 
