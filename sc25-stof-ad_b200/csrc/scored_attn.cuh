@@ -253,7 +253,6 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(HALVES))
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     __shared__ int2 row_docs[HALVES * 4];                    // smallest and largest document of each softmax warp's rows
-    __shared__ __align__(16) int key_docs[HALVES][2][SA_T];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int* abort_flag = &abort_word;
@@ -457,7 +456,6 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(HALVES))
             const int full_prefix = prefix / SA_T, full_from = p.window > 0 ? max(pos1 - p.window + SA_T, 0) / SA_T : 0;
             const int full_to = max(min(p.causal ? pos0 + 1 : p.window > 0 ? pos0 + p.window : p.k_len, k_end), 0) / SA_T;
             float m_ref = -INFINITY, l_sum = 0.f;
-            int doc_tile = -1, doc_ahead = 0;
             int done = 0;
             for (int t = mine.prefix > 0 ? 0 : mine.lo; t < mine.hi; ++t) {
                 if (t < mine.lo && t >= mine.prefix) {                       // from the prefix to the window
@@ -470,18 +468,27 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(HALVES))
                 }
                 const int k0 = t * SA_T;
                 const bool full = t < full_prefix || (t >= full_from && t < full_to);
-                bool same_doc = true, mixed = false;         // mixed: the half's rows or the tile's keys are of more than one document
+                // Which keys are of the row's document: a ballot for each document among the warp's rows (one to three of them, where
+                // sequences are packed), before the scores are there
+                bool one_doc = true;
+                uint32_t doc_keys[4] = {0u, 0u, 0u, 0u};
                 if (DOCS) {
                     const int2 d = range[t];
-                    same_doc = d.x == d.y && warp_docs.x == warp_docs.y && d.x == warp_docs.x;
-                    mixed = d.x != d.y || mine.doc_min != mine.doc_max;
-                    if (mixed) {                             // the keys' documents, 128 threads together: all warps of the half or none
-                        int* stage = key_docs[h][done & 1];
-                        stage[tid] = t == doc_tile ? doc_ahead : k0 + tid < k_end ? __ldca(docs + k0 + tid) : 0;
-                        doc_tile = t + 1;                    // most likely the next one
-                        doc_ahead = k0 + SA_T + tid < k_end ? __ldca(docs + k0 + SA_T + tid) : 0;
-                        if (HALVES == 1 || h == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
-                        else asm volatile("bar.sync 2, 128;" ::: "memory");
+                    one_doc = d.x == d.y && warp_docs.x == warp_docs.y && d.x == warp_docs.x;
+                    if (!one_doc) {
+                        int key_doc[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) key_doc[i] = __ldca(docs + min(k0 + 32 * i + lane, p.k_len - 1));
+                        for (unsigned rest = 0xffffffffu; rest != 0u;) {
+                            const int doc = __shfl_sync(0xffffffffu, my_doc, __ffs(rest) - 1);
+                            const bool is = my_doc == doc;
+                            rest &= ~__ballot_sync(0xffffffffu, is);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const uint32_t keys = __ballot_sync(0xffffffffu, key_doc[i] == doc);
+                                doc_keys[i] = is ? keys : doc_keys[i];
+                            }
+                        }
                     }
                 }
                 wait_inline(s_bar, static_cast<uint32_t>(done & 1), wctx, SB_S + h);
@@ -600,23 +607,16 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(HALVES))
                         }
                     }
                 }
-                if (__builtin_expect(!full, 0)) {
-                    const uint4 on = visible_keys(see_lo - k0, see_hi - k0, prefix - k0, k_end - k0);
-                    const uint32_t word[4] = {on.x, on.y, on.z, on.w};
+                if (__builtin_expect(!full || !one_doc, DOCS)) {
+                    const uint4 on = full ? make_uint4(~0u, ~0u, ~0u, ~0u) : visible_keys(see_lo - k0, see_hi - k0, prefix - k0, k_end - k0);
+                    uint32_t word[4] = {on.x, on.y, on.z, on.w};
+                    if (DOCS && !one_doc) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) word[i] &= doc_keys[i];
+                    }
 #pragma unroll
                     for (int c = 0; c < SA_T; ++c)
                         if ((word[c >> 5] & (1u << (c & 31))) == 0) S_AT(c) = 0xFF800000u;
-                }
-                if (__builtin_expect(mixed && !same_doc, 0)) {
-                    const int* stage = key_docs[h][done & 1];
-#pragma unroll
-                    for (int c = 0; c < SA_T; c += 4) {
-                        const int4 k = *reinterpret_cast<const int4*>(stage + c);
-                        S_AT(c) = k.x == my_doc ? S_AT(c) : 0xFF800000u;
-                        S_AT(c + 1) = k.y == my_doc ? S_AT(c + 1) : 0xFF800000u;
-                        S_AT(c + 2) = k.z == my_doc ? S_AT(c + 2) : 0xFF800000u;
-                        S_AT(c + 3) = k.w == my_doc ? S_AT(c + 3) : 0xFF800000u;
-                    }
                 }
                 if (in_loop == 0 || !full) {
                     mx[0] = mx[1] = mx[2] = mx[3] = -INFINITY;
