@@ -1,0 +1,136 @@
+"""`cache_attention` where a warp takes several steps: caches of so many keys that the pieces that thread blocks take are of two units of 128
+keys and more.  Against the definition in 64 bits (on the GPU, whole requests at a time), with bounds from the keys that carry weight."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+MOST = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
+
+
+def _status():
+    from stof_b200 import _lib
+    torch.cuda.synchronize()
+    _lib.check_status(torch.device("cuda"), "test")
+
+
+def _steps(lengths, kv_heads, rows, dim):
+    """Units of a piece, as the kernel deals them: the fewest steps that a warp of a full piece takes (row tiles of 8: one up to 8 rows)."""
+    resident = torch.cuda.get_device_properties(0).multi_processor_count * (2 if rows > 8 else 4 if dim == 64 else 3)
+    pairs = kv_heads * -(-rows // (16 if rows > 8 else 8))
+    total, some = pairs * sum(-(-n // 128) for n in lengths), pairs * sum(n > 0 for n in lengths)
+    target = max(resident - some // 2 if some < resident else resident, min(total // 16, 4 * resident))
+    return max(-(-total // target), 1)
+
+
+def _cache(lengths, kv_heads, page, dim, entry, seed):
+    """Pages in random order with random entries and scales that make values of unit size."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    blocks = [-(-n // page) for n in lengths]
+    pages = sum(blocks) + 3
+    order = torch.randperm(pages, generator=g, device="cuda").int()
+    table, at = torch.zeros(len(lengths), max(blocks), dtype=torch.int32, device="cuda"), 0
+    for b, n in enumerate(blocks):
+        table[b, :n] = order[at:at + n]
+        at += n
+
+    def entries():
+        x = (torch.randn(pages, kv_heads, page, dim, generator=g, device="cuda") * (MOST[entry] / 4)).clamp(-MOST[entry], MOST[entry])
+        return (x.round() if entry == torch.int8 else x).to(entry)
+
+    scales = [(torch.rand(pages, kv_heads, generator=g, device="cuda") + 0.5) * 4 / MOST[entry] for _ in range(2)]
+    return entries(), entries(), *scales, table, torch.tensor(lengths, dtype=torch.int32, device="cuda")
+
+
+def _q(requests, tokens, heads, dim, dtype, seed, scale=2.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(requests, tokens, heads, dim, generator=g, device="cuda") * scale).to(dtype)
+
+
+def _request(pages, scales, row, length):
+    """(Hkv, length, D) float64 of one request, and every key's scale (Hkv, length)."""
+    at = row[:-(-length // pages.shape[2])].long()
+    x = pages.view(torch.int8)[at].view(pages.dtype).float().double().transpose(0, 1).flatten(1, 2)[:, :length]
+    s = scales[at].double().t().repeat_interleave(pages.shape[2], 1)[:, :length]
+    return x * s[..., None], s
+
+
+def _check(q, cache, **rules):
+    """What rounding allows.  With u = 2^-11 or 2^-8 of the output's type: the output is rounded once, u |o|.  Every p is rounded to fp16
+    for the product, together with V's scale: 2^-11 of sum(p |v|), and 2^-25 each where it is that small beside a largest p |scale| of
+    a half at least, so n 2^-24 max(p |scale|) max|entry|.  Sums in fp32: 2^-14 of sum(p |v|) is more than chains of a hundred make
+    of it.  A score is off by 2^-20 of the sum of its parts' magnitudes (products of 128 terms added in fp32, a few factors), a capped
+    one by 3e-6 of itself and 3e-7 of the cap; its p by as much relative, and so the sums that it is in."""
+    import stof_b200
+    kp, vp, ks, vs, table, lengths = cache
+    got = stof_b200.cache_attention(q, *cache, **rules)
+    _status()
+    B, T, H, D = q.shape
+    N = kp.shape[1]
+    group, window, cap, slopes, bias = H // N, rules.get("window"), rules.get("softcap"), rules.get("slopes"), rules.get("distance_bias")
+    scale, u = rules.get("softmax_scale", D ** -0.5), torch.finfo(q.dtype).eps / 2
+    assert got.shape == q.shape and got.dtype == q.dtype and bool(torch.isfinite(got).all())
+    for b, length in enumerate(lengths.tolist()):
+        if length == 0:
+            assert not got[b].any()
+            continue
+        k, _ = _request(kp, ks, table[b], length)
+        v, v_scale = _request(vp, vs, table[b], length)
+        qd = q[b].double().transpose(0, 1).reshape(N, group * T, D)                          # heads of a K/V head, tokens inside
+        x, off = scale * (qd @ k.transpose(1, 2)), scale * (qd.abs() @ k.abs().transpose(1, 2)) * 2.0 ** -20
+        if cap:
+            x = cap * torch.tanh(x / cap)
+            off = off + 3e-6 * x.abs() + 3e-7 * cap
+        pos = (torch.arange(T, device="cuda") + length - T).repeat(group)
+        away = torch.arange(length, device="cuda")[None, :] - pos[:, None]
+        add = torch.zeros(H, T, length, dtype=torch.float64, device="cuda")
+        if slopes is not None:
+            add = add + slopes.double().view(H, 1, 1) * away.view(group, T, length)[0]
+        if bias is not None:
+            radius = bias.shape[1] // 2
+            add = add + bias.double()[:, away.view(group, T, length)[0].clamp(-radius, radius) + radius]
+        add = add.view(N, group * T, length)
+        x, off = x + add, off + add.abs() * 2.0 ** -20
+        on = (away <= 0) & (pos >= 0)[:, None]
+        if window is not None:
+            on &= away > -window
+        x = x.masked_fill(~on, -math.inf)
+        none = ~on.any(1)
+        x[:, none] = 0.0
+        p = torch.softmax(x, 2)
+        p[:, none] = 0.0
+        off = torch.where(p > 0, off, 0.0)
+        want, size = p @ v, p @ v.abs()
+        allow = u * want.abs() + (2.0 ** -11 + 2.0 ** -14) * size + (p * off) @ v.abs() + want.abs() * (p * off).sum(2, keepdim=True) \
+            + length * 2.0 ** -24 * (p * v_scale.abs()[:, None]).amax(2, keepdim=True) * MOST[vp.dtype] + 2.0 ** -25
+        mine = got[b].double().transpose(0, 1).reshape(N, group * T, D)
+        over = (mine - want).abs() - allow
+        assert float(over.max()) <= 0, f"request {b}: off by {float((mine - want).abs().max()):.3e}, bound exceeded by {float(over.max()):.3e}"
+    return got
+
+
+LONG = [4000, 1, 4100, 0, 2049, 3333, 5000, 4224]
+
+
+@pytest.mark.parametrize("dim,heads,kv_heads,tokens,dtype", [(64, 8, 8, 1, torch.float16), (64, 8, 8, 4, torch.bfloat16), (128, 16, 8, 2, torch.bfloat16), (64, 16, 4, 5, torch.float16),
+                                                             (128, 32, 8, 6, torch.float16)])
+@pytest.mark.parametrize("entry,page", [(torch.int8, 16), (torch.float8_e4m3fn, 64), (torch.int8, 128)])
+def test_several_steps(dim, heads, kv_heads, tokens, dtype, entry, page):
+    assert _steps(LONG, kv_heads, tokens * heads // kv_heads, dim) >= 2
+    _check(_q(len(LONG), tokens, heads, dim, dtype, 1), _cache(LONG, kv_heads, page, dim, entry, 2))
+
+
+@pytest.mark.parametrize("rules", [dict(softcap=3.0), dict(softcap=30.0), dict(window=1000), dict(window=2500, softcap=40.0), dict(slopes=True), dict(slopes=True, window=3000), dict(bias=128),
+                                   dict(bias=2048, softcap=5.0)])
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_several_steps_under_rules(rules, tokens):
+    """(slopes up to one a key: the references of rows move at every step)"""
+    lengths = LONG * 3
+    assert _steps([min(n, rules.get("window", n)) for n in lengths], 8, tokens, 64) >= 2
+    rules, g = dict(rules), torch.Generator(device="cuda").manual_seed(3)
+    if rules.pop("slopes", False):
+        rules["slopes"] = torch.exp2(-torch.arange(8, device="cuda") * 1.5)
+    if "bias" in rules:
+        rules["distance_bias"] = torch.randn(8, 2 * rules.pop("bias") + 1, generator=g, device="cuda")
+    _check(_q(len(lengths), tokens, 8, 64, torch.float16, 4), _cache(lengths, 8, 32, 64, torch.float8_e4m3fn, 5), **rules)
