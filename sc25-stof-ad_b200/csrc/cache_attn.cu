@@ -402,7 +402,8 @@ __global__ void __launch_bounds__(CT_THREADS, ct_blocks(NT, D)) cache_attn_kerne
             float v_size = 0.f;
 #pragma unroll
             for (int t = 0; t < CT_TILES; ++t) v_size = fabsf(v_scale[t]) <= v_size ? v_size : fabsf(v_scale[t]);    // (a NaN stays)
-            if (!(v_size <= v_ref * 256.f) || v_ref == 0.f) {
+            // (P is at most 2^8, see below: with 2^7 their product stays inside fp16, whose largest number is below 2^16)
+            if (!(v_size <= v_ref * 128.f) || v_ref == 0.f) {
                 const float f = v_size != 0.f ? v_ref / v_size : 1.f;
                 v_ref = v_size != 0.f ? v_size : v_ref;
                 v_ref_inv = v_ref > 0.f ? 1.f / v_ref : 1.f;

@@ -134,3 +134,17 @@ def test_several_steps_under_rules(rules, tokens):
     if "bias" in rules:
         rules["distance_bias"] = torch.randn(8, 2 * rules.pop("bias") + 1, generator=g, device="cuda")
     _check(_q(len(lengths), tokens, 8, 64, torch.float16, 4), _cache(lengths, 8, 32, 64, torch.float8_e4m3fn, 5), **rules)
+
+
+def test_largest_p_beside_largest_scale_stays_in_fp16():
+    """P may be 2^8 before a row's reference moves; V's scale beside it must leave the product inside fp16.  Scores of the last 128 keys are 8
+    units of log2 above those in front, their page's scale is 256 times the other's; entries are 0 here and there."""
+    lengths = [256] * 16
+    assert _steps(lengths, 20, 1, 64) >= 2
+    kp, vp, ks, vs, table, n = _cache(lengths, 20, 128, 64, torch.int8, 11)
+    ks.zero_()
+    vs[table[:, 0].long()] = 1.0 / 64
+    vs[table[:, 1].long()] = 256.0 / 64
+    bias = torch.zeros(20, 2 * 200 + 1, device="cuda")
+    bias[:, 200 - 127:] = 8.0 / 1.4426950408889634 * (1 - 1e-6)
+    _check(_q(16, 1, 20, 64, torch.bfloat16, 12), (kp, vp, ks, vs, table, n), distance_bias=bias)
