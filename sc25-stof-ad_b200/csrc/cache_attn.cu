@@ -4,8 +4,8 @@
 //   S^T (16 keys x 8 rows) = K (16 keys x D) Q^T       O^T (D x 8 rows) += V^T (D x 16 keys) P^T
 // on mma.sync m16n8k16.  A tcgen05 product has at least 64 rows of which a decoding step fills one to eight, and takes its operands
 // from shared memory as 8 or 16 bits; here the entries become fp16 (exactly) on their way from shared memory to registers and are
-// multiplied.  The scales stay out of the products: K's goes into the score, V's into P,
-// relative to a reference that the accumulator carries (so that P keeps fp16's precision whatever the scales are).
+// multiplied.  The scales stay out of the products: K's goes into the score, V's into P, relative to a reference of the row's own
+// that follows the largest p * |scale| it has met: what carries weight keeps fp16's precision, whatever the scales are and in whatever order.
 //
 // Which lane holds which entry is free as long as both operands agree, so that every read is 16 bytes of a row: with g = lane / 4,
 // c = lane % 4, a lane reads chunk c (and c + 4) of the rows of keys g and g + 8 for S, and chunk g of the rows of keys 2c, 2c + 1,
@@ -22,6 +22,8 @@
 #include "cache_common.cuh"
 #include "stof_host.h"
 #include "stof_ptx.cuh"
+
+#include <type_traits>
 
 namespace stof {
 namespace {
@@ -274,12 +276,15 @@ __global__ void __launch_bounds__(CT_THREADS, ct_blocks(NT, D)) cache_attn_kerne
         }
 
         // m: reference of the row's P, 0 as long as it has seen nothing; most: what a score may be above it, minus infinity until then
-        float o[NT][MT][4], m[NT][2], most[NT][2], l[NT][2], v_ref = 0.f, v_ref_inv = 1.f;
+        // (NO_VALUE: it has seen keys, but no values other than 0).  o holds sum(P * scale * v) * c, with c a power of two, 0 until there are
+        // values: the largest |P * scale * c| that has gone into it was 2^-5 at least, and is 2^15 at most.
+        constexpr float NO_VALUE = -1e30f;
+        float o[NT][MT][4], m[NT][2], most[NT][2], l[NT][2], c_row[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             m[nt][0] = m[nt][1] = 0.f;
             most[nt][0] = most[nt][1] = -INFINITY;
-            l[nt][0] = l[nt][1] = 0.f;
+            l[nt][0] = l[nt][1] = c_row[nt][0] = c_row[nt][1] = 0.f;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -398,24 +403,12 @@ __global__ void __launch_bounds__(CT_THREADS, ct_blocks(NT, D)) cache_attn_kerne
                             s[t][nt][e] = on ? x - m[nt][e & 1] : -INFINITY;
                         }
             }
-            // V's scale against the reference that o is held in
-            float v_size = 0.f;
+            // Rows' references move where a score is more than 2^8 above one (P is at most that, then), where the first values come, and where V's
+            // scale leaves P * scale * c more than 2^15
+            float v_size = 0.f, c_most = 0.f;
 #pragma unroll
             for (int t = 0; t < CT_TILES; ++t) v_size = fabsf(v_scale[t]) <= v_size ? v_size : fabsf(v_scale[t]);    // (a NaN stays)
-            // (P is at most 2^8, see below: with 2^7 their product stays inside fp16, whose largest number is below 2^16)
-            if (!(v_size <= v_ref * 128.f) || v_ref == 0.f) {
-                const float f = v_size != 0.f ? v_ref / v_size : 1.f;
-                v_ref = v_size != 0.f ? v_size : v_ref;
-                v_ref_inv = v_ref > 0.f ? 1.f / v_ref : 1.f;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[nt][mt][e] *= f;
-            }
-            // a row's reference follows its maximum when that has grown by more than 2^8 (P is at most that, then)
-            bool grown = false;
+            bool move = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -423,50 +416,100 @@ __global__ void __launch_bounds__(CT_THREADS, ct_blocks(NT, D)) cache_attn_kerne
                     float top = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
 #pragma unroll
                     for (int t = 1; t < CT_TILES; ++t) top = fmaxf(top, fmaxf(s[t][nt][e], s[t][nt][2 + e]));
-                    grown = grown || top > most[nt][e];
+                    move = move || top > most[nt][e];
+                    c_most = fmaxf(c_most, c_row[nt][e]);
                 }
-            if (__any_sync(0xffffffffu, grown)) {
+            bool uneven = false;                             // V's scale * c of some row is large, or none at all
+            if (__any_sync(0xffffffffu, move || !(v_size * c_most <= 128.f))) {
+                // the largest P * |scale| of a row: where the tiles' scales are alike, the largest P's will do
+                float v_log[CT_TILES];
+                bool alike = true;
+#pragma unroll
+                for (int t = 0; t < CT_TILES; ++t) {
+                    alike = alike && fabsf(v_scale[t]) * 16.f >= v_size;
+                    v_log[t] = __log2f(fabsf(v_scale[t]));
+                }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float top = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
+                        float top = -INFINITY, weight = -INFINITY;           // of the row: log2 of the largest P, P * |scale|
 #pragma unroll
-                        for (int t = 1; t < CT_TILES; ++t) top = fmaxf(top, fmaxf(s[t][nt][e], s[t][nt][2 + e]));
+                        for (int t = 0; t < CT_TILES; ++t) {
+                            const float of_tile = fmaxf(s[t][nt][e], s[t][nt][2 + e]);
+                            top = fmaxf(top, of_tile);
+                            weight = fmaxf(weight, of_tile + v_log[t]);
+                        }
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                        if (top > -INFINITY && (top > 0.f || most[nt][e] < 0.f)) {
-                            const float f = most[nt][e] < 0.f ? 0.f : fast_exp2(-top);       // 0: the first that this row sees
-                            m[nt][e] += top;
-                            most[nt][e] = 8.f;
-                            l[nt][e] *= f;
+                        if (alike) {
+                            weight = top + v_log[0];
+                        } else {
 #pragma unroll
-                            for (int mt = 0; mt < MT; ++mt) {
-                                o[nt][mt][e] *= f;
-                                o[nt][mt][2 + e] *= f;
+                            for (int d = 4; d < 32; d <<= 1) weight = fmaxf(weight, __shfl_xor_sync(0xffffffffu, weight, d));
+                        }
+                        if (top > -INFINITY) {
+                            const bool first = most[nt][e] == -INFINITY;
+                            float up = 0.f;
+                            if (first || top > 0.f) {        // by a whole number of powers of two, behind the first
+                                const float to = m[nt][e] + (first ? top : ceilf(top));
+                                up = to - m[nt][e];
+                                m[nt][e] = to;
+                                l[nt][e] *= first ? 0.f : fast_exp2(-up);
+                                weight -= up;
+#pragma unroll
+                                for (int t = 0; t < CT_TILES; ++t) {
+                                    s[t][nt][e] -= up;
+                                    s[t][nt][2 + e] -= up;
+                                }
                             }
+                            const float c_old = c_row[nt][e], log_c = static_cast<float>(static_cast<int>(__float_as_uint(c_old) >> 23) - 127);
+                            // as P shrinks by 2^up c may grow by it, and o stays as it is, unless the new P * |scale| asks for less
+                            float log_to = log_c + rintf(up);
+                            if (c_old == 0.f || weight + log_to > 7.f) log_to = floorf(-weight);
+                            log_to = fminf(fmaxf(log_to, -126.f), 126.f);
+                            most[nt][e] = 8.f;
+                            if (c_old == 0.f && weight == -INFINITY) {
+                                most[nt][e] = NO_VALUE;
+                            } else {
+                                c_row[nt][e] = __uint_as_float(static_cast<uint32_t>(127 + static_cast<int>(log_to)) << 23);
+                                const float f = c_old == 0.f ? 0.f : fast_exp2(log_to - log_c - up);
+                                if (f != 1.f) {
 #pragma unroll
-                            for (int t = 0; t < CT_TILES; ++t) {
-                                s[t][nt][e] -= top;
-                                s[t][nt][2 + e] -= top;
+                                    for (int mt = 0; mt < MT; ++mt) {
+                                        o[nt][mt][e] *= f;
+                                        o[nt][mt][2 + e] *= f;
+                                    }
+                                }
                             }
                         }
+                        uneven = uneven || !(v_size * c_row[nt][e] <= 128.f);
                     }
+                uneven = __any_sync(0xffffffffu, uneven);
             }
             uint32_t pf[CT_TILES][NT][2];
+            // `masked`: p * scale where p is not 0 (zero times infinity or NaN for a row that sees nothing of the tile)
+            auto weights = [&](auto masked) {
 #pragma unroll
-            for (int t = 0; t < CT_TILES; ++t) {
-                const float v_rel = v_scale[t] * v_ref_inv;
+                for (int t = 0; t < CT_TILES; ++t)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const float p0 = fast_exp2(s[t][nt][0]), p1 = fast_exp2(s[t][nt][1]), p2 = fast_exp2(s[t][nt][2]), p3 = fast_exp2(s[t][nt][3]);
-                    l[nt][0] += p0 + p2;
-                    l[nt][1] += p1 + p3;
-                    // to fp16 for the product, as the other attention kernels do; the sum is of the values before rounding
-                    pf[t][nt][0] = transpose8x8(pack_half2(p0 * v_rel, p1 * v_rel));
-                    pf[t][nt][1] = transpose8x8(pack_half2(p2 * v_rel, p3 * v_rel));
-                }
-            }
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float x[4], w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            x[e] = fast_exp2(s[t][nt][e]);
+                            w[e] = x[e] * (v_scale[t] * c_row[nt][e & 1]);
+                            if constexpr (decltype(masked)::value) w[e] = x[e] == 0.f ? 0.f : w[e];
+                        }
+                        l[nt][0] += x[0] + x[2];
+                        l[nt][1] += x[1] + x[3];
+                        // to fp16 for the product, as the other attention kernels do; the sum is of the values before rounding
+                        pf[t][nt][0] = transpose8x8(pack_half2(w[0], w[1]));
+                        pf[t][nt][1] = transpose8x8(pack_half2(w[2], w[3]));
+                    }
+            };
+            if (__builtin_expect(uneven, 0)) weights(std::true_type());
+            else weights(std::false_type());
 #pragma unroll
             for (int t = 0; t < CT_TILES; ++t) {
                 uint4 v[4];                                  // keys 2c, 2c + 1, 2c + 8, 2c + 9 (D = 64: the first half)
@@ -519,7 +562,7 @@ __global__ void __launch_bounds__(CT_THREADS, ct_blocks(NT, D)) cache_attn_kerne
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                if (most[nt][e] < 0.f) m[nt][e] = -INFINITY;
+                if (most[nt][e] == -INFINITY) m[nt][e] = -INFINITY;
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], d);
                 if (g == 0) {
@@ -538,7 +581,7 @@ __global__ void __launch_bounds__(CT_THREADS, ct_blocks(NT, D)) cache_attn_kerne
 #pragma unroll
                 for (int w = 1; w < CT_WARPS; ++w) top = fmaxf(top, merge_m[w][r]);
                 // a row without a maximum saw nothing (sum 0) or only NaN (sum NaN, which has to come out)
-                weight[nt][e] = m[nt][e] == -INFINITY ? l[nt][e] : fast_exp2(m[nt][e] - top) * v_ref;
+                weight[nt][e] = m[nt][e] == -INFINITY ? l[nt][e] : fast_exp2(m[nt][e] - top) * (c_row[nt][e] > 0.f ? 1.f / c_row[nt][e] : 1.f);
             }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)

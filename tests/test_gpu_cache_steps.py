@@ -148,3 +148,75 @@ def test_largest_p_beside_largest_scale_stays_in_fp16():
     bias = torch.zeros(20, 2 * 200 + 1, device="cuda")
     bias[:, 200 - 127:] = 8.0 / 1.4426950408889634 * (1 - 1e-6)
     _check(_q(16, 1, 20, 64, torch.bfloat16, 12), (kp, vp, ks, vs, table, n), distance_bias=bias)
+
+
+@pytest.mark.parametrize("ratio", [12, 18, 24, 40, 100])
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_a_large_scale_without_weight_takes_no_digits(ratio, tokens):
+    """The first pages' V scales are 2^ratio times the others', their scores e^-120 of them: what carries weight keeps its digits."""
+    lengths = [768] * 16
+    assert _steps(lengths, 8, tokens, 64) >= 2
+    kp, vp, ks, vs, table, n = _cache(lengths, 8, 16, 64, torch.int8, 13)
+    vs[table[:, :9].long()] = 2.0 ** (ratio - 5)
+    bias = torch.zeros(8, 2 * 600 + 1, device="cuda")
+    bias[:, 0] = -120.0
+    _check(_q(16, tokens, 8, 64, torch.bfloat16, 14), (kp, vp, ks, vs, table, n), distance_bias=bias)
+
+
+@pytest.mark.parametrize("dim,heads,tokens,entry", [(64, 8, 1, torch.int8), (64, 16, 3, torch.float8_e4m3fn), (128, 16, 1, torch.float8_e4m3fn), (128, 32, 5, torch.int8)])
+@pytest.mark.parametrize("spread", [4, 20, 60])
+def test_scales_of_any_size_in_any_order(dim, heads, tokens, entry, spread):
+    """V scales of 2^-spread to 2^spread, rising, falling and mixed, zeros among them, and scores that favour small scales, large ones or none."""
+    lengths = [4000, 1, 900, 0, 2049, 3333, 5000, 4224]
+    assert _steps(lengths, 8, tokens * heads // 8, dim) >= 2
+    kp, vp, ks, vs, table, n = _cache(lengths, 8, 32, dim, entry, 15)
+    width = table.shape[1]
+    size = torch.linspace(-1, 1, width, device="cuda")
+    q = _q(8, tokens, heads, dim, torch.bfloat16, 16)
+    for order in (size, -size, torch.rand(width, device="cuda", generator=torch.Generator(device="cuda").manual_seed(17)) * 2 - 1):
+        by_page = torch.zeros(vs.shape[0], device="cuda")
+        for b, length in enumerate(lengths):
+            blocks = -(-length // 32)
+            by_page[table[b, :blocks].long()] = order[:blocks]
+        scales = torch.exp2(by_page * spread)[:, None].expand_as(vs).contiguous()
+        scales[::7] = 0.0
+        for slope in (0.0, 0.05):
+            _check(q, (kp, vp, ks, scales / 64, table, n), slopes=torch.full((heads,), slope, device="cuda"))
+
+
+def test_pages_of_scale_zero_in_front():
+    """Rows that have seen keys but no values yet."""
+    lengths = [768] * 16
+    kp, vp, ks, vs, table, n = _cache(lengths, 8, 16, 64, torch.int8, 18)
+    for scale in (2.0 ** -100, 2.0 ** -20, 1.0, 2.0 ** 90):
+        vs[table[:, :20].long()] = 0.0
+        vs[table[:, 20:].long()] = scale
+        _check(_q(16, 1, 8, 64, torch.bfloat16, 19), (kp, vp, ks, vs, table, n))
+        vs[table.long()] = 0.0
+        assert not _check(_q(16, 1, 8, 64, torch.bfloat16, 19), (kp, vp, ks, vs, table, n)).any()
+
+
+def test_nan_and_infinite_scales_reach_who_sees_them():
+    import stof_b200
+    lengths = [768] * 16
+    kp, vp, ks, vs, table, n = _cache(lengths, 8, 16, 64, torch.int8, 20)
+    q = _q(16, 3, 8, 64, torch.float16, 21)
+    clean = stof_b200.cache_attention(q, kp, vp, ks, vs, table, n)
+    for bad in (math.nan, math.inf):
+        for scales in (ks, vs):
+            broken = scales.clone()
+            broken[table[3, 7].long(), 5] = bad
+            args = (kp, vp, broken, vs, table, n) if scales is ks else (kp, vp, ks, broken, table, n)
+            got = stof_b200.cache_attention(q, *args)
+            _status()
+            assert not bool(torch.isfinite(got[3, :, 5]).any())
+            got[3, :, 5] = clean[3, :, 5]
+            assert torch.equal(got, clean)
+    # a page that begins behind the first of three tokens: that token does not see its scale
+    kp, vp, ks, vs, table, n = _cache([50] * 8, 2, 16, 64, torch.int8, 22)
+    q = _q(8, 3, 2, 64, torch.float16, 23)
+    clean = stof_b200.cache_attention(q, kp, vp, ks, vs, table, n)
+    vs[table[:, 3].long()] = math.nan
+    got = stof_b200.cache_attention(q, kp, vp, ks, vs, table, n)
+    _status()
+    assert torch.equal(got[:, 0], clean[:, 0]) and not bool(torch.isfinite(got[:, 1:]).any())
