@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(CT_THREADS, ct_blocks(NT, D)) cache_attn_kerne
         // m: reference of the row's P, 0 as long as it has seen nothing; most: what a score may be above it, minus infinity until then
         // (NO_VALUE: it has seen keys, but no values other than 0).  o holds sum(P * scale * v) * c, with c a power of two, 0 until there are
         // values: the largest |P * scale * c| that has gone into it was 2^-5 at least, and is 2^15 at most.
-        constexpr float NO_VALUE = -1e30f;
+        constexpr float NO_VALUE = -1e30f, FAR = 320.f;      // (2^254 is the largest ratio of two scales)
         float o[NT][MT][4], m[NT][2], most[NT][2], l[NT][2], c_row[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -310,99 +310,102 @@ __global__ void __launch_bounds__(CT_THREADS, ct_blocks(NT, D)) cache_attn_kerne
             }
             if (!any) return;
             float s[CT_TILES][NT][4];
-#pragma unroll
-            for (int t = 0; t < CT_TILES; ++t)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[t][nt][e] = 0.f;
-#pragma unroll
-            for (int i = 0; i < CH; ++i) {
-                uint4 x[CT_TILES], y[CT_TILES];
-#pragma unroll
-                for (int t = 0; t < CT_TILES; ++t) {
-                    x[t] = *reinterpret_cast<const uint4*>(tiles + t * R::TILE + R::k_at(g, c + 4 * i));
-                    y[t] = *reinterpret_cast<const uint4*>(tiles + t * R::TILE + R::k_at(g + 8, c + 4 * i));
-                }
-#pragma unroll
-                for (int w = 0; w < 4; ++w)
-#pragma unroll
-                    for (int t = 0; t < CT_TILES; ++t) {
-                        uint32_t a0, a1, a2, a3;
-                        entries_to_half<E4M3>(word(x[t], w), a0, a2);
-                        entries_to_half<E4M3>(word(y[t], w), a1, a3);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma16816(s[t][nt], a0, a1, a2, a3, qf[nt][4 * i + w][0], qf[nt][4 * i + w][1]);
-                    }
-            }
-            // scores in units of log2, less the row's reference; element e: key g + 8 * (e / 2), row 2c + e % 2
-            if (p.softcap > 0.f) {
-                const float to = 1.f / (p.softcap * LOG2E), from = p.softcap * LOG2E;
-                float top = 0.f;                             // of |score / softcap|
+            auto scores = [&] {                              // of the step's keys
 #pragma unroll
                 for (int t = 0; t < CT_TILES; ++t)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            s[t][nt][e] *= k_scale[t] * row_scale[nt][e & 1] * to;
-                            top = fmaxf(top, fabsf(s[t][nt][e]));
+                        for (int e = 0; e < 4; ++e) s[t][nt][e] = 0.f;
+#pragma unroll
+                for (int i = 0; i < CH; ++i) {
+                    uint4 x[CT_TILES], y[CT_TILES];
+#pragma unroll
+                    for (int t = 0; t < CT_TILES; ++t) {
+                        x[t] = *reinterpret_cast<const uint4*>(tiles + t * R::TILE + R::k_at(g, c + 4 * i));
+                        y[t] = *reinterpret_cast<const uint4*>(tiles + t * R::TILE + R::k_at(g + 8, c + 4 * i));
+                    }
+#pragma unroll
+                    for (int w = 0; w < 4; ++w)
+#pragma unroll
+                        for (int t = 0; t < CT_TILES; ++t) {
+                            uint32_t a0, a1, a2, a3;
+                            entries_to_half<E4M3>(word(x[t], w), a0, a2);
+                            entries_to_half<E4M3>(word(y[t], w), a1, a3);
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) mma16816(s[t][nt], a0, a1, a2, a3, qf[nt][4 * i + w][0], qf[nt][4 * i + w][1]);
                         }
-                if (__all_sync(0xffffffffu, top <= 0.35f)) {
-                    // an odd polynomial, off by 2.9e-6 of the value at most (weighted least squares moved towards the minimax one)
+                }
+                // in units of log2, less the row's reference; element e: key g + 8 * (e / 2), row 2c + e % 2
+                if (p.softcap > 0.f) {
+                    const float to = 1.f / (p.softcap * LOG2E), from = p.softcap * LOG2E;
+                    float top = 0.f;                             // of |score / softcap|
 #pragma unroll
                     for (int t = 0; t < CT_TILES; ++t)
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                const float u = s[t][nt][e], w = u * u;
-                                s[t][nt][e] = u * from * fmaf(w, fmaf(w, 0.1239503026008606f, -0.33290955424308777f), 0.9999971389770508f);
+                                s[t][nt][e] *= k_scale[t] * row_scale[nt][e & 1] * to;
+                                top = fmaxf(top, fabsf(s[t][nt][e]));
                             }
+                    if (__all_sync(0xffffffffu, top <= 0.35f)) {
+                        // an odd polynomial, off by 2.9e-6 of the value at most (weighted least squares moved towards the minimax one)
+#pragma unroll
+                        for (int t = 0; t < CT_TILES; ++t)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const float u = s[t][nt][e], w = u * u;
+                                    s[t][nt][e] = u * from * fmaf(w, fmaf(w, 0.1239503026008606f, -0.33290955424308777f), 0.9999971389770508f);
+                                }
+                    } else {
+                        // tanh(u) = 1 - 2 / (1 + e^(2u)): off by 1e-7
+#pragma unroll
+                        for (int t = 0; t < CT_TILES; ++t)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) s[t][nt][e] = fmaf(-2.f * from, fast_reciprocal(1.f + fast_exp2(s[t][nt][e] * (2.f * LOG2E))), from);
+                    }
                 } else {
-                    // tanh(u) = 1 - 2 / (1 + e^(2u)): off by 1e-7
 #pragma unroll
                     for (int t = 0; t < CT_TILES; ++t)
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) s[t][nt][e] = fmaf(-2.f * from, fast_reciprocal(1.f + fast_exp2(s[t][nt][e] * (2.f * LOG2E))), from);
+                            for (int e = 0; e < 4; ++e) s[t][nt][e] *= k_scale[t] * row_scale[nt][e & 1];
                 }
-            } else {
-#pragma unroll
-                for (int t = 0; t < CT_TILES; ++t)
+                if (key >= see_from && key + CT_STEP - 1 <= see_to && left[0] > 0 && left[CT_TILES - 1] > 0) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) s[t][nt][e] *= k_scale[t] * row_scale[nt][e & 1];
-            }
-            if (key >= see_from && key + CT_STEP - 1 <= see_to && left[0] > 0 && left[CT_TILES - 1] > 0) {
+                        for (int e = 0; e < 2; ++e) {
+                            const float away = static_cast<float>(key + g - pos[nt][e]), less = fmaf(slope[nt][e], away, -m[nt][e]);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float away = static_cast<float>(key + g - pos[nt][e]), less = fmaf(slope[nt][e], away, -m[nt][e]);
-#pragma unroll
-                        for (int t = 0; t < CT_TILES; ++t) {
-                            s[t][nt][e] += fmaf(slope[nt][e], static_cast<float>(16 * t), less);
-                            s[t][nt][2 + e] += fmaf(slope[nt][e], static_cast<float>(16 * t + 8), less);
+                            for (int t = 0; t < CT_TILES; ++t) {
+                                s[t][nt][e] += fmaf(slope[nt][e], static_cast<float>(16 * t), less);
+                                s[t][nt][2 + e] += fmaf(slope[nt][e], static_cast<float>(16 * t + 8), less);
+                            }
                         }
-                    }
-            } else {
+                } else {
 #pragma unroll
-                for (int t = 0; t < CT_TILES; ++t)
+                    for (int t = 0; t < CT_TILES; ++t)
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float x = s[t][nt][e];
-                            const int away = key + 16 * t + g + 8 * (e >> 1) - pos[nt][e & 1];   // at most 0 where visible
-                            x += slope[nt][e & 1] * static_cast<float>(away);
-                            const bool on = left[t] > 0 && pos[nt][e & 1] >= 0 && away <= 0 && (p.window == 0 || away > -p.window);
-                            if (p.distance_bias != nullptr && on) x += __ldca(table[nt][e & 1] + max(away, -p.radius)) * LOG2E;
-                            s[t][nt][e] = on ? x - m[nt][e & 1] : -INFINITY;
-                        }
-            }
+                            for (int e = 0; e < 4; ++e) {
+                                float x = s[t][nt][e];
+                                const int away = key + 16 * t + g + 8 * (e >> 1) - pos[nt][e & 1];   // at most 0 where visible
+                                x += slope[nt][e & 1] * static_cast<float>(away);
+                                const bool on = left[t] > 0 && pos[nt][e & 1] >= 0 && away <= 0 && (p.window == 0 || away > -p.window);
+                                if (p.distance_bias != nullptr && on) x += __ldca(table[nt][e & 1] + max(away, -p.radius)) * LOG2E;
+                                s[t][nt][e] = on ? x - m[nt][e & 1] : -INFINITY;
+                            }
+                }
+            };
+            scores();
             // Rows' references move where a score is more than 2^8 above one (P is at most that, then), where the first values come, and where V's
             // scale leaves P * scale * c more than 2^15
             float v_size = 0.f, c_most = 0.f;
@@ -421,6 +424,44 @@ __global__ void __launch_bounds__(CT_THREADS, ct_blocks(NT, D)) cache_attn_kerne
                 }
             bool uneven = false;                             // V's scale * c of some row is large, or none at all
             if (__any_sync(0xffffffffu, move || !(v_size * c_most <= 128.f))) {
+                float tops[NT][2];
+                auto largest = [&] {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            tops[nt][e] = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
+#pragma unroll
+                            for (int t = 1; t < CT_TILES; ++t) tops[nt][e] = fmaxf(tops[nt][e], fmaxf(s[t][nt][e], s[t][nt][2 + e]));
+#pragma unroll
+                            for (int d = 4; d < 32; d <<= 1) tops[nt][e] = fmaxf(tops[nt][e], __shfl_xor_sync(0xffffffffu, tops[nt][e], d));
+                        }
+                };
+                largest();
+                // A score so far above the reference has lost digits to it, and nothing that came before has weight beside it (no ratio of
+                // scales makes up for it): the row begins anew, from scores less nothing
+                bool anew = false;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) anew = anew || (tops[nt][0] > FAR && most[nt][0] > -INFINITY) || (tops[nt][1] > FAR && most[nt][1] > -INFINITY);
+                if (__builtin_expect(__any_sync(0xffffffffu, anew), 0)) {
+                    asm volatile("" ::: "memory");           // (the step's keys are read again, not kept)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (tops[nt][e] > FAR && most[nt][e] > -INFINITY) {
+                                m[nt][e] = c_row[nt][e] = 0.f;
+                                most[nt][e] = -INFINITY;
+                                l[nt][e] *= 0.f;             // (a NaN stays)
+#pragma unroll
+                                for (int mt = 0; mt < MT; ++mt) {
+                                    o[nt][mt][e] *= 0.f;
+                                    o[nt][mt][2 + e] *= 0.f;
+                                }
+                            }
+                    scores();
+                    largest();
+                }
                 // the largest P * |scale| of a row: where the tiles' scales are alike, the largest P's will do
                 float v_log[CT_TILES];
                 bool alike = true;
@@ -433,18 +474,12 @@ __global__ void __launch_bounds__(CT_THREADS, ct_blocks(NT, D)) cache_attn_kerne
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float top = -INFINITY, weight = -INFINITY;           // of the row: log2 of the largest P, P * |scale|
+                        const float top = tops[nt][e];       // log2 of the row's largest P; and P * |scale|
+                        float weight = top + v_log[0];
+                        if (!alike) {
+                            weight = -INFINITY;
 #pragma unroll
-                        for (int t = 0; t < CT_TILES; ++t) {
-                            const float of_tile = fmaxf(s[t][nt][e], s[t][nt][2 + e]);
-                            top = fmaxf(top, of_tile);
-                            weight = fmaxf(weight, of_tile + v_log[t]);
-                        }
-#pragma unroll
-                        for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                        if (alike) {
-                            weight = top + v_log[0];
-                        } else {
+                            for (int t = 0; t < CT_TILES; ++t) weight = fmaxf(weight, fmaxf(s[t][nt][e], s[t][nt][2 + e]) + v_log[t]);
 #pragma unroll
                             for (int d = 4; d < 32; d <<= 1) weight = fmaxf(weight, __shfl_xor_sync(0xffffffffu, weight, d));
                         }

@@ -220,3 +220,27 @@ def test_nan_and_infinite_scales_reach_who_sees_them():
     got = stof_b200.cache_attention(q, kp, vp, ks, vs, table, n)
     _status()
     assert torch.equal(got[:, 0], clean[:, 0]) and not bool(torch.isfinite(got[:, 1:]).any())
+
+
+@pytest.mark.parametrize("low", [-1e4, -1e9, -1e30, -3e38])
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_scores_far_below_the_first_ones_lose_nothing(low, tokens):
+    """A table that masks far keys by a low value: the reference that the first steps leave must not take the digits of the later scores."""
+    lengths = [768] * 16
+    assert _steps(lengths, 8, tokens, 64) >= 2
+    cache = _cache(lengths, 8, 16, 64, torch.int8, 24)
+    bias = torch.randn(8, 2 * 600 + 1, device="cuda")
+    for reach in (600, 350, 40):                         # keys at this distance and beyond
+        bias[:, :601 - reach] = low
+        _check(_q(16, tokens, 8, 64, torch.float16, 25), cache, distance_bias=bias)
+
+
+def test_first_pages_of_huge_scores():
+    """The same by K's scales: scores of the first pages at -1e5 and below, of those behind them near zero."""
+    lengths = [768] * 16
+    kp, vp, ks, vs, table, n = _cache(lengths, 8, 16, 64, torch.int8, 26)
+    q = _q(16, 1, 8, 64, torch.float16, 27).abs() + 0.5
+    kp[table[:, :11].long()] = -100
+    for big in (1e2, 1e6):
+        ks[table[:, :11].long()] = big
+        _check(q, (kp, vp, ks, vs, table, n))
