@@ -782,7 +782,9 @@ int launch(const CacheAttnParams& p, const Shape& s, cudaStream_t stream) {
 using namespace stof;
 
 extern "C" size_t stof_cache_attn_workspace_bytes(int requests, int tokens, int heads, int kv_heads, int head_dim, int page_size, int table_width) {
-    if (requests <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || page_size <= 0 || table_width < 0) return 0;
+    if (requests <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || page_size <= 0 || table_width < 0 ||
+        static_cast<long long>(tokens) * (heads / kv_heads) > (1ll << 30))
+        return 0;
     const Shape s = shape_of(requests, tokens, heads, kv_heads, head_dim, page_size, table_width);
     return (static_cast<size_t>(s.joins) * sizeof(int2) + 15) / 16 * 16 + static_cast<size_t>(s.blocks) * (8 * s.nt) * (static_cast<size_t>(head_dim) + 2) * sizeof(float);
 }
@@ -799,6 +801,7 @@ extern "C" int stof_cache_attn(const void* q, void* out, int dtype, const long l
     STOF_REQUIRE(cache_dtype == STOF_DTYPE_INT8 || cache_dtype == STOF_DTYPE_E4M3, "cache_attn: cache entries must be int8 or e4m3");
     STOF_REQUIRE(dtype == STOF_DTYPE_F16 || dtype == STOF_DTYPE_BF16, "cache_attn: queries must be fp16 or bf16");
     STOF_REQUIRE(static_cast<long long>(table_width) * page_size <= (1ll << 30), "cache_attn: a row of the block table spans more than 2^30 tokens");
+    STOF_REQUIRE(static_cast<long long>(tokens) * (heads / kv_heads) <= (1ll << 30), "cache_attn: more than 2^30 query rows of a K/V head");
     STOF_REQUIRE(rules != nullptr, "cache_attn: null rules");
     STOF_REQUIRE(rules->softmax_scale > 0.f && rules->softmax_scale < INFINITY, "cache_attn: softmax_scale must be positive and finite");
     STOF_REQUIRE(rules->softcap >= 0.f && rules->softcap < INFINITY, "cache_attn: softcap must not be negative");
@@ -830,7 +833,9 @@ extern "C" int stof_cache_attn(const void* q, void* out, int dtype, const long l
     p.slopes = rules->slopes; p.distance_bias = rules->distance_bias; p.radius = rules->bias_radius;
     p.parts = static_cast<int2*>(workspace);
     p.workspace = reinterpret_cast<float*>(static_cast<char*>(workspace) + (static_cast<size_t>(s.joins) * sizeof(int2) + 15) / 16 * 16); p.status = status_dev;
-    p.scale = rules->softmax_scale; p.softcap = usable_cap(rules->softcap); p.window = rules->window;
+    p.scale = rules->softmax_scale; p.softcap = usable_cap(rules->softcap);
+    // (a window as long as a request may be hides nothing; below that, positions less it stay inside 32 bits)
+    p.window = rules->window >= static_cast<long long>(table_width) * page_size ? 0 : rules->window;
     p.requests = requests; p.tokens = tokens; p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads;
     p.rows = s.rows; p.row_groups = s.row_groups; p.resident = s.resident;
     p.table_width = table_width; p.page_count = pages; p.bf16 = dtype == STOF_DTYPE_BF16;

@@ -244,3 +244,31 @@ def test_first_pages_of_huge_scores():
     for big in (1e2, 1e6):
         ks[table[:, :11].long()] = big
         _check(q, (kp, vp, ks, vs, table, n))
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 30, 4097, 4096, 4095])
+@pytest.mark.parametrize("tokens", [1, 5])
+def test_windows_longer_than_any_request_at_the_c_entry(window, tokens):
+    """Requests of nothing, shorter than the new tokens and long, whatever the window is taken from."""
+    import ctypes
+
+    from stof_b200 import _lib
+    lengths = [0, 1, 4000, 2, 4096, 300]
+    q, cache = _q(6, tokens, 4, 64, torch.float16, 28), _cache(lengths, 2, 32, 64, torch.int8, 29)
+    want = _check(q, cache)
+    kp, vp, ks, vs, table, n = cache
+    assert table.shape[1] * 32 == 4096
+    L, out = _lib.lib(), torch.full_like(q, 7.0)
+    rules = _lib.ScoreRules(softmax_scale=0.125, window=window)
+    st = _lib.strides3(q.stride()[:3])
+    size = L.stof_cache_attn_workspace_bytes(6, tokens, 4, 2, 64, 32, 128)
+    space = torch.empty(size, dtype=torch.uint8, device="cuda")
+    at = lambda t: ctypes.c_void_p(t.data_ptr())
+    rc = L.stof_cache_attn(at(q), at(out), _lib.STOF_DTYPE_F16, st, st, at(kp), at(vp), at(ks), at(vs), _lib.STOF_DTYPE_INT8, kp.shape[0], 32, 2, 64, at(table), 128, 128,
+                           at(n), 6, tokens, 4, ctypes.byref(rules), at(space), size, at(_lib.status_word(torch.device("cuda"))), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+    assert rc == 0, L.stof_last_error()
+    _status()
+    if window >= 4096:
+        assert torch.equal(out, want)
+    else:
+        assert torch.equal(out, _check(q, cache, window=window))

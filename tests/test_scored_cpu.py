@@ -159,3 +159,8 @@ def test_restated_page_tables():
     assert missing == 0 and starts == [0, 1, 1, 41] and count == 0
     assert table[0][:2] == [5, 3] and table[2] == [2, 8, 7]
     assert slots[:2] == [3 * 16, 2 * 16] and slots[41:] == [-1, -1]
+
+
+def test_cache_attn_refuses_rows_beyond_32_bits(lib):
+    assert _cache(lib, heads=64, kv_heads=1, tokens=(1 << 24) + 1) == -1 and b"2^30" in lib.stof_last_error()
+    assert lib.stof_cache_attn_workspace_bytes(1, (1 << 24) + 1, 64, 1, 64, 16, 4) == 0
