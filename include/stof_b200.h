@@ -298,7 +298,8 @@ int stof_scored_attn(const void* q, const void* k, const void* v, void* out, int
  * request b sits at position lengths[b] - tokens + t; keys behind a token's position are not visible to it, nor, with
  * window > 0, those window or more in front of it.  softcap, slopes, distance_bias as above (causal, documents, prefix_lens and
  * key_lens of `rules` are not read).  lengths int32 (requests), counted to at most table_width * page_size; requests of length
- * 0 give zeros.  A page number outside [0, pages) is reported through status_dev and its keys are left out.
+ * 0 give zeros.  A page number outside [0, pages) is reported through status_dev and its keys are left out.  Behind a request's
+ * length, and for pages that a window hides from all of its tokens, the table may hold anything.
  * Work is dealt evenly over the GPU whatever the lengths; what a thread block computes of a request's head goes to `workspace`
  * (stof_cache_attn_workspace_bytes bytes, 16-byte aligned, not shared with a call that may run at the same time) where it is not
  * all of it, and a second kernel joins the parts in a fixed order.

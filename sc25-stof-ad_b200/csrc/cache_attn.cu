@@ -173,6 +173,8 @@ __global__ void __launch_bounds__(CT_THREADS, ct_blocks(NT, D)) cache_attn_kerne
     {
         const int* pages = p.block_table + b * p.table_stride;
         const int last_key = min(span.length, span.first + u1 * CT_UNIT);
+        // tiles that end in front of what the first token sees (a unit may begin with some) are not there: their pages may be anybody's
+        const int seen_from = p.window > 0 ? span.length - p.tokens - p.window + 1 : 0;
         struct Pages { int of[CT_TILES]; };
         auto pages_of = [&](int key) {                       // of the tiles from this key on; -1 behind the last
             Pages r;
@@ -185,7 +187,7 @@ __global__ void __launch_bounds__(CT_THREADS, ct_blocks(NT, D)) cache_attn_kerne
 #pragma unroll
             for (int i = 0; i < CT_TILES; ++i) {
                 const int offset = stage * R::STAGE + i * R::TILE;
-                const bool there = key + 16 * i < last_key, good = there && static_cast<unsigned>(page.of[i]) < static_cast<unsigned>(p.page_count);
+                const bool there = key + 16 * i < last_key && key + 16 * i + 15 >= seen_from, good = there && static_cast<unsigned>(page.of[i]) < static_cast<unsigned>(p.page_count);
                 if (lane == 0) {
                     *reinterpret_cast<int*>(ring + offset + 2 * R::SIDE + 8) = good;
                     if (there && !good && p.status != nullptr) atomicCAS(p.status, 0, STATUS_BAD_INDEX);

@@ -33,7 +33,8 @@ def cache_attention(q, k_pages, v_pages, k_scales, v_scales, block_table, length
     stands for entry * scale.  Key j of request b lies in page block_table[b, j // page_size] (int32), row j % page_size.  Token t sits
     at position lengths[b] - n + t (`lengths` int32, the new tokens included) and sees what is not behind it and, with `window`, less
     than `window` away.  `softcap`, `slopes`, `distance_bias` and `softmax_scale` as for `scored_attention`.  Requests of length 0, and tokens at
-    negative positions, give zeros.  A page number outside the cache is reported through the status word and its keys are left out."""
+    negative positions, give zeros.  A page number outside the cache is reported through the status word and its keys are left out; the
+    table may hold anything behind a request's length and for pages that the window hides from all of its tokens."""
     return (_lib._native or _lib.native()).cache_attention(q, k_pages, v_pages, k_scales, v_scales, block_table, lengths, out, window, softcap, slopes,
                                                            distance_bias, softmax_scale)
 

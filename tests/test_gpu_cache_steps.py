@@ -272,3 +272,29 @@ def test_windows_longer_than_any_request_at_the_c_entry(window, tokens):
         assert torch.equal(out, want)
     else:
         assert torch.equal(out, _check(q, cache, window=window))
+
+
+@pytest.mark.parametrize("tokens", [1, 4])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("window", [1, 17, 100, 700])
+def test_pages_in_front_of_the_window_may_be_anything(tokens, page, window):
+    """Given back and marked, or somebody else's by now, with scales and entries of any kind."""
+    lengths = [3000, 129, 128, 1000, 5, 2047]
+    q = _q(6, tokens, 4, 64, torch.float16, 30)
+    kp, vp, ks, vs, table, n = _cache(lengths, 2, page, 64, torch.float8_e4m3fn, 31)
+    want = _check(q, (kp, vp, ks, vs, table, n), window=window)
+    marked, other = table.clone(), table.clone()
+    # a page of NaN under scales of NaN
+    spare = [i for i in range(kp.shape[0]) if i not in set(table.flatten().tolist())]
+    for x in (kp, vp):
+        x.view(torch.uint8)[spare[0]] = 0x7F
+    for x in (ks, vs):
+        x[spare[0]] = math.nan
+    for b, length in enumerate(lengths):
+        hidden = max(length - tokens - window + 1, 0) // page
+        marked[b, :hidden], other[b, :hidden] = -1, spare[0]
+    import stof_b200
+    for t in (marked, other):
+        got = stof_b200.cache_attention(q, kp, vp, ks, vs, t, n, window=window)
+        _status()
+        assert torch.equal(got, want)
