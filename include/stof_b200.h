@@ -321,7 +321,8 @@ int stof_cache_attn(const void* q, void* out, int dtype, const long long q_strid
  * begins its page sets the page's scale to its largest magnitude / 127 (int8) or / 448 (e4m3), per head, and what the page held
  * counts no more; any other run keeps the larger of that and the scale that is there, and where the scale grows the
  * entries in front of the run are rounded again to it.  entry = round(x * (1 / scale)), to nearest even; a scale below the
- * smallest normal fp32 counts as 0.  A page may hold one run of a call only: two runs in the same page write it unordered.
+ * smallest normal fp32 counts as 0.  An infinity makes its page's scale infinite; a NaN makes its page's scale NaN (int8; until a
+ * run begins the page again) or its own entry (e4m3).  A page may hold one run of a call only: two runs in the same page write it unordered.
  * Slots at or behind pages * page_size are reported through status_dev and not written.
  * ------------------------------------------------------------------------------------------ */
 int stof_cache_append(void* k_pages, void* v_pages, float* k_scales, float* v_scales, int cache_dtype,

@@ -35,12 +35,19 @@ struct Rows {
     static constexpr int LANES = D / 8;                      // lanes that share a row, 16 bytes each
     static constexpr int EACH = 32 / LANES;                  // rows of one warp-wide load
 
+    // An e4m3 entry can be NaN itself, an int8 one cannot: there a NaN goes into the page's scale, so that it comes out of what reads the page
+    static __device__ __forceinline__ float larger(float a, float b) {
+        if constexpr (E4M3) return fmaxf(a, b);
+        float c;
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+        return c;
+    }
     static __device__ __forceinline__ float magnitude(const uint4& u) {
         auto pair = [](uint32_t w) {
             const float2 f = unpack_pair<BF16>(w);
-            return fmaxf(fabsf(f.x), fabsf(f.y));
+            return larger(fabsf(f.x), fabsf(f.y));
         };
-        return fmaxf(fmaxf(pair(u.x), pair(u.y)), fmaxf(pair(u.z), pair(u.w)));
+        return larger(larger(pair(u.x), pair(u.y)), larger(pair(u.z), pair(u.w)));
     }
     static __device__ __forceinline__ uint2 entries(const uint4& u, float inv) {
         return make_uint2(quantise4<E4M3>(unpack_pair<BF16>(u.x), unpack_pair<BF16>(u.y), inv), quantise4<E4M3>(unpack_pair<BF16>(u.z), unpack_pair<BF16>(u.w), inv));
@@ -79,22 +86,22 @@ __device__ __forceinline__ void write_run(const AppendParams& p, int head, int t
 #pragma unroll
         for (int side = 0; side < 2; ++side)
 #pragma unroll
-            for (int i = 0; i < NV; ++i) top[side] = fmaxf(top[side], R::magnitude(v[side][i]));
+            for (int i = 0; i < NV; ++i) top[side] = R::larger(top[side], R::magnitude(v[side][i]));
         if (from + pass >= n) break;
         from += pass;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
-        top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], o));
+        top[0] = R::larger(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
+        top[1] = R::larger(top[1], __shfl_xor_sync(0xffffffffu, top[1], o));
     }
     if (parts > 1) {
         if (lane < 2) shared[part][lane] = lane == 0 ? top[0] : top[1];
         __syncthreads();                                     // (and everyone has read the old scales)
 #pragma unroll
         for (int w = 0; w < CA_WARPS; ++w) {
-            top[0] = fmaxf(top[0], shared[w][0]);
-            top[1] = fmaxf(top[1], shared[w][1]);
+            top[0] = R::larger(top[0], shared[w][0]);
+            top[1] = R::larger(top[1], shared[w][1]);
         }
     }
     float inv[2], ratio[2];
@@ -102,7 +109,7 @@ __device__ __forceinline__ void write_run(const AppendParams& p, int head, int t
     for (int side = 0; side < 2; ++side) {
         float now = top[side] * (1.0f / entry_max<E4M3>());
         if (now < 1.17549435e-38f) now = 0.f;
-        now = fmaxf(now, old[side]);
+        now = R::larger(now, old[side]);
         inv[side] = now > 0.f ? 1.0f / now : 0.f;
         ratio[side] = row > 0 && now > old[side] ? old[side] / now : 1.f;    // 1: what is in front of the run stays
         if (part == 0 && lane == 0) p.scales[side][at] = now;

@@ -49,7 +49,8 @@ def cache_append(k_pages, v_pages, k_scales, v_scales, k, v, slots) -> None:
 
     A page may hold one run of a call only: with two runs in one page - the same slot twice, say - its contents and scales are
     undefined.  Keys and values have pages and scales of their own.  Slots behind the cache are reported through the status word and
-    not written.  An infinity in k or v makes its page's scale infinite."""
+    not written.  An infinity in k or v makes its page's scale infinite, a NaN makes an int8 page's scale NaN (an e4m3 page holds it as
+    an entry), until a run begins the page again."""
     (_lib._native or _lib.native()).cache_append(k_pages, v_pages, k_scales, v_scales, k, v, slots)
 
 

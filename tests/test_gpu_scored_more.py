@@ -1,0 +1,49 @@
+"""`cache_append`, `scored_attention` and the stacks' generation at values and in orders that their other tests leave out."""
+import math
+
+import pytest
+import torch
+
+from oracle import scored as os_
+from test_gpu_scored import _both, _both_cache, _cache, _rand, _status
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("entry", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("side", [0, 1])
+@pytest.mark.parametrize("first,count", [(0, 40), (3, 2), (17, 20), (0, 1)])
+def test_an_appended_nan_comes_out_of_attention(entry, dtype, side, first, count):
+    """Prompts (a block's run) and steps (a warp's): who sees the page gets NaN, the other request and the other heads what they had."""
+    import stof_b200
+    cache = [x.cuda() for x in _cache([first + count, 50], 2, 16, 64, entry, 1)]
+    for b, length in enumerate((first + count, 50)):         # (what lies behind the keys may be anything, here it is not)
+        for x in cache[:2]:
+            x.view(torch.uint8)[cache[4][b, -(-length // 16) - 1].item(), :, length % 16 or 16:] = 0
+    x = [_rand((count, 2, 64), 2 + i, 1.0, dtype).cuda() for i in range(2)]
+    at = first + torch.arange(count, device="cuda")
+    slots = (cache[4][0][at // 16] * 16 + at % 16).int()
+    q = _rand((2, 1, 4, 64), 4).cuda()
+
+    def outputs(bad):
+        mine = [t.clone() for t in cache]
+        rows = [t.clone() for t in x]
+        if bad:
+            rows[side][count // 2, 1, 5] = math.nan
+        stof_b200.cache_append(*mine[:4], *rows, slots)
+        return stof_b200.cache_attention(q, *mine), mine
+
+    (clean, _), (got, mine) = outputs(False), outputs(True)
+    _status()
+    seen = got[0, 0, 2:]                                     # of head 1
+    if side == 0 or entry == torch.int8:
+        assert bool(torch.isnan(seen).all())
+    else:
+        assert bool(torch.isnan(seen[:, 5]).all())
+    assert torch.equal(got[1], clean[1]) and torch.equal(got[0, 0, :2], clean[0, 0, :2])
+    # a run that begins the pages again leaves nothing of it
+    at = torch.arange(first + count, device="cuda")
+    rows = _rand((first + count, 2, 64), 9, 1.0, dtype).cuda()
+    stof_b200.cache_append(*mine[:4], rows, rows, (cache[4][0][at // 16] * 16 + at % 16).int())
+    assert bool(torch.isfinite(stof_b200.cache_attention(q, *mine)).all())
