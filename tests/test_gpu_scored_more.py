@@ -47,3 +47,25 @@ def test_an_appended_nan_comes_out_of_attention(entry, dtype, side, first, count
     rows = _rand((first + count, 2, 64), 9, 1.0, dtype).cuda()
     stof_b200.cache_append(*mine[:4], rows, rows, (cache[4][0][at // 16] * 16 + at % 16).int())
     assert bool(torch.isfinite(stof_b200.cache_attention(q, *mine)).all())
+
+
+@pytest.mark.parametrize("low", [torch.finfo(torch.float32).min, -3e38, -1e30])
+def test_a_table_of_the_lowest_value_masks_as_a_low_score_does(low):
+    """Keys under it have no weight beside others, and a row of nothing else is a softmax over them: scores next to it lose all their digits,
+    in 64 bits too, so that all keys count alike."""
+    q, k, v = _rand((1, 2, 300, 64), 51, 2.0), _rand((1, 2, 300, 64), 52), _rand((1, 2, 300, 64), 53)
+    g = torch.Generator().manual_seed(5)
+    near = torch.randn(2, 2 * 200 + 1, generator=g)
+    near[:, :120] = low                                      # 81 and more behind
+    near[1, 300:] = low                                      # 99 and more ahead
+    for table in (near, torch.full((2, 41), low)):
+        for rules in (dict(), dict(causal=True), dict(softcap=20.0), dict(slopes=torch.tensor([0.25, 0.0]))):
+            _both(q, k, v, distance_bias=table, **rules)
+    lengths = [300, 1, 500]
+    for table in (near, torch.full((2, 41), low)):
+        for rules in (dict(), dict(window=130), dict(softcap=20.0), dict(slopes=torch.tensor([0.25, 0.0]))):
+            _both_cache(_rand((3, 3, 2, 64), 54, 2.0), _cache(lengths, 1, 32, 64, torch.int8, 55), distance_bias=table, **rules)
+    far = torch.full((2, 2 * 20 + 1), low)
+    far[:, :15] = 0.5                                        # what is near is masked, what is far is not
+    _both(q, k, v, causal=True, distance_bias=far)
+    _both_cache(_rand((3, 3, 2, 64), 54, 2.0), _cache(lengths, 1, 32, 64, torch.int8, 55), distance_bias=far)
