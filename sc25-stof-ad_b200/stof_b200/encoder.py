@@ -132,11 +132,12 @@ class BertEncoder:
         T = hidden.shape[0]
         if T > MAX_PROMPT_TOKENS:
             raise _lib.StofError(f"generation: {T} tokens of prompts in one call, beyond the maximum of {MAX_PROMPT_TOKENS}")
+        lengths = lengths.clamp(min=0)
         came = (lengths - cache.lengths).clamp(min=0)
         # tokens behind the last prompt, and all of them where pages are missing, are nobody's: a document of their own
         ends = came.cumsum(0)
         documents = torch.searchsorted(ends, torch.arange(T, device=hidden.device), right=True, out_int32=True).view(1, T)
-        slots, _ = cache.resize(lengths, T)
+        slots, _ = cache._resize(lengths, T)
 
         def attend(layer, q, k, v):
             q, k, v = (t.transpose(0, 1).unsqueeze(0) for t in (q, k, v))
@@ -157,7 +158,7 @@ class BertEncoder:
         if active is None:
             active = (cache.lengths > 0).int()
         # tokens of requests that take none have no slot: the slots of those that do, put to their rows
-        slots, starts = cache.resize(cache.lengths + active * n, R * n)
+        slots, starts = cache._resize(cache.lengths + active * n, R * n)
         at = starts[:-1].unsqueeze(1) + torch.arange(n, dtype=torch.int32, device=hidden.device)
         slots = torch.where(active.unsqueeze(1) > 0, slots[at.clamp(max=R * n - 1).long()], -1).view(-1)
 

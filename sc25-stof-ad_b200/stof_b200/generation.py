@@ -39,7 +39,10 @@ class GenerationCache:
     def resize(self, lengths, new_tokens: int):
         """Every request r is to hold lengths[r] tokens (0: it is done, and its pages are free again).  Returns (slots, starts) of
         the `new_tokens` tokens that come in, request by request.  Where pages are missing nothing changes and all slots are -1;
-        `check()` tells."""
+        `check()` tells.  Negative lengths count as 0."""
+        return self._resize(lengths.clamp(min=0), new_tokens)
+
+    def _resize(self, lengths, new_tokens: int):
         slots, starts, left, missing = page_tables(lengths, self.lengths, self.block_table, self.free_pages, self.free_count, self.page_size, new_tokens)
         self.free_count.copy_(left)
         self.lengths.copy_(torch.where(missing == 0, lengths, self.lengths))

@@ -69,3 +69,30 @@ def test_a_table_of_the_lowest_value_masks_as_a_low_score_does(low):
     far[:, :15] = 0.5                                        # what is near is masked, what is far is not
     _both(q, k, v, causal=True, distance_bias=far)
     _both_cache(_rand((3, 3, 2, 64), 54, 2.0), _cache(lengths, 1, 32, 64, torch.int8, 55), distance_bias=far)
+
+
+def _stack():
+    import stof_b200
+    from test_gpu_generation import HEADS, _weights
+    return stof_b200.gpt2_stack([stof_b200.EncoderWeights.from_dict(w, "cuda") for w in _weights(1)], HEADS), stof_b200.GenerationCache(1, HEADS, 3, 100, page_size=16)
+
+
+def _i32(*x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def test_negative_lengths_are_no_lengths():
+    """A request let go with a negative length holds nothing: what comes into its row next is as in a fresh cache."""
+    x, y = _rand((30, 256), 1).cuda(), _rand((3, 1, 256), 2).cuda()
+    results = []
+    for gone in (None, _i32(-1, 0, -7)):
+        stack, cache = _stack()
+        if gone is not None:
+            stack.prefill(_rand((33, 256), 3).cuda(), cache, _i32(20, 0, 13))
+            cache.resize(gone, 0)
+            assert cache.lengths.tolist() == [0, 0, 0]
+        results.append((stack.prefill(x, cache, _i32(12, 18, -3)), stack.step(y, cache)[:2], cache.lengths.tolist()))
+        cache.check()
+    _status()
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+    assert results[0][2] == results[1][2] == [13, 19, 0]
