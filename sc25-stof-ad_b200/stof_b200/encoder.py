@@ -125,19 +125,25 @@ class BertEncoder:
     def prefill(self, hidden: torch.Tensor, cache, lengths: torch.Tensor, **rules) -> torch.Tensor:
         """Prompts into a `GenerationCache`: hidden (T, hidden), T at most 131072, the prompts of the requests that come in back to back in the
         order of the requests; lengths (max_requests) int32: what every request holds afterwards (requests that are in the cache
-        already keep theirs, or are let go with 0; their tokens come by `step`, not here).  Returns (T, hidden).  The prompts attend
-        to themselves causally as they are, the cache holds them in 8 bits for the steps to come.  `rules`: softcap, slopes,
-        distance_bias, window, softmax_scale of `scored_attention`."""
+        already keep theirs or fewer, or are let go with 0; their tokens come by `step`, not here).  Returns (T, hidden).  The prompts attend
+        to themselves causally as they are, the cache holds them in 8 bits for the steps to come.  Where a request that holds tokens
+        is given more, or the prompts are longer than hidden, the call changes nothing in the cache and `cache.check()` raises.
+        `rules`: softcap, slopes, distance_bias, window, softmax_scale of `scored_attention`."""
         self._fits(hidden, cache, 2)
         T = hidden.shape[0]
         if T > MAX_PROMPT_TOKENS:
             raise _lib.StofError(f"generation: {T} tokens of prompts in one call, beyond the maximum of {MAX_PROMPT_TOKENS}")
+        if lengths.shape != cache.lengths.shape:
+            raise _lib.StofError(f"generation: lengths must be an int32 vector of {cache.lengths.shape[0]}")
         lengths = lengths.clamp(min=0)
         came = (lengths - cache.lengths).clamp(min=0)
         # tokens behind the last prompt, and all of them where pages are missing, are nobody's: a document of their own
         ends = came.cumsum(0)
         documents = torch.searchsorted(ends, torch.arange(T, device=hidden.device), right=True, out_int32=True).view(1, T)
-        slots, _ = cache._resize(lengths, T)
+        # what cannot be served is known on the GPU only: those calls leave every request as it is
+        wrong = ((came > 0) & (cache.lengths > 0)).any() | (ends[-1:] > T).any()
+        cache.refused += wrong
+        slots, _ = cache._resize(torch.where(wrong, cache.lengths, lengths), T)
 
         def attend(layer, q, k, v):
             q, k, v = (t.transpose(0, 1).unsqueeze(0) for t in (q, k, v))

@@ -31,6 +31,7 @@ class GenerationCache:
         self.free_count = torch.full((1,), pages, dtype=torch.int32, device=device)
         self.lengths = torch.zeros(max_requests, dtype=torch.int32, device=device)
         self.missing = torch.zeros(1, dtype=torch.int32, device=device)
+        self.refused = torch.zeros(1, dtype=torch.int32, device=device)
 
     @property
     def layers(self) -> int:
@@ -50,10 +51,14 @@ class GenerationCache:
         return slots, starts
 
     def check(self):
-        """Host-side check (synchronises): every `resize` so far found its pages."""
-        n = int(self.missing.item())
+        """Host-side check (synchronises): every `resize` so far found its pages, every `prefill` had lengths that it can serve."""
+        n, refused = torch.cat((self.missing, self.refused)).tolist()
+        self.missing.zero_()
+        self.refused.zero_()
+        if refused != 0:
+            raise _lib.StofError(f"GenerationCache: {refused} calls of prefill changed nothing: they gave tokens to requests that hold some already, or "
+                                 "more tokens to the requests than they brought")
         if n != 0:
-            self.missing.zero_()
             raise _lib.StofError(f"GenerationCache: {n} pages short, the last resizes changed nothing")
 
     def append(self, layer: int, k, v, slots):

@@ -96,3 +96,35 @@ def test_negative_lengths_are_no_lengths():
     _status()
     assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
     assert results[0][2] == results[1][2] == [13, 19, 0]
+
+
+@pytest.mark.parametrize("lengths", [(25, 0, 10), (20, 0, 0, ), (20, 31, 0), (-1, 30, 30)])
+def test_prompts_that_cannot_be_served_change_nothing(lengths):
+    """More tokens for a request that holds some; more tokens than there are."""
+    import stof_b200
+    stack, cache = _stack()
+    stack.prefill(_rand((20, 256), 1).cuda(), cache, _i32(15, 0, 5))
+    cache.check()
+    before = [x.view(torch.int8).clone() if x.dtype == torch.float8_e4m3fn else x.clone() for x in (cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, cache.block_table,
+                                                                                                      cache.free_pages, cache.free_count, cache.lengths)]
+    stack.prefill(_rand((30, 256), 2).cuda(), cache, _i32(*lengths))
+    after = [cache.k_pages.view(torch.int8), cache.v_pages.view(torch.int8), cache.k_scales, cache.v_scales, cache.block_table, cache.free_pages, cache.free_count, cache.lengths]
+    assert all(torch.equal(a, b) for a, b in zip(before, after))
+    with pytest.raises(stof_b200.StofError, match="1 calls of prefill changed nothing"):
+        cache.check()
+    cache.check()
+    # what follows is served: fewer tokens for one, none for another, a prompt for the third, tokens behind the last prompt
+    y = stack.prefill(_rand((30, 256), 2).cuda(), cache, _i32(10, 12, 0))
+    cache.check()
+    assert cache.lengths.tolist() == [10, 12, 0]
+    other, fresh = _stack()
+    assert torch.equal(other.prefill(_rand((30, 256), 2).cuda(), fresh, _i32(0, 12, 0))[:12], y[:12])
+
+
+def test_prompts_refuse_other_numbers_of_lengths():
+    import stof_b200
+    stack, cache = _stack()
+    for bad in (_i32(1, 2), _i32(5), torch.zeros(3, 1, dtype=torch.int32, device="cuda")):
+        with pytest.raises(stof_b200.StofError, match="lengths"):
+            stack.prefill(_rand((5, 256), 1).cuda(), cache, bad)
+    assert cache.lengths.tolist() == [0, 0, 0]
