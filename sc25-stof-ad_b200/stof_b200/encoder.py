@@ -114,6 +114,8 @@ class BertEncoder:
 
     def _generate(self, x, cache, slots, attend):
         """x (T, hidden) through all layers: new keys and values go to the cache, `attend(layer, q, k, v)` gives (T, hidden)."""
+        if x.shape[0] == 0:                                  # (requests left, none came)
+            return torch.empty_like(x)
         for i, w in enumerate(self.layers):
             q, k, v = gemm_bias(x, w.Wqkv, w.bqkv).view(-1, 3, cache.heads, cache.head_dim).unbind(1)
             cache.append(i, k, v, slots)

@@ -128,3 +128,15 @@ def test_prompts_refuse_other_numbers_of_lengths():
         with pytest.raises(stof_b200.StofError, match="lengths"):
             stack.prefill(_rand((5, 256), 1).cuda(), cache, bad)
     assert cache.lengths.tolist() == [0, 0, 0]
+
+
+def test_prompts_and_steps_of_nothing():
+    """Requests that leave while none come; no new tokens."""
+    stack, cache = _stack()
+    stack.prefill(_rand((20, 256), 1).cuda(), cache, _i32(15, 0, 5))
+    assert stack.prefill(_rand((0, 256), 1).cuda(), cache, _i32(0, 0, 5)).shape == (0, 256)
+    assert cache.lengths.tolist() == [0, 0, 5]
+    assert stack.step(_rand((3, 0, 256), 1).cuda(), cache).shape == (3, 0, 256)
+    cache.check()
+    _status()
+    assert cache.lengths.tolist() == [0, 0, 5]
