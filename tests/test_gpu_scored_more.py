@@ -140,3 +140,37 @@ def test_prompts_and_steps_of_nothing():
     cache.check()
     _status()
     assert cache.lengths.tolist() == [0, 0, 5]
+
+
+SHAPES = {"scored_attn_kernel<128, 2,": (1, 40, 500, 128), "scored_attn_kernel<128, 1,": (2, 40, 500, 128), "scored_attn_kernel<64, 1,": (8, 40, 500, 64)}
+RECORD = """
+import sys
+import torch
+from torch.profiler import ProfilerActivity, profile
+import stof_b200
+for shape in {shapes}:
+    q = torch.zeros(shape, dtype=torch.float16, device="cuda")
+    stof_b200.scored_attention(q, q, q)
+    torch.cuda.synchronize()
+    with profile(activities=[ProfilerActivity.CUDA]) as record:
+        stof_b200.scored_attention(q, q, q)
+        torch.cuda.synchronize()
+    print("|".join(e.name for e in record.events() if "stof::" in e.name))
+"""
+
+
+def test_shapes_run_on_their_kernels_in_a_process_of_its_own():
+    """(late in a long process the profiler records nothing): the shapes of the tests of two stretches that share their tiles take that kernel, those
+    of twice the batch do not."""
+    import os
+    import subprocess
+    import sys
+
+    import stof_b200
+    if torch.cuda.get_device_properties(0).multi_processor_count != 148:
+        pytest.skip("the sizes are those of 148 SMs")
+    path = os.path.dirname(os.path.dirname(os.path.abspath(stof_b200.__file__)))
+    run = subprocess.run([sys.executable, "-c", RECORD.format(shapes=list(SHAPES.values()))], env={**os.environ, "PYTHONPATH": path}, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr
+    names = run.stdout.strip("\n").split("\n")
+    assert len(names) == len(SHAPES) and all(kernel in name for kernel, name in zip(SHAPES, names)), names
