@@ -1052,6 +1052,7 @@ PyObject* py_page_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
              as_int(fresh, "new tokens"), static_cast<int*>(starts.data_ptr()), static_cast<int*>(left.data_ptr()), static_cast<int*>(missing.data_ptr()),
              l.status, l.stream);
         PyObject* tuple = PyTuple_New(4);
+        if (tuple == nullptr) throw PythonFail{};
         const at::Tensor* o[4] = {&slots, &starts, &left, &missing};
         for (int i = 0; i < 4; ++i) PyTuple_SET_ITEM(tuple, i, wrap(*o[i]));
         return tuple;
@@ -1178,6 +1179,7 @@ PyObject* py_sparse_storage(PyObject*, PyObject* const* a, Py_ssize_t n) {
         }
         const at::Tensor* out[8] = {&nnz, &frp, &fci, &prp, &pci, &tiles, &lrp, &lci};
         PyObject* tuple = PyTuple_New(8);
+        if (tuple == nullptr) throw PythonFail{};
         for (int i = 0; i < 8; ++i) PyTuple_SET_ITEM(tuple, i, wrap(*out[i]));
         return tuple;
     });
