@@ -352,24 +352,19 @@ __global__ void __launch_bounds__(CT_THREADS, ct_blocks(NT, D)) cache_attn_kerne
                                 top = fmaxf(top, fabsf(s[t][nt][e]));
                             }
                     if (__all_sync(0xffffffffu, top <= 0.35f)) {
-                        // an odd polynomial, off by 2.9e-6 of the value at most (weighted least squares moved towards the minimax one)
 #pragma unroll
                         for (int t = 0; t < CT_TILES; ++t)
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    const float u = s[t][nt][e], w = u * u;
-                                    s[t][nt][e] = u * from * fmaf(w, fmaf(w, 0.1239503026008606f, -0.33290955424308777f), 0.9999971389770508f);
-                                }
+                                for (int e = 0; e < 4; ++e) s[t][nt][e] = from * tanh_near_zero(s[t][nt][e]);
                     } else {
-                        // tanh(u) = 1 - 2 / (1 + e^(2u)): off by 1e-7
 #pragma unroll
                         for (int t = 0; t < CT_TILES; ++t)
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) s[t][nt][e] = fmaf(-2.f * from, fast_reciprocal(1.f + fast_exp2(s[t][nt][e] * (2.f * LOG2E))), from);
+                                for (int e = 0; e < 4; ++e) s[t][nt][e] = from * tanh_any(s[t][nt][e]);
                     }
                 } else {
 #pragma unroll

@@ -119,8 +119,6 @@ static __device__ __forceinline__ float2 odd_polynomial_plus(float2 s, const flo
     for (int i = N - 2; i >= 0; --i) q = fma2(q, w, pk2(c[i], c[i]));
     return fma2(q, s, added);
 }
-// tanh(u) = 1 - 2 / (1 + e^(2u)): off by 1e-7, where it is not near zero
-static __device__ __forceinline__ float tanh_any(float u) { return 1.f - 2.f * fast_reciprocal(1.f + fast_exp2(u * (2.f * SA_LOG2E))); }
 
 // The bounded wait without a call of a function (which does not go with moved registers)
 static __device__ __forceinline__ void wait_inline(uint32_t bar, uint32_t parity, const WaitCtx& ctx, int barrier_id) {

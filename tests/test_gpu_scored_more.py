@@ -174,3 +174,15 @@ def test_shapes_run_on_their_kernels_in_a_process_of_its_own():
     assert run.returncode == 0, run.stderr
     names = run.stdout.strip("\n").split("\n")
     assert len(names) == len(SHAPES) and all(kernel in name for kernel, name in zip(SHAPES, names)), names
+
+
+@pytest.mark.parametrize("rules", [dict(), dict(causal=True), dict(slopes=torch.tensor([0.25, 0.1, 0.0, 0.02]))])
+def test_a_large_cap_beside_one_row_of_huge_scores(rules):
+    """The row's neighbours, whose scores are of size one, keep their digits under a cap of a million."""
+    q, k, v = (_rand((1, 4, 200, 64), 61 + i, 1.5, torch.bfloat16) for i in range(3))
+    q[0, :, 70] *= 1e6
+    _both(q, k, v, torch.bfloat16, softcap=1e6, **rules)
+    rules = {n: x for n, x in rules.items() if n != "causal"}
+    q = _rand((2, 2, 4, 64), 64, 1.5, torch.bfloat16)
+    q[:, 1, 2] *= 1e6
+    _both_cache(q, _cache([300, 77], 1, 32, 64, torch.int8, 65), softcap=1e6, **rules)
