@@ -84,12 +84,16 @@ static __device__ __forceinline__ float min3f(float a, float b, float c) {
 // 3e-4 at most, less than P's rounding to fp16 makes of it.
 struct NearTanh {
     float near[3], far[5];                   // of s, s^3, s^5, ..
-    float near_end, far_end;                 // up to which |s| they are used: -1, not even for 0, where powers of to_u leave fp32's range
+    float near_end, far_end;                 // up to which |s| they are used: -1, not even for 0, where a coefficient leaves fp32's range
     __device__ __forceinline__ NearTanh() : near{}, far{}, near_end(-1.f), far_end(-1.f) {}
     __device__ __forceinline__ NearTanh(float to_u, float from_u) {
         const float w = to_u * to_u, a = to_u * from_u;
-        near_end = to_u < 1e8f ? 0.35f / to_u : -1.f;         // (below 1e-10 the higher terms vanish, and so do they in the sum)
-        far_end = to_u > 2e-4f && to_u < 5e3f ? 1.f / to_u : -1.f;
+        // Where a coefficient is below fp32's normal numbers the polynomial ends where the term is below 1e-7 of the sum, and where the
+        // smallest number that stands for the last one (below) makes 1e-7 of it
+        const float u_end = a * w * w > 1e-36f ? 0.35f : a * w > 1e-36f ? 0.03f : 5e-4f;
+        near_end = to_u > 1e-37f && a * w * w < 1e37f ? u_end / to_u : -1.f;
+        if (u_end < 0.35f) near_end = fminf(near_end, sqrtf(sqrtf(fminf(a, 1.f) * 7e37f)));
+        far_end = a * w * w * w * w > 1e-34f && a * w * w * w * w < 1e37f ? 1.f / to_u : -1.f;
         near[0] = a * 0.9999971389770508f;
         near[1] = a * w * -0.33290955424308777f;
         near[2] = a * w * w * 0.1239503026008606f;
@@ -135,15 +139,16 @@ static __device__ __forceinline__ void wait_inline(uint32_t bar, uint32_t parity
     }
 }
 
-// tanh of a whole row's scores in tensor memory that are not near enough to zero for a polynomial: s = from_u * tanh(s * to_u), in place
-static __device__ __forceinline__ void cap_in_tmem(uint32_t t_s, float to_u, float from_u) {
+// tanh of a whole row's scores in tensor memory that are not near enough to zero for a polynomial: s = from_u * tanh(s * scale * to_u), in place (one after
+// the other: together they may be no normal number)
+static __device__ __forceinline__ void cap_in_tmem(uint32_t t_s, float scale, float to_u, float from_u) {
 #pragma unroll 1
     for (int c = 0; c < SA_T; c += 16) {
         uint32_t s[16];
         tmem_ld16(t_s + c, s);
         tc_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = __float_as_uint(tanh_any(__uint_as_float(s[i]) * to_u) * from_u);
+        for (int i = 0; i < 16; ++i) s[i] = __float_as_uint(tanh_any(__uint_as_float(s[i]) * scale * to_u) * from_u);
         tmem_st16(t_s + c, s);
     }
     tc_wait_st();
@@ -508,7 +513,7 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(HALVES))
                     return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 };
                 auto cap_exactly = [&] {
-                    cap_in_tmem(t_s, to_u, from_u);
+                    cap_in_tmem(t_s, p.scale, 1.f / p.softcap, from_u);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) tmem_ld32(t_s + 32 * i, s[i]);
                     tc_wait_ld();

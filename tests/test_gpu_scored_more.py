@@ -186,3 +186,15 @@ def test_a_large_cap_beside_one_row_of_huge_scores(rules):
     q = _rand((2, 2, 4, 64), 64, 1.5, torch.bfloat16)
     q[:, 1, 2] *= 1e6
     _both_cache(q, _cache([300, 77], 1, 32, 64, torch.int8, 65), softcap=1e6, **rules)
+
+
+@pytest.mark.parametrize("power", [100, 60, 50, 30, 15, -15, -30, -60, -100])
+@pytest.mark.parametrize("cap", [1e-3, 2.0, 20.0, 1e6, 1e12, 1e20, 3e38])
+def test_caps_under_scales_far_from_one(power, cap):
+    """Queries of 2^power under a softmax_scale that takes it back: the cap's polynomial is of the raw score, whose powers may leave fp32."""
+    q, k, v = (_rand((1, 2, 200, 64), 71 + i, 1.5, torch.bfloat16) for i in range(3))
+    big = (q.float() * 2.0 ** power).bfloat16()
+    for rules in (dict(), dict(causal=True, slopes=torch.tensor([0.25, 0.02]))):
+        _both(big, k, v, torch.bfloat16, softcap=cap, softmax_scale=2.0 ** (-power - 3), **rules)
+        rules.pop("causal", None)
+        _both_cache(big[0].transpose(0, 1)[:4].reshape(2, 2, 2, 64), _cache([300, 77], 1, 32, 64, torch.int8, 65), softcap=cap, softmax_scale=2.0 ** (-power - 3), **rules)
