@@ -341,7 +341,7 @@ int stof_cache_append(void* k_pages, void* v_pages, float* k_scales, float* v_sc
  * request r, -1 behind the last token; *free_count_out (may be free_count); *missing_out = 0.
  * All or nothing: where the stack holds too few pages, or a row too few entries, *missing_out is the number of pages short, all
  * slots are -1 and nothing else changes; where the pages given back do not fit the stack it is negative.
- * Negative lengths count as 0; held is counted to at most table_width * page_size; starts and missing stop at 2^31 - 1.
+ * The table has fewer than 2^31 entries.  Negative lengths count as 0; held is counted to at most table_width * page_size; starts and missing stop at 2^31 - 1.
  * ------------------------------------------------------------------------------------------ */
 int stof_page_tables(const int* lengths, const int* held, int requests, int* block_table, long long table_stride, int table_width,
                      int* free_pages, int free_capacity, const int* free_count, int page_size,

@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(PT_THREADS) page_tables_kernel(const PageTable
             q.need = static_cast<int>((static_cast<long long>(len) + page - 1) >> p.page_shift);
             q.fresh = static_cast<unsigned>(max(len - q.held, 0));
             if (count && q.need > p.table_width) atomicAdd(&beyond, static_cast<unsigned long long>(q.need - p.table_width));
-            q.need = min(q.need, p.table_width);             // (sums of what rows hold fit 32 bits, as the table fits memory)
+            q.need = min(q.need, p.table_width);             // (sums of what rows hold fit 32 bits: the table has fewer entries)
             own = {static_cast<unsigned>(max(q.need - q.have, 0)), static_cast<unsigned>(max(q.have - q.need, 0)), q.fresh};
         }
         Sums s = own;
@@ -244,6 +244,7 @@ extern "C" int stof_page_tables(const int* lengths, const int* held, int request
     STOF_REQUIRE(page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128, "page_tables: page size %d not in {16, 32, 64, 128}", page_size);
     STOF_REQUIRE(requests == 0 || (lengths && held), "page_tables: null lengths or held");
     STOF_REQUIRE(requests == 0 || table_width == 0 || (block_table && table_stride >= table_width), "page_tables: null block table, or a row stride below its width");
+    STOF_REQUIRE(static_cast<long long>(requests) * table_width < (1ll << 31), "page_tables: a block table of 2^31 entries or more");
     STOF_REQUIRE((free_pages || free_capacity == 0) && free_count && free_count_out && missing_out && starts, "page_tables: null pointer");
     STOF_REQUIRE(slots || slot_count == 0, "page_tables: null slots");
     PageTablesParams p;

@@ -164,3 +164,8 @@ def test_restated_page_tables():
 def test_cache_attn_refuses_rows_beyond_32_bits(lib):
     assert _cache(lib, heads=64, kv_heads=1, tokens=(1 << 24) + 1) == -1 and b"2^30" in lib.stof_last_error()
     assert lib.stof_cache_attn_workspace_bytes(1, (1 << 24) + 1, 64, 1, 64, 16, 4) == 0
+
+
+def test_page_tables_refuse_tables_beyond_32_bits(lib):
+    rc = lib.stof_page_tables(ONE, ONE, 1 << 16, ONE, 1 << 15, 1 << 15, ONE, 8, ONE, 16, ONE, 4, ONE, ONE, ONE, None, None)
+    assert rc == -1 and b"2^31 entries" in lib.stof_last_error()
