@@ -198,3 +198,25 @@ def test_caps_under_scales_far_from_one(power, cap):
         _both(big, k, v, torch.bfloat16, softcap=cap, softmax_scale=2.0 ** (-power - 3), **rules)
         rules.pop("causal", None)
         _both_cache(big[0].transpose(0, 1)[:4].reshape(2, 2, 2, 64), _cache([300, 77], 1, 32, 64, torch.int8, 65), softcap=cap, softmax_scale=2.0 ** (-power - 3), **rules)
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, torch.float16), (128, torch.bfloat16)])
+def test_documents_over_the_longest_row(dim, dtype):
+    """131072 packed tokens, the most that documents may name: rows at the beginning, at tiles' borders and at the end."""
+    import stof_b200
+    n = 131072
+    g = torch.Generator().manual_seed(81)
+    docs = torch.randint(1, 9000, (64,), generator=g).cumsum(0)
+    docs = torch.searchsorted(docs, torch.arange(n), right=True).int()
+    q, k, v = (_rand((1, h, n, dim), 82 + i, 1.5, dtype) for i, h in enumerate((2, 1, 1)))
+    slopes = torch.tensor([0.01, 0.0])
+    got = stof_b200.scored_attention(q.cuda(), k.cuda(), v.cuda(), causal=True, documents=docs[None].cuda(), slopes=slopes.cuda()).cpu()
+    _status()
+    border = [int(i) for i in (docs[1:] != docs[:-1]).nonzero()[:40:5, 0]]
+    for row in [0, 1, 127, 128, 65535, 65536, 131071, *border, *(i + 1 for i in border)]:
+        first = int((docs == docs[row]).nonzero()[0, 0])
+        for h in range(2):
+            x = os_.changed_scores(q[0, h, row:row + 1], k[0, 0, first:row + 1], torch.tensor([row - first]), scale=dim ** -0.5, slope=slopes[h])
+            want = torch.softmax(x, 1) @ v[0, 0, first:row + 1].double()
+            u = torch.finfo(dtype).eps / 2
+            assert bool(((got[0, h, row].double() - want[0]).abs() <= u * want[0].abs() + (u + 6e-4) * float(v.abs().max()) + 1e-6).all()), (row, h)
