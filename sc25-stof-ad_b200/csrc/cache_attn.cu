@@ -5,7 +5,8 @@
 // on mma.sync m16n8k16.  A tcgen05 product has at least 64 rows of which a decoding step fills one to eight, and takes its operands
 // from shared memory as 8 or 16 bits; here the entries become fp16 (exactly) on their way from shared memory to registers and are
 // multiplied.  The scales stay out of the products: K's goes into the score, V's into P, relative to a reference of the row's own
-// that follows the largest p * |scale| it has met: what carries weight keeps fp16's precision, whatever the scales are and in whatever order.
+// that follows the largest p * |scale| it has met: what carries weight keeps fp16's precision, whatever the scales are and in whatever order
+// (a p below 2^-126 of its row's largest is 0 in fp32, as it would be in any softmax).
 //
 // Which lane holds which entry is free as long as both operands agree, so that every read is 16 bytes of a row: with g = lane / 4,
 // c = lane % 4, a lane reads chunk c (and c + 4) of the rows of keys g and g + 8 for S, and chunk g of the rows of keys 2c, 2c + 1,
@@ -531,7 +532,10 @@ __global__ void __launch_bounds__(CT_THREADS, ct_blocks(NT, D)) cache_attn_kerne
                         for (int e = 0; e < 4; ++e) {
                             x[e] = fast_exp2(s[t][nt][e]);
                             w[e] = x[e] * (v_scale[t] * c_row[nt][e & 1]);
-                            if constexpr (decltype(masked)::value) w[e] = x[e] == 0.f ? 0.f : w[e];
+                            if constexpr (decltype(masked)::value) {
+                                const float c = c_row[nt][e & 1];            // (large, its product with a large scale may leave fp32; small, p's may)
+                                w[e] = x[e] == 0.f ? 0.f : c >= 1.f ? x[e] * v_scale[t] * c : w[e];
+                            }
                         }
                         l[nt][0] += x[0] + x[2];
                         l[nt][1] += x[1] + x[3];

@@ -61,7 +61,8 @@ def _check(q, cache, **rules):
     for the product, together with V's scale: 2^-11 of sum(p |v|), and 2^-25 each where it is that small beside a largest p |scale| of
     a half at least, so n 2^-24 max(p |scale|) max|entry|.  Sums in fp32: 2^-14 of sum(p |v|) is more than chains of a hundred make
     of it.  A score is off by 2^-20 of the sum of its parts' magnitudes (products of 128 terms added in fp32, a few factors), a capped
-    one by 3e-6 of itself and 3e-7 of the cap; its p by as much relative, and so the sums that it is in."""
+    one by 3e-6 of itself and 3e-7 of the cap; its p by as much relative, and so the sums that it is in.  A p of 2^-126 of its row's largest
+    and below is no normal fp32 number and counts as 0 (to 2^-125: the reference that it is held to may be a rounding off)."""
     import stof_b200
     kp, vp, ks, vs, table, lengths = cache
     got = stof_b200.cache_attention(q, *cache, **rules)
@@ -103,7 +104,8 @@ def _check(q, cache, **rules):
         off = torch.where(p > 0, off, 0.0)
         want, size = p @ v, p @ v.abs()
         allow = u * want.abs() + (2.0 ** -11 + 2.0 ** -14) * size + (p * off) @ v.abs() + want.abs() * (p * off).sum(2, keepdim=True) \
-            + length * 2.0 ** -24 * (p * v_scale.abs()[:, None]).amax(2, keepdim=True) * MOST[vp.dtype] + 2.0 ** -25
+            + length * 2.0 ** -24 * (p * v_scale.abs()[:, None]).amax(2, keepdim=True) * MOST[vp.dtype] + 2.0 ** -25 \
+            + torch.where(p < p.amax(2, keepdim=True) * 2.0 ** -125, p, 0.0) @ v.abs()
         mine = got[b].double().transpose(0, 1).reshape(N, group * T, D)
         over = (mine - want).abs() - allow
         assert float(over.max()) <= 0, f"request {b}: off by {float((mine - want).abs().max()):.3e}, bound exceeded by {float(over.max()):.3e}"
@@ -298,3 +300,18 @@ def test_pages_in_front_of_the_window_may_be_anything(tokens, page, window):
         got = stof_b200.cache_attention(q, kp, vp, ks, vs, t, n, window=window)
         _status()
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("low", [100, 120, 122, 124, 126, 140])
+@pytest.mark.parametrize("up", [-90, -20])
+@pytest.mark.parametrize("ratio", [110, 129, 131, 133, 140])
+def test_a_large_scale_under_little_weight(low, up, ratio):
+    """Values of 2^up at full weight, then values 2^ratio larger at 2^-low of it: neither factor of the second product may leave fp32 alone."""
+    lengths = [256] * 16
+    kp, vp, ks, vs, table, n = _cache(lengths, 20, 128, 64, torch.int8, 32)
+    ks.zero_()
+    vs[table[:, 0].long()] = 2.0 ** up / 64
+    vs[table[:, 1].long()] = 2.0 ** (up + ratio) / 64
+    bias = torch.zeros(20, 2 * 200 + 1, device="cuda")
+    bias[:, 200 - 127:] = -low * math.log(2)
+    _check(_q(16, 1, 20, 64, torch.bfloat16, 33), (kp, vp, ks, vs, table, n), distance_bias=bias)
