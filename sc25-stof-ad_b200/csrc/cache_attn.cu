@@ -472,8 +472,21 @@ __global__ void __launch_bounds__(CT_THREADS, ct_blocks(NT, D)) cache_attn_kerne
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float top = tops[nt][e];       // log2 of the row's largest P; and P * |scale|
-                        float weight = top + v_log[0];
+                        const float top = tops[nt][e];
+                        const bool seen = top > -INFINITY, first = most[nt][e] == -INFINITY;
+                        float up = 0.f;
+                        if (seen && (first || top > 0.f)) {  // by a whole number of powers of two, behind the first
+                            const float to = m[nt][e] + (first ? top : ceilf(top));
+                            up = to - m[nt][e];
+                            m[nt][e] = to;
+                            l[nt][e] *= first ? 0.f : fast_exp2(-up);
+#pragma unroll
+                            for (int t = 0; t < CT_TILES; ++t) {
+                                s[t][nt][e] -= up;
+                                s[t][nt][2 + e] -= up;
+                            }
+                        }
+                        float weight = top - up + v_log[0];  // log2 of the row's largest P * |scale|
                         if (!alike) {
                             weight = -INFINITY;
 #pragma unroll
@@ -481,21 +494,7 @@ __global__ void __launch_bounds__(CT_THREADS, ct_blocks(NT, D)) cache_attn_kerne
 #pragma unroll
                             for (int d = 4; d < 32; d <<= 1) weight = fmaxf(weight, __shfl_xor_sync(0xffffffffu, weight, d));
                         }
-                        if (top > -INFINITY) {
-                            const bool first = most[nt][e] == -INFINITY;
-                            float up = 0.f;
-                            if (first || top > 0.f) {        // by a whole number of powers of two, behind the first
-                                const float to = m[nt][e] + (first ? top : ceilf(top));
-                                up = to - m[nt][e];
-                                m[nt][e] = to;
-                                l[nt][e] *= first ? 0.f : fast_exp2(-up);
-                                weight -= up;
-#pragma unroll
-                                for (int t = 0; t < CT_TILES; ++t) {
-                                    s[t][nt][e] -= up;
-                                    s[t][nt][2 + e] -= up;
-                                }
-                            }
+                        if (seen) {
                             const float c_old = c_row[nt][e], log_c = static_cast<float>(static_cast<int>(__float_as_uint(c_old) >> 23) - 127);
                             // as P shrinks by 2^up c may grow by it, and o stays as it is, unless the new P * |scale| asks for less
                             float log_to = log_c + rintf(up);

@@ -315,3 +315,19 @@ def test_a_large_scale_under_little_weight(low, up, ratio):
     bias = torch.zeros(20, 2 * 200 + 1, device="cuda")
     bias[:, 200 - 127:] = -low * math.log(2)
     _check(_q(16, 1, 20, 64, torch.bfloat16, 33), (kp, vp, ks, vs, table, n), distance_bias=bias)
+
+
+@pytest.mark.parametrize("low", [-1e3, -1e9, -3e38])
+@pytest.mark.parametrize("spread", [4, 30])
+def test_low_scores_under_scales_of_any_size(low, spread):
+    """What the first steps leave at scores that masks make is in no way of what carries weight, large scales among it."""
+    lengths = [4000, 1500, 900, 0, 2049, 3333, 5000, 4224]
+    assert _steps(lengths, 8, 1, 64) >= 2
+    kp, vp, ks, vs, table, n = _cache(lengths, 8, 32, 64, torch.int8, 34)
+    g = torch.Generator(device="cuda").manual_seed(35)
+    vs = vs * torch.exp2((torch.rand(vs.shape, generator=g, device="cuda") * 2 - 1) * spread)
+    bias = torch.randn(8, 2 * 2000 + 1, generator=g, device="cuda")
+    for reach in (2000, 1400, 700, 33):                  # keys at this distance and beyond
+        bias[:, :2001 - reach] = low
+        _check(_q(8, 1, 8, 64, torch.bfloat16, 36), (kp, vp, ks, vs, table, n), distance_bias=bias)
+        _check(_q(8, 1, 8, 64, torch.bfloat16, 36), (kp, vp, ks, vs, table, n), distance_bias=bias, slopes=torch.full((8,), 0.04, device="cuda"))
