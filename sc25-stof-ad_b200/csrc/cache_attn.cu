@@ -498,7 +498,7 @@ __global__ void __launch_bounds__(CT_THREADS, ct_blocks(NT, D)) cache_attn_kerne
                             const float c_old = c_row[nt][e], log_c = static_cast<float>(static_cast<int>(__float_as_uint(c_old) >> 23) - 127);
                             // as P shrinks by 2^up c may grow by it, and o stays as it is, unless the new P * |scale| asks for less
                             float log_to = log_c + rintf(up);
-                            if (c_old == 0.f || weight + log_to > 7.f) log_to = floorf(-weight);
+                            if (c_old == 0.f || weight + log_to > 0.f) log_to = floorf(-weight);
                             log_to = fminf(fmaxf(log_to, -126.f), 126.f);
                             most[nt][e] = 8.f;
                             if (c_old == 0.f && weight == -INFINITY) {
