@@ -398,7 +398,11 @@ __global__ void __launch_bounds__(CT_THREADS, ct_blocks(NT, D)) cache_attn_kerne
                                 const int away = key + 16 * t + g + 8 * (e >> 1) - pos[nt][e & 1];   // at most 0 where visible
                                 x += slope[nt][e & 1] * static_cast<float>(away);
                                 const bool on = left[t] > 0 && pos[nt][e & 1] >= 0 && away <= 0 && (p.window == 0 || away > -p.window);
-                                if (p.distance_bias != nullptr && on) x += bias_log2(__ldca(table[nt][e & 1] + max(away, -p.radius)));
+                                if (p.distance_bias != nullptr && on) {
+                                    const float bias = __ldca(table[nt][e & 1] + max(away, -p.radius));
+                                    const float y = finite_or_nan(fmaf(bias, LOG2E, x));
+                                    x = bias == -INFINITY ? bias : y;
+                                }
                                 s[t][nt][e] = on ? x - m[nt][e & 1] : -INFINITY;
                             }
                 }

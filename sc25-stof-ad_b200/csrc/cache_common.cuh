@@ -27,11 +27,12 @@ __device__ __forceinline__ void entries_to_half(uint32_t w, uint32_t& lo, uint32
 // A cap whose inverse and multiples stay inside fp32: scores capped to 1e-30 are all alike, and 1e30 caps none that are told apart
 inline float usable_cap(float cap) { return cap > 0.f ? (cap < 1e-30f ? 1e-30f : cap > 1e30f ? 1e30f : cap) : 0.f; }
 
-// A table's bias in units of log2.  A finite one stays finite: keys masked by fp32's lowest value are still visible, and a row that sees no
-// others is a softmax over them (those beyond 2.3e38 count as alike).
-__device__ __forceinline__ float bias_log2(float bias) {
-    const float x = bias * 1.4426950408889634f, most = 3.40282347e38f;
-    return fabsf(bias) <= most ? fminf(fmaxf(x, -most), most) : x;
+// A finite bias stays finite in units of log2: keys masked by fp32's lowest value are still visible, and a row that sees no others is a softmax
+// over them (those beyond 2.3e38 count as alike).  A NaN stays.
+__device__ __forceinline__ float finite_or_nan(float x) {
+    float y;
+    asm("{\n\t.reg .f32 a;\n\tmax.NaN.f32 a, %1, 0fFF7FFFFF;\n\tmin.NaN.f32 %0, a, 0f7F7FFFFF;\n\t}" : "=f"(y) : "f"(x));
+    return y;
 }
 
 // 1 / x to a unit in the last place

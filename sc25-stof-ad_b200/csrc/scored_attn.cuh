@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(scored_threads(HALVES), scored_per_sm(HALVES))
             for (int j = 0; j < 4; ++j) v[j] = __ldca(src + min(max(i0 + j * helpers - SA_PAD, 0), 2 * p.radius));
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (i0 + j * helpers < count) table[i0 + j * helpers] = bias_log2(v[j]);
+                if (i0 + j * helpers < count) table[i0 + j * helpers] = v[j] == -INFINITY ? v[j] : finite_or_nan(v[j] * SA_LOG2E);
         }
     }
     // the documents of the tiles that the rules may want, whatever the lengths are
