@@ -563,10 +563,13 @@ __global__ void __launch_bounds__(CT_THREADS, ct_blocks(NT, D)) cache_attn_kerne
                         v[j] = make_uint4(w.x, w.y, 0u, 0u);
                     }
                 }
-                if (left[t] < 16) {
+                const int hidden = seen_from - key - 16 * t;             // keys of the tile in front of every token's window
+                if (left[t] < 16 || hidden > 0) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (2 * c + (j & 1) + 8 * (j >> 1) >= left[t]) v[j] = make_uint4(0u, 0u, 0u, 0u);
+                    for (int j = 0; j < 4; ++j) {
+                        const int row = 2 * c + (j & 1) + 8 * (j >> 1);
+                        if (row >= left[t] || row < hidden) v[j] = make_uint4(0u, 0u, 0u, 0u);
+                    }
                 }
 #pragma unroll
                 for (int w = 0; w < V_BYTES / 4; ++w) {

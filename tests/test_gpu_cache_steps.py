@@ -331,3 +331,22 @@ def test_low_scores_under_scales_of_any_size(low, spread):
         bias[:, :2001 - reach] = low
         _check(_q(8, 1, 8, 64, torch.bfloat16, 36), (kp, vp, ks, vs, table, n), distance_bias=bias)
         _check(_q(8, 1, 8, 64, torch.bfloat16, 36), (kp, vp, ks, vs, table, n), distance_bias=bias, slopes=torch.full((8,), 0.04, device="cuda"))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("tokens,window", [(1, 1), (1, 70), (3, 70), (2, 333)])
+def test_values_in_front_of_the_window_take_no_part(dim, tokens, window):
+    """A NaN leaves the results when the window leaves it, not when it leaves the page."""
+    import stof_b200
+    lengths = [600, 129, 75, 40, 350]
+    q = _q(5, tokens, 4, dim, torch.float16, 37)
+    kp, vp, ks, vs, table, n = _cache(lengths, 2, 64, dim, torch.float8_e4m3fn, 38)
+    want = _check(q, (kp, vp, ks, vs, table, n), window=window)
+    for b, length in enumerate(lengths):
+        for key in range(max(length - tokens - window + 1, 0)):
+            page = table[b, key // 64].item()
+            for x in (kp, vp):
+                x.view(torch.uint8)[page, :, key % 64] = 0x7F
+    got = stof_b200.cache_attention(q, kp, vp, ks, vs, table, n, window=window)
+    _status()
+    assert torch.equal(got, want)
