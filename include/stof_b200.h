@@ -251,8 +251,10 @@ int stof_bias_residual_layernorm(const void* x, long long ldx, const void* bias,
  * (STOF_DTYPE_F16 / STOF_DTYPE_BF16), fp32 accumulation, head_dim 64 or 128; heads a multiple of kv_heads, query head h reads
  * K/V head h / (heads / kv_heads).  Query i sits at position i + k_len - q_len among the keys.  With
  *   x = softmax_scale * (q . k);  softcap > 0: x = softcap * tanh(x / softcap);
+ *   (off by up to 7e-6 of itself)
  *   slopes (heads): x -= slopes[h] * |position - j|;
- *   distance_bias (heads, 2 * bias_radius + 1): x += distance_bias[h][bias_radius + clamp(j - position, -radius, radius)];
+ *   distance_bias (heads, 2 * bias_radius + 1): x += distance_bias[h][bias_radius + clamp(j - position, -radius, radius)],
+ *   where minus infinity takes keys out and a finite low value leaves them visible;
  * key j is visible to the query if
  *   j < key_lens[b] (where given), documents[b][j] == documents[b][position] (where given), and
  *   j < prefix_lens[b] (where given), or (not causal or j <= position) and (window == 0 or |position - j| < window).
@@ -298,8 +300,10 @@ int stof_scored_attn(const void* q, const void* k, const void* v, void* out, int
  * request b sits at position lengths[b] - tokens + t; keys behind a token's position are not visible to it, nor, with
  * window > 0, those window or more in front of it.  softcap, slopes, distance_bias as above (causal, documents, prefix_lens and
  * key_lens of `rules` are not read).  lengths int32 (requests), counted to at most table_width * page_size; requests of length
- * 0 give zeros.  A page number outside [0, pages) is reported through status_dev and its keys are left out.  Behind a request's
- * length, and for pages that a window hides from all of its tokens, the table may hold anything.
+ * 0 give zeros.  A page number outside [0, pages) is reported through status_dev, its keys are left out and `out` is not to be
+ * used.  Behind a request's length, and for pages that a window hides from all of its tokens, the table may hold anything.
+ * A NaN or an infinity in a value that one of a request's tokens sees reaches its other tokens, one in a page's scale those
+ * that see the page.
  * Work is dealt evenly over the GPU whatever the lengths; what a thread block computes of a request's head goes to `workspace`
  * (stof_cache_attn_workspace_bytes bytes, 16-byte aligned, not shared with a call that may run at the same time) where it is not
  * all of it, and a second kernel joins the parts in a fixed order.
@@ -323,7 +327,8 @@ int stof_cache_attn(const void* q, void* out, int dtype, const long long q_strid
  * entries in front of the run are rounded again to it.  entry = round(x * (1 / scale)), to nearest even; a scale below the
  * smallest normal fp32 counts as 0.  An infinity makes its page's scale infinite; a NaN makes its page's scale NaN (int8; until a
  * run begins the page again) or its own entry (e4m3).  A page may hold one run of a call only: two runs in the same page write it unordered.
- * Slots at or behind pages * page_size are reported through status_dev and not written.
+ * Slots at or behind pages * page_size are reported through status_dev and not written; what the call leaves of the other
+ * tokens is then not to be used.
  * ------------------------------------------------------------------------------------------ */
 int stof_cache_append(void* k_pages, void* v_pages, float* k_scales, float* v_scales, int cache_dtype,
                       int pages, int page_size, int kv_heads, int head_dim,

@@ -2,7 +2,7 @@
 // the tokens of a step).
 //
 // What bounds it: the chain slots -> rows -> maximum -> entries, of which the SM has to hold many at once: 18000 tokens of 8 heads of 128
-// (111 MB) take 24 us, 4.6 TB/s, with eight blocks of 64 registers on an SM; 29 with six of 80, 30 with ten of 48 that spill, 31 with twice
+// (111 MB) take 24 to 25 us, 4.4 to 4.6 TB/s, with eight blocks of 64 registers on an SM; 29 with six of 80, 30 with ten of 48 that spill, 31 with twice
 // the warps for a run, 97 with keys and values in blocks of their own and runs held whole (168 registers).
 //
 // A run is a stretch of tokens whose slots follow one another inside a page; its scale needs the largest magnitude of all its

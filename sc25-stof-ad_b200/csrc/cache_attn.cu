@@ -16,10 +16,11 @@
 // pieces of about the same length everywhere, a piece a block, whatever the lengths of the requests (which only the device knows).
 // What one block covers is written at once, the rest in parts that cache_attn_join_kernel adds in the order of the blocks.
 //
-// Measured (int8 or e4m3 alike, pages of 16 to 128 alike): 96 requests of up to 16000 tokens, 32 heads on 8 of 128 (1.78 GB), 297 us = 6.0 TB/s,
-// bound by memory; 48 of up to 8000, 32 heads on 8 of 64 (0.22 GB), 76 us = 2.9 TB/s, bound by the instructions of a key, of which a row of 64
-// has almost as many as one of 128 for half the bytes (issue slots 60 % taken); one request of 4000 tokens 9.5 us, where the chain launch -
-// lengths - pages' numbers - entries - parts - joining launch is all there is.
+// Measured (int8 or e4m3 alike, pages of 16 to 128 alike): 96 requests of up to 16000 tokens, 32 heads on 8 of 128 (1.82 GB), 301 us = 6.0 TB/s,
+// bound by memory (with a cap, in a run of seconds, 321 to 338 us = 5.2 to 5.5 TB/s, by the box); 48 of up to 8000, 32 heads on 8 of 64
+// (0.22 GB), 64 us = 3.4 TB/s, bound by the instructions of a key, of which a row of 64 has almost as many as one of 128 for half the bytes
+// (issue slots 61 % taken), 89 us with a distance table; one request of 4000 tokens 10.2 us, where the chain launch - lengths - pages' numbers -
+// entries - parts - joining launch is all there is.  References of V for each row cost 0 to 6 % of that (one for all rows: 300, 63, 84, 9.9 us).
 #include "cache_common.cuh"
 #include "stof_host.h"
 #include "stof_ptx.cuh"
@@ -35,7 +36,7 @@ constexpr int CT_STEP = 16 * CT_TILES, CT_UNIT = CT_STEP * CT_WARPS;     // keys
 constexpr int CT_STAGES = 2;                 // of a warp's ring: one step on its way while one is used (three: the same times, and less on an SM)
 constexpr unsigned CT_LONG = 16, CT_WAVES = 4;                           // see piece_units
 // Blocks on an SM: as many as registers (and for D = 128 shared memory) hold without spills.  D = 64, 16 requests of 12 heads: 22.0 us with
-// four, 25.7 with three, 22.0 to 22.8 with five and six that spill a little (before slopes had a path without tests: 19.0 now).
+// four, 25.7 with three, 22.0 to 22.8 with five and six that spill a little (before slopes had a path without tests: 19.9 now).
 constexpr int ct_blocks(int nt, int dim) { return nt == 2 ? 2 : dim == 64 ? 4 : 3; }
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -73,7 +74,7 @@ __device__ __forceinline__ Span span_of(const CacheAttnParams& p, int b) {
 // How long the pieces are that the (request, K/V head, row group)s are cut into, in units, for `total` units in `pairs` of them: such that
 // there are about as many pieces as blocks that the GPU holds at once (a piece too many would wait for a whole round: every pair rounds
 // up, by half a piece on average), or more of CT_LONG units where there is work for more, up to CT_WAVES times as many, so that blocks that
-// get on faster take over from the others towards the end (96 requests of up to 16000 tokens: 297 us; once as many 355, twice 312, eight
+// get on faster take over from the others towards the end (96 requests of up to 16000 tokens, when this was chosen: 297 us; once as many 355, twice 312, eight
 // times 302; pieces of 8 or 32 units at least make no difference).
 __device__ __forceinline__ unsigned piece_units(unsigned total, unsigned pairs, unsigned resident) {
     const unsigned at_once = pairs < resident ? resident - pairs / 2 : resident;

@@ -8,8 +8,8 @@
 // longer (a prompt, a request that leaves) is done by warps.  The slots of many tokens are written by a second kernel over the whole
 // GPU, which looks its requests up in the running counts.
 //
-// Measured: 256 requests that take a token each or leave 6.2 us (with 256 threads 9.7: a request that leaves is a warp's work, and waits
-// for one), 1000 that come, go and take prompts of hundreds of tokens 11.4 us; the launches and the
+// Measured: 256 requests that take a token each or leave 6.2 to 6.4 us (with 256 threads 9.7: a request that leaves is a warp's work, and waits
+// for one), 1000 that come, go and take prompts of hundreds of tokens 11.4 to 11.8 us; the launches and the
 // chain lengths - sums - stack - table are all of it (a block scans 1000 requests in about 2 us; with sums by atomics of 64 bits in shared
 // memory, or loads behind stores that they cannot pass, the second took 32 us).
 #include "stof_host.h"

@@ -13,11 +13,12 @@
 // A tile is classified per warp (32 rows): nothing to mask, or masked by 128 bits a row.
 // What a call does not use is not in its kernel's loop (WHAT): the loop a warp spends its time in has to fit the instruction caches.
 //
-// What bounds it: long sequences the softmax warps.  A tile of 2 x 128 rows costs the tensor core 1024 cycles (D = 128) and the
-// exponentials 2048 (16 a cycle on an SM); with the loads from tensor memory, the maxima and the packing a warp comes to
-// about 3300 between two tiles of its own: 8192 x 8192, 32 heads on 8 of 128: 856 us = 1284 TFLOP/s, causal 457 (bf16 442), causal with cap
-// 530; heads of 64, where the exponentials stand against half the products: 729 us = 755 TFLOP/s, causal 374, with slopes 526, dense with a
-// table 839.  Short ones a block's beginning and end (the chain
+// What bounds it: long sequences the hand-overs between tensor core and softmax warps.  A tile of 2 x 128 rows costs the tensor core 2048
+// cycles (D = 128: 16.8 MFLOP at 8192 a cycle; heads of 64 half of that) and the exponentials 2048 too (16 a cycle on an SM), side by side;
+// with the loads from tensor memory, the maxima and the packing a warp comes to about 3300 between two tiles of its own: 8192 x 8192, 32
+// heads on 8 of 128: 860 us = 1278 TFLOP/s, causal 462 (bf16 447), causal with cap 529 to 540; heads of 64, which the exponentials bound:
+// 729 us = 754 TFLOP/s, causal 379, with slopes 525, dense with a table 840 (all of them 1 to 3 % more in long runs; the cap with a prefix
+// in a run of seconds 608, at the power cap).  Short ones a block's beginning and end (the chain
 // launch - Q, K - S - softmax - O - store, 4 to 6 us, half of it hidden by the other block on the SM).  Measured and slower: a persistent grid
 // (1.8 us less per block, more per tile: 4 x 12 x 1120 with documents 35 us against 29, 2 x 32 x 2048 queries with a window 145 against
 // 138); part of the exponentials as polynomials (plain 3 % faster, with a cap slower, and a NaN is lost); eight chains of maxima;

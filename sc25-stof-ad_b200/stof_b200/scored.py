@@ -14,6 +14,8 @@ def scored_attention(q, k, v, *, causal: bool = False, window=None, softcap=None
 
     Scores, in this order: x = softmax_scale * q.k (default 1 / sqrt(D)); `softcap`: x = softcap * tanh(x / softcap); `slopes` (H) float32:
     x -= slopes[h] * |position - j|; `distance_bias` (H, 2R + 1) float32, R at most 2048: x += distance_bias[h, R + clamp(j - position, -R, R)].
+    The capped score is off by up to 7e-6 of itself.  Minus infinity in the table takes keys out; a finite low value leaves them visible, and
+    a query that sees nothing else averages over them.
 
     Key j is visible where j < key_lens[b], documents[b, j] == documents[b, position], and either j < prefix_lens[b] or (not causal or
     j <= position) and (no window or |position - j| < window).  `key_lens`, `prefix_lens` (B) and `documents` (B, Sk; Sq <= Sk) are int32;
@@ -33,8 +35,11 @@ def cache_attention(q, k_pages, v_pages, k_scales, v_scales, block_table, length
     stands for entry * scale.  Key j of request b lies in page block_table[b, j // page_size] (int32), row j % page_size.  Token t sits
     at position lengths[b] - n + t (`lengths` int32, the new tokens included) and sees what is not behind it and, with `window`, less
     than `window` away.  `softcap`, `slopes`, `distance_bias` and `softmax_scale` as for `scored_attention`.  Requests of length 0, and tokens at
-    negative positions, give zeros.  A page number outside the cache is reported through the status word and its keys are left out; the
-    table may hold anything behind a request's length and for pages that the window hides from all of its tokens."""
+    negative positions, give zeros.  A page number outside the cache is reported through the status word, its keys are left out and the result
+    is not to be used; the table may hold anything behind a request's length and for pages that the window hides from all of its tokens.
+
+    The weights are rounded to 16 bits relative to the largest that has entered a sum, whatever the pages' scales.  A NaN or an infinity in
+    a value that one of a request's tokens sees reaches its other tokens too; one in a page's scale those that see the page."""
     return (_lib._native or _lib.native()).cache_attention(q, k_pages, v_pages, k_scales, v_scales, block_table, lengths, out, window, softcap, slopes,
                                                            distance_bias, softmax_scale)
 
