@@ -350,3 +350,22 @@ def test_values_in_front_of_the_window_take_no_part(dim, tokens, window):
     got = stof_b200.cache_attention(q, kp, vp, ks, vs, table, n, window=window)
     _status()
     assert torch.equal(got, want)
+
+
+def test_a_captured_call_follows_lengths_and_scales():
+    """Captured over requests of five tokens, replayed over thousands: pieces, steps and references are found at every replay."""
+    import stof_b200
+    kp, vp, ks, vs, table, n = _cache([4000] * 12, 8, 32, 64, torch.int8, 39)
+    q = _q(12, 1, 8, 64, torch.bfloat16, 40)
+    n.fill_(5)
+    stof_b200.cache_attention(q, kp, vp, ks, vs, table, n, window=3000)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = stof_b200.cache_attention(q, kp, vp, ks, vs, table, n, window=3000)
+    g = torch.Generator(device="cuda").manual_seed(41)
+    for _ in range(3):
+        n.copy_(torch.randint(0, 4001, (12,), generator=g, device="cuda").int())
+        vs.copy_(torch.exp2(torch.randn(vs.shape, generator=g, device="cuda") * 8) / 64)
+        graph.replay()
+        assert torch.equal(out, _check(q, (kp, vp, ks, vs, table, n), window=3000))
